@@ -6,4 +6,4 @@ sm_100a kernels behind the C ABI in ``include/foundry_cuda.h``
 the reference's loader / forward-pass seam used by the tests and the
 benchmark.
 """
-__all__ = ["gguf", "ggufgen", "loader", "runtime", "build"]
+__all__ = ["gguf", "ggufgen", "loader", "runtime", "paged", "speculate", "build"]

@@ -25,6 +25,8 @@ FL_ARCH_LLAMA, FL_ARCH_MISTRAL, FL_ARCH_GEMMA2, FL_ARCH_QWEN2 = 0, 1, 2, 3
 
 FL_PROF_MATVEC, FL_PROF_ATTN, FL_PROF_OTHER, FL_PROF_STEP, FL_PROF_N = 0, 1, 2, 3, 4
 
+FL_KV_F32, FL_KV_F16, FL_KV_Q8, FL_KV_F8 = 0, 1, 2, 3
+
 FL_TOPK_DEVICE_MAX_N = 262144
 FL_TP_HANDLE_BYTES = 64
 FL_TP_ALL = -1  # fl_model_desc.tp_rank of a group driven from one thread
@@ -85,6 +87,77 @@ class FlSamplerDesc(C.Structure):
     ]
 
 
+class FlPagedKv(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("kv_dtype", C.c_int32),
+        ("n_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("n_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+    ]
+
+
+class FlPagedBatch(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("n_seqs", C.c_int32),
+        ("table_cols", C.c_int32),
+        ("max_rows", C.c_int32),
+        ("page_table", C.c_void_p),
+        ("seq_len", C.c_void_p),
+        ("row_start", C.c_void_p),
+    ]
+
+
+class FlPagedAttnDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("type", C.c_int32),
+        ("n_rows", C.c_int32),
+        ("n_heads", C.c_int32),
+        ("window", C.c_int32),
+        ("scale", C.c_float),
+        ("softcap", C.c_float),
+        ("reserved", C.c_int32),
+        ("q", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("out", C.c_void_p),
+        ("out_stride", C.c_int64),
+        ("lse", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class FlVerifyDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("type", C.c_int32),
+        ("n_rows", C.c_int32),
+        ("n_seqs", C.c_int32),
+        ("vocab", C.c_int32),
+        ("reserved", C.c_int32),
+        ("logits", C.c_void_p),
+        ("logits_stride", C.c_int64),
+        ("draft_probs", C.c_void_p),
+        ("probs_stride", C.c_int64),
+        ("row_start", C.c_void_p),
+        ("draft", C.c_void_p),
+        ("temperature", C.c_void_p),
+        ("u_accept", C.c_void_p),
+        ("u_sample", C.c_void_p),
+        ("tokens", C.c_void_p),
+        ("accepted", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+    ]
+
+
 # Every entry point declared in include/foundry_cuda.h: (name, restype, argtypes)
 PUBLIC_API = [
     ("fl_last_error", C.c_char_p, []),
@@ -104,6 +177,16 @@ PUBLIC_API = [
                                    C.c_void_p]),
     ("fl_topk", C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
     ("fl_topk_device", C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("fl_kv_append_device", C.c_int, [C.POINTER(FlPagedKv), C.POINTER(FlPagedBatch), C.c_int32, C.c_int32, C.c_void_p,
+                                      C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    ("fl_kv_gather_device", C.c_int, [C.POINTER(FlPagedKv), C.POINTER(FlPagedBatch), C.c_int32, C.c_int32, C.c_void_p,
+                                      C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    ("fl_attn_paged_workspace", C.c_int, [C.POINTER(FlPagedKv), C.POINTER(FlPagedBatch), C.c_int32, C.c_int32,
+                                          C.POINTER(C.c_uint64)]),
+    ("fl_attn_paged_device", C.c_int, [C.POINTER(FlPagedKv), C.POINTER(FlPagedBatch), C.POINTER(FlPagedAttnDesc),
+                                       C.c_void_p]),
+    ("fl_verify_workspace", C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
+    ("fl_verify_device", C.c_int, [C.POINTER(FlVerifyDesc), C.c_void_p]),
     ("fl_sample", C.c_int, [C.c_void_p, C.POINTER(FlSamplerDesc), C.c_void_p, C.c_int32, C.c_float,
                             C.POINTER(C.c_int32)]),
     ("fl_session_tp_handle", C.c_int, [C.c_void_p, C.c_void_p]),

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "foundry_cuda.h" /* FL_KV_* */
+
 #define FL_MV_MAX_SEG 3
 #define FL_TP_MAX 8        /* ranks of one tensor-parallel group */
 #define FL_MV_WARPS 8
@@ -275,6 +277,47 @@ size_t fl_tc_gemm_smem_bytes(int bn);
 
 /* Bit-exact block dequantization (fl_dequant). */
 cudaError_t fl_launch_dequant(int32_t ggml_type, const uint8_t* src, int64_t n_blocks, float* dst, cudaStream_t st);
+
+/* ── operators on a paged KV cache (fl_kv_cache.cu, fl_paged_attn.cu) ─────
+ * The pool and the batch of fl_paged_kv / fl_paged_batch, checked. */
+struct FlPaged {
+    int32_t kv_dtype, n_pages, page_shift, n_kv, hd;
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int32_t n_seqs, cols, max_rows, n_rows;
+    const int32_t *table, *seq_len, *row_start;
+};
+cudaError_t fl_launch_kv_append(const FlPaged& c, int type, const void* k, int64_t k_stride, const void* v,
+                                int64_t v_stride, cudaStream_t st);
+cudaError_t fl_launch_kv_gather(const FlPaged& c, int type, void* k, int64_t k_stride, void* v, int64_t v_stride,
+                                cudaStream_t st);
+struct FlPagedAttn {
+    int32_t type, n_heads, window;
+    float scale, softcap;
+    const void* q;
+    int64_t q_stride;
+    void* out;
+    int64_t out_stride;
+    float* lse;
+    void* workspace;
+};
+size_t fl_paged_attn_workspace(const FlPaged& c, int n_heads);
+cudaError_t fl_launch_paged_attn(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
+
+/* Verification of drafted tokens (fl_verify.cu); fields as fl_verify_desc. */
+struct FlVerify {
+    int32_t type, n_rows, n_seqs, vocab;
+    const void* logits;
+    int64_t logits_stride;
+    const float* probs;
+    int64_t probs_stride;
+    const int32_t *row_start, *draft;
+    const float *temperature, *u_accept, *u_sample;
+    int32_t *tokens, *accepted;
+    void* workspace;
+};
+size_t fl_verify_workspace_bytes(int n_rows, int n_seqs, int vocab);
+cudaError_t fl_launch_verify(const FlVerify& v, cudaStream_t st);
 
 /* Top-k of a logits vector: k largest (value desc, index asc). */
 cudaError_t fl_launch_topk(const float* logits, int32_t n, int32_t k, int32_t* ids, float* vals, uint8_t* scratch,

@@ -1,0 +1,298 @@
+/*
+ * fl_kv_cache.cu — append to and gather from a paged KV cache
+ * (fl_kv_append_device, fl_kv_gather_device).
+ *
+ * Work: (row, kv head) pairs, K and V together.  A pair's head_dim elements
+ * are spread over head_dim / 8 lanes, eight each (one or two 16-byte loads),
+ * so that a row's maximum is a few shuffles and every access is a full
+ * sector; a warp holds 32 / (head_dim / 8) pairs.  Both directions are one
+ * pass: every element read once and written once.
+ */
+#include "fl_paged.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+/* q = x / s rounded to the nearest integer, ties to even, from the exact
+ * quotient: x * (1/s) is off by a few ulp at most, so the rounded candidate
+ * can only be wrong next to a border k + 1/2; the remainder x - q s is exact in
+ * one FMA (a multiple of the smaller ulp, at most about s/2), and comparing
+ * it with s/2 decides. */
+__device__ __forceinline__ int quant_q8(float x, float s, float inv)
+{
+    float q = rintf(x * inv);
+    const float r = fmaf(-q, s, x), h = 0.5f * s;
+    if (fabsf(r) >= h) {
+        const float up = r > 0.0f ? 1.0f : -1.0f;
+        if (fabsf(r) > h || ((int)q & 1)) q += up;
+    }
+    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+
+/* x / s as a float that rounds to e4m3 as the exact quotient does.  Borders
+ * between e4m3 values have at most 5 significant bits; where x * (1/s) comes
+ * within a few ulp of such a number t, the sign of x - t s (one FMA, exact in
+ * sign) tells on which side the quotient lies, and t or its neighbour stands
+ * for it. */
+__device__ __forceinline__ float quot_f8(float x, float s, float inv)
+{
+    const float y = x * inv;
+    if (fabsf(y) < 2.4414062e-4f) return y; /* 2^-12: far below half the smallest value, 2^-10 */
+    const uint32_t b = __float_as_uint(y);
+    const uint32_t t = (b + (1u << 18)) & ~((1u << 19) - 1u); /* nearest with 4 fraction bits */
+    const int d = (int)(b - t);
+    if (d > 8 || d < -8) return y;
+    const float tf = __uint_as_float(t);
+    const float r = fmaf(-tf, s, x);
+    if (r == 0.0f) return tf;
+    return __uint_as_float((r > 0.0f) == (tf > 0.0f) ? t + 1u : t - 1u);
+}
+
+template <int KV>
+struct Packed8 { /* eight elements in the cache */
+    uint2 w;
+};
+template <>
+struct Packed8<FL_KV_F16> {
+    uint4 w;
+};
+
+/* Eight elements of a row and the row's scale; `lanes` consecutive lanes hold the row. */
+template <int KV, int LANES>
+__device__ __forceinline__ Packed8<KV> quantize8(const float (&x)[8], float& scale)
+{
+    Packed8<KV> out;
+    if constexpr (KV == FL_KV_F16) {
+        __half2* h = reinterpret_cast<__half2*>(&out.w);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float v[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float f = x[2 * i + j];
+                v[j] = fabsf(f) > 65504.0f ? copysignf(65504.0f, f) : f; /* NaN stays */
+            }
+            h[i] = __floats2half2_rn(v[0], v[1]);
+        }
+    } else {
+        /* the maximum magnitude by integer compares: NaN above infinity above every number */
+        uint32_t a = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) a = max(a, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const bool finite = a < 0x7f800000u;
+        constexpr float top = KV == FL_KV_Q8 ? 127.0f : 448.0f;
+        const float s = finite ? __fdiv_rn(__uint_as_float(a), top) : __uint_as_float(0x7fffffffu);
+        scale = s;
+        uint32_t w[2] = {0, 0};
+        if (s > 0.0f) { /* false for NaN */
+            /* a scale below 2^-100 is scaled up with its row, so that its reciprocal is finite */
+            const float up = s < 7.8886091e-31f ? 1.2676506e30f : 1.0f; /* 2^100 */
+            const float su = s * up, inv = __fdiv_rn(1.0f, su);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                uint32_t p;
+                if constexpr (KV == FL_KV_Q8) {
+                    const int q0 = quant_q8(x[i] * up, su, inv), q1 = quant_q8(x[i + 1] * up, su, inv);
+                    p = ((uint32_t)q0 & 0xffu) | (((uint32_t)q1 & 0xffu) << 8);
+                } else {
+                    const float2 f = make_float2(quot_f8(x[i] * up, su, inv), quot_f8(x[i + 1] * up, su, inv));
+                    p = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+                }
+                w[i >> 2] |= p << (8 * (i & 2));
+            }
+        }
+        out.w = make_uint2(w[0], w[1]);
+    }
+    return out;
+}
+
+template <int KV>
+__device__ __forceinline__ void dequantize8(const Packed8<KV>& p, float s, float (&x)[8])
+{
+    if constexpr (KV == FL_KV_F16) {
+        const __half2* h = reinterpret_cast<const __half2*>(&p.w);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(h[i]);
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    } else {
+        const uint32_t w[2] = {p.w.x, p.w.y};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t b = (w[i >> 2] >> (8 * (i & 3))) & 0xffu;
+            float f;
+            if constexpr (KV == FL_KV_Q8) {
+                f = (float)(int8_t)b;
+            } else {
+                f = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+            }
+            x[i] = f * s;
+        }
+    }
+}
+
+template <int KV>
+__device__ __forceinline__ void store_cache(const FlPaged& c, bool v, int64_t at, int e, const Packed8<KV>& p, float s)
+{
+    constexpr int ES = KV == FL_KV_F16 ? 2 : 1;
+    uint8_t* base = static_cast<uint8_t*>(v ? c.v : c.k) + (at * c.hd + e) * ES;
+    if constexpr (KV == FL_KV_F16) {
+        *reinterpret_cast<uint4*>(base) = p.w;
+    } else {
+        *reinterpret_cast<uint2*>(base) = p.w;
+        if (e == 0) (v ? c.v_scale : c.k_scale)[at] = s;
+    }
+}
+
+template <typename T, int KV, int HD>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const FlPaged c, const T* __restrict__ k, int64_t k_stride,
+                                                             const T* __restrict__ v, int64_t v_stride)
+{
+    constexpr int LANES = HD / 8, PER_WARP = 32 / LANES;
+    const int lane = threadIdx.x & 31, e = (lane % LANES) * 8;
+    const int64_t warp = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
+    const int64_t pair0 = warp * PER_WARP, n_pairs = (int64_t)c.n_rows * c.n_kv;
+    if (pair0 >= n_pairs) return;
+    int64_t at[PER_WARP];
+    /* each pair's place; consecutive pairs are mostly heads of one row */
+    int prev = -1, s = -1;
+#pragma unroll
+    for (int i = 0; i < PER_WARP; i++) {
+        const int64_t pair = pair0 + i;
+        at[i] = -1;
+        if (pair < n_pairs) {
+            const int row = (int)(pair / c.n_kv), head = (int)(pair - (int64_t)row * c.n_kv);
+            if (row != prev) s = fl_row_seq(c.row_start, c.n_seqs, row);
+            prev = row;
+            if (s >= 0) at[i] = fl_cache_row(c, s, __ldg(c.seq_len + s) - (__ldg(c.row_start + s + 1) - row), head);
+        }
+    }
+    const int mine = lane / LANES;
+    int64_t my_at = -1;
+#pragma unroll
+    for (int i = 0; i < PER_WARP; i++)
+        if (i == mine) my_at = at[i];
+    const int64_t pair = pair0 + mine;
+    const int row = (int)(pair / c.n_kv), head = (int)(pair - (int64_t)row * c.n_kv);
+    float xk[8] = {}, xv[8] = {};
+    if (my_at >= 0) {
+        fl_load8(k + row * k_stride + head * HD + e, xk);
+        fl_load8(v + row * v_stride + head * HD + e, xv);
+    }
+    float sk = 0.0f, sv = 0.0f;
+    const Packed8<KV> pk = quantize8<KV, LANES>(xk, sk), pv = quantize8<KV, LANES>(xv, sv);
+    if (my_at >= 0) {
+        store_cache<KV>(c, false, my_at, e, pk, sk);
+        store_cache<KV>(c, true, my_at, e, pv, sv);
+    }
+}
+
+template <typename T, int KV, int HD>
+__global__ void __launch_bounds__(kThreads) kv_gather_kernel(const FlPaged c, T* __restrict__ k, int64_t k_stride,
+                                                             T* __restrict__ v, int64_t v_stride)
+{
+    constexpr int LANES = HD / 8, PER_WARP = 32 / LANES, ES = KV == FL_KV_F16 ? 2 : 1;
+    const int lane = threadIdx.x & 31, e = (lane % LANES) * 8;
+    const int64_t warp = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
+    const int64_t pair0 = warp * PER_WARP, n_pairs = (int64_t)c.n_rows * c.n_kv;
+    if (pair0 >= n_pairs) return;
+    const int mine = lane / LANES;
+    int prev = -1, s = -1, my_s = -1;
+#pragma unroll
+    for (int i = 0; i < PER_WARP; i++) {
+        const int64_t pair = pair0 + i;
+        if (pair < n_pairs) {
+            const int row = (int)(pair / c.n_kv);
+            if (row != prev) s = fl_row_seq(c.row_start, c.n_seqs, row);
+            prev = row;
+            if (i == mine) my_s = s;
+        }
+    }
+    if (my_s < 0) return;
+    const int64_t pair = pair0 + mine;
+    const int row = (int)(pair / c.n_kv), head = (int)(pair - (int64_t)row * c.n_kv);
+    const int64_t at = fl_cache_row(c, my_s, __ldg(c.seq_len + my_s) - (__ldg(c.row_start + my_s + 1) - row), head);
+    float xk[8] = {}, xv[8] = {};
+    if (at >= 0) {
+        Packed8<KV> pk, pv;
+        const uint8_t* kb = static_cast<const uint8_t*>(c.k) + (at * HD + e) * ES;
+        const uint8_t* vb = static_cast<const uint8_t*>(c.v) + (at * HD + e) * ES;
+        float sk = 1.0f, sv = 1.0f;
+        if constexpr (KV == FL_KV_F16) {
+            pk.w = *reinterpret_cast<const uint4*>(kb);
+            pv.w = *reinterpret_cast<const uint4*>(vb);
+        } else {
+            pk.w = *reinterpret_cast<const uint2*>(kb);
+            pv.w = *reinterpret_cast<const uint2*>(vb);
+            sk = c.k_scale[at];
+            sv = c.v_scale[at];
+        }
+        dequantize8<KV>(pk, sk, xk);
+        dequantize8<KV>(pv, sv, xv);
+    }
+    fl_store8(k + row * k_stride + head * HD + e, xk);
+    fl_store8(v + row * v_stride + head * HD + e, xv);
+}
+
+template <typename T, int KV, int HD>
+cudaError_t launch(bool append, const FlPaged& c, void* k, int64_t ks, void* v, int64_t vs, cudaStream_t st)
+{
+    const int64_t pairs = (int64_t)c.n_rows * c.n_kv, per_block = (int64_t)(kThreads / 32) * (256 / HD);
+    const unsigned grid = (unsigned)((pairs + per_block - 1) / per_block);
+    if (append)
+        kv_append_kernel<T, KV, HD><<<grid, kThreads, 0, st>>>(c, static_cast<const T*>(k), ks,
+                                                               static_cast<const T*>(v), vs);
+    else
+        kv_gather_kernel<T, KV, HD><<<grid, kThreads, 0, st>>>(c, static_cast<T*>(k), ks, static_cast<T*>(v), vs);
+    return cudaGetLastError();
+}
+
+template <typename T, int KV>
+cudaError_t launch_hd(bool append, const FlPaged& c, void* k, int64_t ks, void* v, int64_t vs, cudaStream_t st)
+{
+    switch (c.hd) {
+    case 64: return launch<T, KV, 64>(append, c, k, ks, v, vs, st);
+    case 128: return launch<T, KV, 128>(append, c, k, ks, v, vs, st);
+    case 256: return launch<T, KV, 256>(append, c, k, ks, v, vs, st);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+template <typename T>
+cudaError_t launch_kv(bool append, const FlPaged& c, void* k, int64_t ks, void* v, int64_t vs, cudaStream_t st)
+{
+    switch (c.kv_dtype) {
+    case FL_KV_F16: return launch_hd<T, FL_KV_F16>(append, c, k, ks, v, vs, st);
+    case FL_KV_Q8: return launch_hd<T, FL_KV_Q8>(append, c, k, ks, v, vs, st);
+    case FL_KV_F8: return launch_hd<T, FL_KV_F8>(append, c, k, ks, v, vs, st);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+cudaError_t launch_type(bool append, const FlPaged& c, int type, void* k, int64_t ks, void* v, int64_t vs, cudaStream_t st)
+{
+    switch (type) {
+    case 0: return launch_kv<float>(append, c, k, ks, v, vs, st);
+    case 1: return launch_kv<__half>(append, c, k, ks, v, vs, st);
+    case 30: return launch_kv<__nv_bfloat16>(append, c, k, ks, v, vs, st);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+} // namespace
+
+cudaError_t fl_launch_kv_append(const FlPaged& c, int type, const void* k, int64_t k_stride, const void* v,
+                                int64_t v_stride, cudaStream_t st)
+{
+    return launch_type(true, c, type, const_cast<void*>(k), k_stride, const_cast<void*>(v), v_stride, st);
+}
+
+cudaError_t fl_launch_kv_gather(const FlPaged& c, int type, void* k, int64_t k_stride, void* v, int64_t v_stride,
+                                cudaStream_t st)
+{
+    return launch_type(false, c, type, k, k_stride, v, v_stride, st);
+}

@@ -1540,6 +1540,209 @@ extern "C" int fl_topk_device(const float* logits, int32_t n, int32_t k, int32_t
     return FL_OK;
 }
 
+/* ── operators on a paged KV cache and on drafted tokens ────────────────── */
+
+static bool row_type_ok(int32_t type) { return type == 0 || type == 1 || type == 30; }
+
+static bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+
+/* The checks of fl_paged_kv and fl_paged_batch; the launch parameters in c. */
+static int check_paged(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t n_rows, FlPaged& c)
+{
+    if (!kv || !b) return fail(FL_ERR_ARG, "null argument");
+    if (kv->struct_size != (int32_t)sizeof(fl_paged_kv)) return fail(FL_ERR_ARG, "fl_paged_kv size mismatch");
+    if (b->struct_size != (int32_t)sizeof(fl_paged_batch)) return fail(FL_ERR_ARG, "fl_paged_batch size mismatch");
+    if (kv->kv_dtype != FL_KV_F16 && kv->kv_dtype != FL_KV_Q8 && kv->kv_dtype != FL_KV_F8)
+        return fail(FL_ERR_UNSUPPORTED, "paged kv dtype %d", kv->kv_dtype);
+    if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
+        return fail(FL_ERR_UNSUPPORTED, "head_dim %d (64, 128 and 256 are built)", kv->head_dim);
+    if (kv->page_size < 16 || kv->page_size > 1024 || (kv->page_size & (kv->page_size - 1)))
+        return fail(FL_ERR_ARG, "page_size %d is not a power of two in range [16, 1024]", kv->page_size);
+    if (kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->n_kv_heads > 1024)
+        return fail(FL_ERR_ARG, "n_pages %d or n_kv_heads %d out of range", kv->n_pages, kv->n_kv_heads);
+    if (b->n_seqs < 0 || b->table_cols < 0 || b->max_rows < 0 || n_rows < 0)
+        return fail(FL_ERR_ARG, "n_seqs, table_cols, max_rows and n_rows must be >= 0");
+    if ((int64_t)b->table_cols * kv->page_size > INT32_MAX)
+        return fail(FL_ERR_ARG, "%d pages of %d positions: positions are out of 32-bit range", b->table_cols, kv->page_size);
+    if (!kv->k || !kv->v) return fail(FL_ERR_ARG, "null cache pointer");
+    if (misaligned(kv->k, 16) || misaligned(kv->v, 16)) return fail(FL_ERR_ARG, "cache pointers must be 16-byte aligned");
+    if (kv->kv_dtype != FL_KV_F16 && (!kv->k_scale || !kv->v_scale))
+        return fail(FL_ERR_ARG, "an 8-bit cache needs k_scale and v_scale");
+    if (b->n_seqs > 0 && n_rows > 0 && (!b->seq_len || !b->row_start || (!b->page_table && b->table_cols > 0)))
+        return fail(FL_ERR_ARG, "null batch pointer");
+    c.kv_dtype = kv->kv_dtype;
+    c.n_pages = kv->n_pages;
+    c.page_shift = 0;
+    while ((1 << c.page_shift) < kv->page_size) c.page_shift++;
+    c.n_kv = kv->n_kv_heads;
+    c.hd = kv->head_dim;
+    c.k = kv->k;
+    c.v = kv->v;
+    c.k_scale = kv->k_scale;
+    c.v_scale = kv->v_scale;
+    c.n_seqs = b->n_seqs;
+    c.cols = b->table_cols;
+    c.n_rows = n_rows;
+    c.max_rows = b->max_rows > 0 ? std::min(b->max_rows, n_rows) : n_rows;
+    c.table = b->page_table;
+    c.seq_len = b->seq_len;
+    c.row_start = b->row_start;
+    return FL_OK;
+}
+
+/* A packed row array: [n_rows] rows of `width` elements, `stride` apart. */
+static int check_rows(const char* name, const void* p, int64_t stride, int64_t width, int32_t n_rows, int32_t type)
+{
+    const int es = type == 0 ? 4 : 2;
+    if (!p) return fail(FL_ERR_ARG, "null %s", name);
+    if (n_rows > 1 && stride < width)
+        return fail(FL_ERR_ARG, "%s rows %lld elements apart overlap (%lld elements each)", name, (long long)stride,
+                    (long long)width);
+    if (misaligned(p, 16) || (n_rows > 1 && (stride * es) % 16)) return fail(FL_ERR_ARG, "%s rows must be 16-byte aligned", name);
+    return FL_OK;
+}
+
+extern "C" int fl_kv_append_device(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t type, int32_t n_rows,
+                                   const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* stream)
+{
+    FlPaged c;
+    int rc = check_paged(kv, b, n_rows, c);
+    if (rc) return rc;
+    if (!row_type_ok(type)) return fail(FL_ERR_UNSUPPORTED, "row type %d (0 = F32, 1 = F16, 30 = BF16)", type);
+    if (n_rows == 0 || c.n_seqs == 0) return FL_OK;
+    if ((rc = check_rows("k", k, k_stride, (int64_t)c.n_kv * c.hd, n_rows, type))) return rc;
+    if ((rc = check_rows("v", v, v_stride, (int64_t)c.n_kv * c.hd, n_rows, type))) return rc;
+    CK(fl_launch_kv_append(c, type, k, k_stride, v, v_stride, static_cast<cudaStream_t>(stream)));
+    return FL_OK;
+}
+
+extern "C" int fl_kv_gather_device(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t type, int32_t n_rows, void* k,
+                                   int64_t k_stride, void* v, int64_t v_stride, void* stream)
+{
+    FlPaged c;
+    int rc = check_paged(kv, b, n_rows, c);
+    if (rc) return rc;
+    if (!row_type_ok(type)) return fail(FL_ERR_UNSUPPORTED, "row type %d (0 = F32, 1 = F16, 30 = BF16)", type);
+    if (n_rows == 0 || c.n_seqs == 0) return FL_OK;
+    if ((rc = check_rows("k", k, k_stride, (int64_t)c.n_kv * c.hd, n_rows, type))) return rc;
+    if ((rc = check_rows("v", v, v_stride, (int64_t)c.n_kv * c.hd, n_rows, type))) return rc;
+    CK(fl_launch_kv_gather(c, type, k, k_stride, v, v_stride, static_cast<cudaStream_t>(stream)));
+    return FL_OK;
+}
+
+static int check_heads(const FlPaged& c, int32_t n_heads)
+{
+    if (n_heads < 1 || n_heads > 8192 || n_heads % c.n_kv)
+        return fail(FL_ERR_ARG, "Invalid attention head configuration: %d query heads, %d kv heads", n_heads, c.n_kv);
+    if ((int64_t)c.n_rows * n_heads > INT32_MAX)
+        return fail(FL_ERR_ARG, "%d rows of %d heads are out of 32-bit range", c.n_rows, n_heads);
+    return FL_OK;
+}
+
+extern "C" int fl_attn_paged_workspace(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t n_rows, int32_t n_heads,
+                                       uint64_t* bytes)
+{
+    FlPaged c;
+    if (!bytes) return fail(FL_ERR_ARG, "null argument");
+    int rc = check_paged(kv, b, n_rows, c);
+    if (rc || (rc = check_heads(c, n_heads))) return rc;
+    *bytes = fl_paged_attn_workspace(c, n_heads);
+    return FL_OK;
+}
+
+extern "C" int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_paged_attn_desc* a,
+                                    void* stream)
+{
+    if (!a) return fail(FL_ERR_ARG, "null argument");
+    if (a->struct_size != (int32_t)sizeof(fl_paged_attn_desc)) return fail(FL_ERR_ARG, "fl_paged_attn_desc size mismatch");
+    FlPaged c;
+    int rc = check_paged(kv, b, a->n_rows, c);
+    if (rc || (rc = check_heads(c, a->n_heads))) return rc;
+    if (!row_type_ok(a->type)) return fail(FL_ERR_UNSUPPORTED, "row type %d (0 = F32, 1 = F16, 30 = BF16)", a->type);
+    if (!std::isfinite(a->scale) || !std::isfinite(a->softcap))
+        return fail(FL_ERR_ARG, "scale and softcap must be finite");
+    if (a->reserved) return fail(FL_ERR_ARG, "reserved must be 0");
+    if (a->n_rows == 0 || c.n_seqs == 0) return FL_OK;
+    const int64_t width = (int64_t)a->n_heads * c.hd;
+    if ((rc = check_rows("q", a->q, a->q_stride, width, a->n_rows, a->type))) return rc;
+    if ((rc = check_rows("out", a->out, a->out_stride, width, a->n_rows, a->type))) return rc;
+    const size_t need = fl_paged_attn_workspace(c, a->n_heads);
+    if (a->workspace_bytes < need || (need && !a->workspace) || misaligned(a->workspace, 256))
+        return fail(FL_ERR_ARG, "workspace: %llu bytes, 256-byte aligned, are needed (fl_attn_paged_workspace)",
+                    (unsigned long long)need);
+    FlPagedAttn p;
+    p.type = a->type;
+    p.n_heads = a->n_heads;
+    p.window = a->window;
+    p.scale = a->scale;
+    p.softcap = a->softcap;
+    p.q = a->q;
+    p.q_stride = a->q_stride;
+    p.out = a->out;
+    p.out_stride = a->out_stride;
+    p.lse = a->lse;
+    p.workspace = a->workspace;
+    CK(fl_launch_paged_attn(c, p, static_cast<cudaStream_t>(stream)));
+    return FL_OK;
+}
+
+static int check_verify_sizes(int32_t n_rows, int32_t n_seqs, int32_t vocab)
+{
+    if (n_rows < 0 || n_seqs < 0) return fail(FL_ERR_ARG, "n_rows and n_seqs must be >= 0");
+    if (vocab < 1 || vocab > (1 << 24)) return fail(FL_ERR_ARG, "vocab %d is outside [1, %d]", vocab, 1 << 24);
+    return FL_OK;
+}
+
+extern "C" int fl_verify_workspace(int32_t n_rows, int32_t n_seqs, int32_t vocab, uint64_t* bytes)
+{
+    if (!bytes) return fail(FL_ERR_ARG, "null argument");
+    const int rc = check_verify_sizes(n_rows, n_seqs, vocab);
+    if (rc) return rc;
+    *bytes = fl_verify_workspace_bytes(n_rows, n_seqs, vocab);
+    return FL_OK;
+}
+
+extern "C" int fl_verify_device(const fl_verify_desc* d, void* stream)
+{
+    if (!d) return fail(FL_ERR_ARG, "null argument");
+    if (d->struct_size != (int32_t)sizeof(fl_verify_desc)) return fail(FL_ERR_ARG, "fl_verify_desc size mismatch");
+    const int rc = check_verify_sizes(d->n_rows, d->n_seqs, d->vocab);
+    if (rc) return rc;
+    if (!row_type_ok(d->type)) return fail(FL_ERR_UNSUPPORTED, "logits type %d (0 = F32, 1 = F16, 30 = BF16)", d->type);
+    if (d->reserved) return fail(FL_ERR_ARG, "reserved must be 0");
+    if (d->n_seqs == 0) return FL_OK;
+    if (!d->row_start || !d->temperature || !d->u_sample || !d->accepted) return fail(FL_ERR_ARG, "null argument");
+    if (d->n_rows > 0) {
+        if (!d->logits || !d->draft || !d->u_accept || !d->tokens) return fail(FL_ERR_ARG, "null argument");
+        if (d->n_rows > 1 && (d->logits_stride < d->vocab || (d->draft_probs && d->probs_stride < d->vocab)))
+            return fail(FL_ERR_ARG, "rows of %d logits or probabilities overlap", d->vocab);
+        if (misaligned(d->logits, d->type == 0 ? 4 : 2)) return fail(FL_ERR_ARG, "logits must be aligned to their type");
+    }
+    const size_t need = fl_verify_workspace_bytes(d->n_rows, d->n_seqs, d->vocab);
+    if (d->workspace_bytes < need || (need && !d->workspace) || misaligned(d->workspace, 256))
+        return fail(FL_ERR_ARG, "workspace: %llu bytes, 256-byte aligned, are needed (fl_verify_workspace)",
+                    (unsigned long long)need);
+    FlVerify v;
+    v.type = d->type;
+    v.n_rows = d->n_rows;
+    v.n_seqs = d->n_seqs;
+    v.vocab = d->vocab;
+    v.logits = d->logits;
+    v.logits_stride = d->logits_stride;
+    v.probs = d->draft_probs;
+    v.probs_stride = d->probs_stride;
+    v.row_start = d->row_start;
+    v.draft = d->draft;
+    v.temperature = d->temperature;
+    v.u_accept = d->u_accept;
+    v.u_sample = d->u_sample;
+    v.tokens = d->tokens;
+    v.accepted = d->accepted;
+    v.workspace = d->workspace;
+    CK(fl_launch_verify(v, static_cast<cudaStream_t>(stream)));
+    return FL_OK;
+}
+
 /* ── the prompt path ────────────────────────────────────────────────────── */
 
 /* Y[n x N] (fp32, row-major, ld N) = alpha * X[n x K] · W[N x K]^T + beta * Y

@@ -258,6 +258,162 @@ void fl_session_destroy(fl_session* s);
 #define FL_TOPK_DEVICE_MAX_N 262144
 int fl_topk_device(const float* logits, int32_t n, int32_t k, int32_t* ids, float* vals, void* stream);
 
+/* ── operators on a paged KV cache, in caller-owned device memory ─────────
+ *
+ * No counterpart in the reference, whose KvCache.cs is one F32 array per
+ * sequence.  They serve engines that batch requests or decode speculatively:
+ * the keys and values of many sequences live in pages of one pool, in 16 or
+ * 8 bits, and a step handles several new rows (tokens) of each sequence.
+ * Like fl_topk_device they take DEVICE pointers of the current device, are
+ * enqueued on `stream` (a cudaStream_t; NULL = the legacy default stream)
+ * without synchronizing or allocating, may be captured into a graph, and read
+ * lengths and page tables on the device.  Contents that point nowhere (a page
+ * id outside [0, n_pages), a position outside the table) are skipped, never
+ * followed.  Descriptors are host structs, read before the call returns.
+ *
+ * Element types of rows and outputs are GGML type ids: 0 (F32), 1 (F16), 30
+ * (BF16).
+ *
+ * Cache formats, per (position, kv head) row x of K or V:
+ * - FL_KV_F16: x rounded to fp16, magnitudes above 65504 stored as 65504;
+ * - FL_KV_Q8: int8 q with one F32 scale s = max|x| / 127: q = x / s rounded
+ *   to nearest, ties to even (the quotient is not rounded before), stands for
+ *   q * s;
+ * - FL_KV_F8: e4m3 f with one F32 scale s = max|x| / 448: f = x / s rounded to
+ *   nearest even, stands for f * s.
+ * A row of zeros has s = 0.  In the 8-bit formats a row that holds a NaN or an
+ * infinity is stored with s = NaN and zero elements: it reads as NaN.
+ *
+ * Pool layout: k, v [n_pages][n_kv_heads][page_size][head_dim]; k_scale,
+ * v_scale [n_pages][n_kv_heads][page_size] (8-bit formats).  k and v are
+ * 16-byte aligned; page_size is a power of two in [16, 1024], head_dim 64,
+ * 128 or 256. */
+#define FL_KV_F16 1
+#define FL_KV_Q8 2
+#define FL_KV_F8 3
+typedef struct fl_paged_kv {
+    int32_t struct_size;      /* sizeof(fl_paged_kv) */
+    int32_t kv_dtype;         /* FL_KV_F16, FL_KV_Q8, FL_KV_F8 */
+    int32_t n_pages, page_size;
+    int32_t n_kv_heads, head_dim;
+    void *k, *v;
+    float *k_scale, *v_scale; /* NULL for FL_KV_F16 */
+} fl_paged_kv;
+
+/* The new rows of a step: rows row_start[b] .. row_start[b+1]-1 of the packed
+ * row arrays belong to sequence b and are the LAST positions of its seq_len[b]
+ * cached ones, in order (row i of n sits at position seq_len[b] - n + i).
+ * Position p of sequence b lives in page page_table[b][p / page_size] at
+ * offset p % page_size; an entry outside [0, n_pages) is an unmapped page.
+ * Sequences may have no rows; row arrays may hold more than
+ * row_start[n_seqs] rows, those behind are left alone.  Sequences may share
+ * pages that a call only reads. */
+typedef struct fl_paged_batch {
+    int32_t struct_size;      /* sizeof(fl_paged_batch) */
+    int32_t n_seqs;
+    int32_t table_cols;       /* entries of one sequence's page table */
+    int32_t max_rows;         /* the most rows a sequence has, or 0 = not known (affects speed only) */
+    const int32_t* page_table; /* [n_seqs][table_cols] */
+    const int32_t* seq_len;    /* [n_seqs], new rows included */
+    const int32_t* row_start;  /* [n_seqs + 1], not decreasing */
+} fl_paged_batch;
+
+/* Writes new rows into the cache.  k, v: [n_rows][n_kv_heads][head_dim] of
+ * `type`, consecutive rows k_stride / v_stride elements apart (heads and
+ * elements dense), 16-byte aligned rows.  Rows whose position is negative or
+ * unmapped are dropped.  A position is written by at most one row of a call. */
+int fl_kv_append_device(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t type, int32_t n_rows, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, void* stream);
+
+/* Reads rows back: the values the cache's elements stand for, rounded once
+ * to `type`.  Shapes and strides as in fl_kv_append_device; the batch's
+ * "new rows" are the rows to read (to read positions [p0, p1) of a sequence:
+ * p1 - p0 rows and seq_len p1).  Rows at unmapped positions read as zero. */
+int fl_kv_gather_device(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t type, int32_t n_rows, void* k,
+                        int64_t k_stride, void* v, int64_t v_stride, void* stream);
+
+/* Attention of the new rows over the cached ones (the rows' own K and V
+ * already appended): row at position p and query head h of kv head
+ * h / (n_heads / n_kv_heads) sees the mapped positions j with j <= p and, if
+ * window > 0, j > p - window;
+ *   x_j = scale * q . k_j, or softcap * tanh(scale * q . k_j / softcap) if
+ *   softcap > 0;  out = sum_j exp(x_j) v_j / sum_j exp(x_j);
+ *   lse = log sum_j exp(x_j).
+ * A row that sees nothing gets out = 0, lse = -infinity.  What a row does not
+ * see (NaN and infinities in masked places included) does not touch it.
+ * Scores, the softmax's maximum and sum, and the output are accumulated in
+ * F32; results do not depend on the other sequences' rows, and are the same
+ * each time for the same shapes.
+ * q, out: [n_rows][n_heads][head_dim] of `type`, rows q_stride / out_stride
+ * elements apart, 16-byte aligned; out may not overlap q.
+ * workspace: fl_attn_paged_workspace bytes, 256-byte aligned, used during the
+ * call only; its contents do not matter before and after.  Calls that may run
+ * at the same time (other streams, graphs) need workspaces of their own. */
+typedef struct fl_paged_attn_desc {
+    int32_t struct_size;      /* sizeof(fl_paged_attn_desc) */
+    int32_t type;             /* of q and out */
+    int32_t n_rows, n_heads;
+    int32_t window;           /* <= 0: none */
+    float scale, softcap;     /* softcap <= 0: none */
+    int32_t reserved;         /* 0 */
+    const void* q;
+    int64_t q_stride;
+    void* out;
+    int64_t out_stride;
+    float* lse;               /* [n_rows][n_heads], or NULL */
+    void* workspace;
+    uint64_t workspace_bytes;
+} fl_paged_attn_desc;
+int fl_attn_paged_workspace(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t n_rows, int32_t n_heads,
+                            uint64_t* bytes);
+int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_paged_attn_desc* a, void* stream);
+
+/* Verification of drafted tokens (speculative decoding) against the target
+ * model's logits; the draws are the caller's, as in fl_sample.  Sequence b
+ * has rows row_start[b] .. row_start[b+1]-1: row i < last holds the target's
+ * logits for the place of draft[row i], the last row those of the place after
+ * the drafts (its draft entry is ignored).  With p = softmax(logits / T) and q
+ * the distribution draft[row] was drawn from (draft_probs, or certainty of
+ * draft[row] when NULL), rows are taken in order: row i is accepted iff
+ * u_accept[row] * q(draft) < p(draft).  At the first row that is not, the
+ * token is drawn from max(p - q, 0) (from p if that is 0 everywhere); with all
+ * accepted, from p of the last row.  The draw is the first x whose cumulative
+ * weight exceeds u_sample[b] times the total; sums are in 64 bits.
+ * temperature[b] <= 0 is greedy: accepted iff draft is the argmax (first
+ * maximum), the token is the argmax.
+ * tokens[row]: the accepted drafts, then the token, then -1; accepted[b]: how
+ * many drafts were accepted.  Entries of rows behind the last sequence are
+ * left alone; accepted is 0 for a sequence without rows.
+ * A logit of NaN counts as -infinity (masked), +infinity as the largest F32;
+ * NaN and negative draft probabilities count as 0.  A row with everything
+ * masked accepts nothing and its token is -1; so is a draft outside
+ * [0, vocab) accepted never.
+ * logits: [n_rows][vocab] of `type` (GGML type id 0, 1 or 30), rows
+ * logits_stride elements apart; draft_probs: F32, rows probs_stride apart;
+ * elements dense.  workspace: fl_verify_workspace bytes, 256-byte aligned,
+ * as in fl_attn_paged_device. */
+typedef struct fl_verify_desc {
+    int32_t struct_size;      /* sizeof(fl_verify_desc) */
+    int32_t type;
+    int32_t n_rows, n_seqs, vocab;
+    int32_t reserved;         /* 0 */
+    const void* logits;
+    int64_t logits_stride;
+    const float* draft_probs; /* or NULL */
+    int64_t probs_stride;
+    const int32_t* row_start; /* [n_seqs + 1], not decreasing */
+    const int32_t* draft;     /* [n_rows] */
+    const float* temperature; /* [n_seqs] */
+    const float* u_accept;    /* [n_rows], in [0, 1) */
+    const float* u_sample;    /* [n_seqs], in [0, 1) */
+    int32_t* tokens;          /* [n_rows] */
+    int32_t* accepted;        /* [n_seqs] */
+    void* workspace;
+    uint64_t workspace_bytes;
+} fl_verify_desc;
+int fl_verify_workspace(int32_t n_rows, int32_t n_seqs, int32_t vocab, uint64_t* bytes);
+int fl_verify_device(const fl_verify_desc* d, void* stream);
+
 /* Dequantizer.Dequantize (Dequantizer.cs:488-504) on the device, bit-exact:
  * src is host memory with whole blocks, dst receives the F32 values.
  * Returns FL_ERR_ARG for a length that is not a multiple of the block size or a
