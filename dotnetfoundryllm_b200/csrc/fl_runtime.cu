@@ -1568,6 +1568,8 @@ static int check_paged(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t n
     if (misaligned(kv->k, 16) || misaligned(kv->v, 16)) return fail(FL_ERR_ARG, "cache pointers must be 16-byte aligned");
     if (kv->kv_dtype != FL_KV_F16 && (!kv->k_scale || !kv->v_scale))
         return fail(FL_ERR_ARG, "an 8-bit cache needs k_scale and v_scale");
+    if (kv->kv_dtype != FL_KV_F16 && (misaligned(kv->k_scale, 16) || misaligned(kv->v_scale, 16)))
+        return fail(FL_ERR_ARG, "k_scale and v_scale must be 16-byte aligned");
     if (b->n_seqs > 0 && n_rows > 0 && (!b->seq_len || !b->row_start || (!b->page_table && b->table_cols > 0)))
         return fail(FL_ERR_ARG, "null batch pointer");
     c.kv_dtype = kv->kv_dtype;

@@ -285,7 +285,7 @@ int fl_topk_device(const float* logits, int32_t n, int32_t k, int32_t* ids, floa
  * infinity is stored with s = NaN and zero elements: it reads as NaN.
  *
  * Pool layout: k, v [n_pages][n_kv_heads][page_size][head_dim]; k_scale,
- * v_scale [n_pages][n_kv_heads][page_size] (8-bit formats).  k and v are
+ * v_scale [n_pages][n_kv_heads][page_size] (8-bit formats).  All are
  * 16-byte aligned; page_size is a power of two in [16, 1024], head_dim 64,
  * 128 or 256. */
 #define FL_KV_F16 1
@@ -342,8 +342,9 @@ int fl_kv_gather_device(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t 
  * A row that sees nothing gets out = 0, lse = -infinity.  What a row does not
  * see (NaN and infinities in masked places included) does not touch it.
  * Scores, the softmax's maximum and sum, and the output are accumulated in
- * F32; results do not depend on the other sequences' rows, and are the same
- * each time for the same shapes.
+ * F32.  Results are the same each time for the same inputs; how a sequence's
+ * keys are split among the SMs, and with it the last bits of its rows, depends
+ * on the lengths in the batch.
  * q, out: [n_rows][n_heads][head_dim] of `type`, rows q_stride / out_stride
  * elements apart, 16-byte aligned; out may not overlap q.
  * workspace: fl_attn_paged_workspace bytes, 256-byte aligned, used during the
