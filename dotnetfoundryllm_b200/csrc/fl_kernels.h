@@ -292,8 +292,10 @@ cudaError_t fl_launch_kv_append(const FlPaged& c, int type, const void* k, int64
 cudaError_t fl_launch_kv_gather(const FlPaged& c, int type, void* k, int64_t k_stride, void* v, int64_t v_stride,
                                 cudaStream_t st);
 struct FlPagedAttn {
-    int32_t type, n_heads, window;
-    float scale, softcap;
+    int32_t type, n_heads, grp, window; /* grp: query heads of a kv head */
+    unsigned long long grp_inv;         /* floor(2^64 / grp) + 1; 0 for grp = 1 */
+    float score_unit;                   /* of q . k: scale * log2(e), or scale / softcap */
+    float softcap;
     const void* q;
     int64_t q_stride;
     void* out;
@@ -302,6 +304,10 @@ struct FlPagedAttn {
     void* workspace;
 };
 size_t fl_paged_attn_workspace(const FlPaged& c, int n_heads);
+bool fl_paged_attn_fits(const FlPaged& c, int n_heads); /* the schedule's units stay below 2^32 */
+cudaError_t fl_launch_paged_stream_hd64(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
+cudaError_t fl_launch_paged_stream_hd128(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
+cudaError_t fl_launch_paged_stream_hd256(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
 cudaError_t fl_launch_paged_attn(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
 
 /* Verification of drafted tokens (fl_verify.cu); fields as fl_verify_desc. */

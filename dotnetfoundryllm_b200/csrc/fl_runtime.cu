@@ -1638,6 +1638,9 @@ static int check_heads(const FlPaged& c, int32_t n_heads)
         return fail(FL_ERR_ARG, "Invalid attention head configuration: %d query heads, %d kv heads", n_heads, c.n_kv);
     if ((int64_t)c.n_rows * n_heads > INT32_MAX)
         return fail(FL_ERR_ARG, "%d rows of %d heads are out of 32-bit range", c.n_rows, n_heads);
+    if (!fl_paged_attn_fits(c, n_heads))
+        return fail(FL_ERR_UNSUPPORTED, "%d rows of %d heads over tables of %d pages: more work than one call schedules",
+                    c.n_rows, n_heads, c.cols);
     return FL_OK;
 }
 
@@ -1675,8 +1678,10 @@ extern "C" int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch*
     FlPagedAttn p;
     p.type = a->type;
     p.n_heads = a->n_heads;
+    p.grp = a->n_heads / c.n_kv;
+    p.grp_inv = p.grp > 1 ? ~0ull / (unsigned)p.grp + 1 : 0; /* exact: floor((2^64 - 1) / grp) + 1 >= 2^64 / grp */
     p.window = a->window;
-    p.scale = a->scale;
+    p.score_unit = a->softcap > 0.0f ? a->scale / a->softcap : a->scale * 1.44269504f;
     p.softcap = a->softcap;
     p.q = a->q;
     p.q_stride = a->q_stride;
