@@ -27,10 +27,11 @@ OBJ = PKG / "_build"
 CUDA_SOURCES = ["fl_matvec.cu", "fl_misc.cu", "fl_token.cu", "fl_token_hd64.cu", "fl_token_hd128.cu",
                 "fl_token_hd256.cu", "fl_prefill.cu", "fl_sample.cu", "fl_tc_gemm.cu", "fl_kv_cache.cu",
                 "fl_paged_hd64.cu", "fl_paged_hd128.cu", "fl_paged_hd256.cu",
+                "fl_paged_tc_hd64.cu", "fl_paged_tc_hd128.cu", "fl_paged_tc_hd256.cu",
                 "fl_paged_attn.cu", "fl_verify.cu", "fl_runtime.cu"]
 HOST_SOURCES = ["fl_repack.cpp"]
 HEADERS = ["fl_layout.h", "fl_decode.h", "fl_device.cuh", "fl_kernels.h", "fl_repack.h", "fl_mv_core.cuh", "fl_dequant.cuh",
-           "fl_token.cuh", "fl_paged.cuh", "fl_paged_stream.cuh"]
+           "fl_token.cuh", "fl_paged.cuh", "fl_paged_stream.cuh", "fl_paged_tc.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

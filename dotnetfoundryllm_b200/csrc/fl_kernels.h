@@ -284,7 +284,7 @@ struct FlPaged {
     int32_t kv_dtype, n_pages, page_shift, n_kv, hd;
     void *k, *v;
     float *k_scale, *v_scale;
-    int32_t n_seqs, cols, max_rows, n_rows;
+    int32_t n_seqs, cols, max_rows, n_rows; /* max_rows 0: not known */
     const int32_t *table, *seq_len, *row_start;
 };
 cudaError_t fl_launch_kv_append(const FlPaged& c, int type, const void* k, int64_t k_stride, const void* v,
@@ -308,6 +308,9 @@ bool fl_paged_attn_fits(const FlPaged& c, int n_heads); /* the schedule's units 
 cudaError_t fl_launch_paged_stream_hd64(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
 cudaError_t fl_launch_paged_stream_hd128(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
 cudaError_t fl_launch_paged_stream_hd256(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
+cudaError_t fl_launch_paged_tc_hd64(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
+cudaError_t fl_launch_paged_tc_hd128(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
+cudaError_t fl_launch_paged_tc_hd256(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
 cudaError_t fl_launch_paged_attn(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);
 
 /* Verification of drafted tokens (fl_verify.cu); fields as fl_verify_desc. */

@@ -53,7 +53,7 @@ constexpr int kMaxCtas = 148 * 4;
 struct SeqWork {
     int row0, n, first, len; /* packed rows, their count, the first one's position, keys that are mapped at most */
     int tile0, tiles, nrt;   /* first 16-key tile, tiles of an item (1 when there are no keys), row tiles */
-    uint32_t cost, units;    /* of an item, of the sequence */
+    uint32_t cost, units;    /* of an item, of the sequence: kItemCost + tiles, the tiles the last of them */
 };
 
 __device__ __forceinline__ SeqWork seq_work(const FlPaged& c, const FlPagedAttn& a, int s)
@@ -74,53 +74,6 @@ __device__ __forceinline__ SeqWork seq_work(const FlPaged& c, const FlPagedAttn&
     return w;
 }
 
-/* An item takes kItemCost + tiles units of the schedule, its tiles the last of
- * them; range c is units [c * per, (c + 1) * per).  All below 2^32, which the
- * host has checked on the largest possible total. */
-struct Schedule {
-    uint32_t total, per;
-};
-
-/* Workspace: the schedule, then the first unit of each sequence, then the
- * partials' (m, l) and outputs, two slots per CTA: [2c] for a range that
- * continues an item, [2c + 1] for one that starts it. */
-struct Workspace {
-    Schedule* sched;
-    uint32_t* seq_unit;
-    float2* ml;
-    float* o;
-};
-__host__ __device__ __forceinline__ size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
-__host__ __device__ __forceinline__ Workspace workspace(void* p, int n_seqs, int hd, size_t* bytes = nullptr)
-{
-    uint8_t* b = static_cast<uint8_t*>(p);
-    Workspace w;
-    size_t at = 256;
-    w.sched = reinterpret_cast<Schedule*>(b);
-    w.seq_unit = reinterpret_cast<uint32_t*>(b + at);
-    at += align256((size_t)n_seqs * 4);
-    w.ml = reinterpret_cast<float2*>(b + at);
-    at += align256((size_t)2 * kMaxCtas * kRows * 8);
-    w.o = reinterpret_cast<float*>(b + at);
-    at += (size_t)2 * kMaxCtas * kRows * hd * 4;
-    if (bytes) *bytes = at;
-    return w;
-}
-
-/* n / grp by the host's reciprocal floor(2^64 / grp) + 1 (0 for grp = 1). */
-__device__ __forceinline__ int div_grp(const FlPagedAttn& a, int n)
-{
-    return a.grp_inv ? (int)__umul64hi((unsigned long long)(uint32_t)n, a.grp_inv) : n;
-}
-
-/* x * 2^e for any e that a float's exponent range may ask for, in two exact steps. */
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); } /* e in [-126, 127] */
-__device__ __forceinline__ float scale2(float x, int e)
-{
-    const int h = e >> 1;
-    return x * pow2(h) * pow2(e - h);
-}
-
 /* ── fragments ──────────────────────────────────────────────────────────── */
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1)
 {
@@ -129,54 +82,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t 
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) { return half2_bits(__floats2half2_rn(a, b)); }
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 /* All bits of the halves of h that are NaN or infinite. */
 __device__ __forceinline__ uint32_t odd_halves(uint32_t h)
 {
     return ((h & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((h & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
-}
-
-/* Bytes 0, 1 (and 2, 3) of w as two halves. */
-template <int KV>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi)
-{
-    if constexpr (KV == FL_KV_Q8) {
-        /* 0x6400 + u is the half 1024 + u; u = q + 128 */
-        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        lo = half2_bits(__hsub2(*reinterpret_cast<const __half2*>(&a), bias));
-        hi = half2_bits(__hsub2(*reinterpret_cast<const __half2*>(&b), bias));
-    } else {
-        const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-        const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-        lo = (uint32_t)a.x | ((uint32_t)a.y << 16);
-        hi = (uint32_t)b.x | ((uint32_t)b.y << 16);
-    }
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src)
-{
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait()
-{
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <int KV, int HD, bool SPLIT>
@@ -217,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
     __shared__ float s_fr[kRows];                  /* score units of a row's scaled q */
     __shared__ float2 s_ml[kWarps][kRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const Workspace ws = workspace(a.workspace, c.n_seqs, HD);
+    const FlAttnSpace ws = fl_attn_space(a.workspace, c.n_seqs, kMaxCtas, kRows, HD);
     fl_pdl_trigger(); /* the merge kernel may take its place; it waits for this grid's end */
 
     /* ── this CTA's range: a scan over the sequences' units ── */
@@ -234,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
     if (lane == 31) s_scan[warp] = before;
     if (tid == 0) s_seq = -1;
     __syncthreads();
-    Schedule sc;
+    FlSchedule sc;
     sc.total = 0;
     before -= mine;
 #pragma unroll
@@ -286,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
 
         /* ── q fragments ── */
         for (int r = warp; r < kRows; r += kWarps) {
-            const int f = f0 + r, i = div_grp(a, f);
+            const int f = f0 + r, i = fl_div_grp(a, f);
             float x[HD / 32];
             uint32_t top = 0;
             if (r < rows) {
@@ -300,9 +209,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                 top = __reduce_max_sync(0xffffffffu, top);
                 /* q 2^up has its largest magnitude in [2^14, 2^15) */
                 const int up = top < 0x7f800000u ? 14 + 127 - (int)(top >> 23) : 0;
-                if (lane == 0) s_fr[r] = scale2(a.score_unit, -up);
+                if (lane == 0) s_fr[r] = fl_scale2(a.score_unit, -up);
 #pragma unroll
-                for (int e = 0; e < HD / 32; e++) x[e] = scale2(x[e], up);
+                for (int e = 0; e < HD / 32; e++) x[e] = fl_scale2(x[e], up);
             } else {
 #pragma unroll
                 for (int e = 0; e < HD / 32; e++) x[e] = 0.0f;
@@ -358,19 +267,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                     for (int n = 0; n < 2; n++)
 #pragma unroll
                         for (int p = 0; p < C::KC; p++)
-                            cp_async16(dst + (n * C::KC + p) * 512 + lane * 16, kp + n * 2 * C::ROW + p * 64);
+                            fl_cp_async16(dst + (n * C::KC + p) * 512 + lane * 16, kp + n * 2 * C::ROW + p * 64);
 #pragma unroll
                     for (int n = 0; n < 4; n++)
 #pragma unroll
                         for (int p = 0; p < C::VC; p++) {
                             const uint32_t d = dst + C::KBYTES + (n * C::VC + p) * (32 * C::VP) + lane * C::VP;
                             if (C::VP == 16)
-                                cp_async16(d, vp + n * C::ROW + p * 128);
+                                fl_cp_async16(d, vp + n * C::ROW + p * 128);
                             else
-                                cp_async8(d, vp + n * C::ROW);
+                                fl_cp_async8(d, vp + n * C::ROW);
                         }
                     if (C::SCALES && lane < 8)
-                        cp_async16(dst + 2 * C::KBYTES + lane * 16, (lane < 4 ? c.k_scale : c.v_scale) + row + (lane & 3) * 4);
+                        fl_cp_async16(dst + 2 * C::KBYTES + lane * 16, (lane < 4 ? c.k_scale : c.v_scale) + row + (lane & 3) * 4);
                 } else if (U > 1) {
                     /* computed with its neighbour: zeros, which masked weights keep zero */
 #pragma unroll
@@ -379,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + b + lane * 16), "r"(0) : "memory");
                 }
             }
-            cp_async_commit();
+            fl_cp_async_commit();
         };
 #pragma unroll
         for (int i = 0; i < C::STAGES - 1; i++) fetch(i * U);
@@ -396,9 +305,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
         const float fr[2] = {s_fr[g], s_fr[g + 8]};
         int pos[2]; /* last key of rows g, g + 8; rows past the item's see nothing */
 #pragma unroll
-        for (int i = 0; i < 2; i++) pos[i] = g + 8 * i < rows ? sw.first + div_grp(a, f0 + g + 8 * i) : -1;
+        for (int i = 0; i < 2; i++) pos[i] = g + 8 * i < rows ? sw.first + fl_div_grp(a, f0 + g + 8 * i) : -1;
         /* the first and the last position of the item's rows */
-        const int pos_min = sw.first + div_grp(a, f0), pos_max = sw.first + div_grp(a, f0 + rows - 1);
+        const int pos_min = sw.first + fl_div_grp(a, f0), pos_max = sw.first + fl_div_grp(a, f0 + rows - 1);
         const int win = a.window > 0 ? a.window : INT_MAX;
 
         float acc[C::NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -417,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                 any |= mapped[u];
             }
             if (!any) continue;
-            cp_async_wait<C::STAGES - 1>();
+            fl_cp_async_wait<C::STAGES - 1>();
             __syncwarp(); /* scales and zeros are other lanes' */
             const uint8_t* st = ring_p + ((i / U) % C::STAGES) * C::STAGE;
             const int key0 = (tile_first + i * kWarps) * kTile; /* tile u starts at key0 + u * kWarps * kTile */
@@ -448,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                             if constexpr (KV == FL_KV_F16)
                                 b0 = w[u][n][2 * e], b1 = w[u][n][2 * e + 1];
                             else
-                                widen<KV>(w[u][n][e], b0, b1);
+                                fl_widen4<KV>(w[u][n][e], b0, b1);
                             if (SPLIT) mma_f16(s[u][n], lo, b0, b1);
                             mma_f16(s[u][n], hi, b0, b1);
                         }
@@ -513,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 if (mx > m[i2]) {
-                    alpha[i2] = ex2(m[i2] - mx); /* 0 the first time */
+                    alpha[i2] = fl_ex2(m[i2] - mx); /* 0 the first time */
                     m[i2] = mx;
                     moved = true;
                 }
@@ -532,11 +441,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                 top = __reduce_max_sync(0xffffffffu, top);
                 const int en = max((int)(top >> 23) - 127, -100);
                 if (en > ev) {
-                    down = ev == -1000 ? 0.0f : ex2((float)(ev - en));
+                    down = ev == -1000 ? 0.0f : fl_ex2((float)(ev - en));
                     ev = en;
                     moved = true;
                 }
-                up = pow2(14 - ev);
+                up = fl_pow2(14 - ev);
             }
             if (__any_sync(0xffffffffu, moved)) {
                 l[0] *= alpha[0];
@@ -566,16 +475,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                         float w[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const float x = s[u][n][2 * i2 + e], p = ex2(x - ref);
+                            const float x = s[u][n][2 * i2 + e], p = fl_ex2(x - ref);
                             l[i2] += p;
                             w[e] = p * f[2 * n + e];
                             if (masked && C::SCALES && x == -INFINITY) w[e] = 0.0f; /* whatever the scale */
                             if (masked && KV != FL_KV_Q8 && x != -INFINITY) se[n][i2] |= 0x3c00u << (16 * e);
                         }
-                        hi[n][i2] = pack_half2(w[0], w[1]);
+                        hi[n][i2] = fl_pack_half2(w[0], w[1]);
                         if (SPLIT) {
                             const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[n][i2]));
-                            lo[n][i2] = pack_half2(w[0] - h.x, w[1] - h.y);
+                            lo[n][i2] = fl_pack_half2(w[0] - h.x, w[1] - h.y);
                         }
                     }
                 }
@@ -608,10 +517,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                             b0[0] = __byte_perm(w[0][x], w[1][x], 0x5410), b0[1] = __byte_perm(w[0][x], w[1][x], 0x7632);
                             b1[0] = __byte_perm(w[2][x], w[3][x], 0x5410), b1[1] = __byte_perm(w[2][x], w[3][x], 0x7632);
                         } else {
-                            widen<KV>(__byte_perm(w[0][x], w[1][x], 0x5140), b0[0], b0[1]);
-                            widen<KV>(__byte_perm(w[0][x], w[1][x], 0x7362), b0[2], b0[3]);
-                            widen<KV>(__byte_perm(w[2][x], w[3][x], 0x5140), b1[0], b1[1]);
-                            widen<KV>(__byte_perm(w[2][x], w[3][x], 0x7362), b1[2], b1[3]);
+                            fl_widen4<KV>(__byte_perm(w[0][x], w[1][x], 0x5140), b0[0], b0[1]);
+                            fl_widen4<KV>(__byte_perm(w[0][x], w[1][x], 0x7362), b0[2], b0[3]);
+                            fl_widen4<KV>(__byte_perm(w[2][x], w[3][x], 0x5140), b1[0], b1[1]);
+                            fl_widen4<KV>(__byte_perm(w[2][x], w[3][x], 0x7362), b1[2], b1[3]);
                         }
 #pragma unroll
                         for (int e = 0; e < PER; e++) {
@@ -638,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
             }
             __syncwarp(); /* the stage's scales are read before another lane's copy may land there */
         }
-        cp_async_wait<0>();
+        fl_cp_async_wait<0>();
 
         /* ── the CTA's warps, merged in order ── */
 #pragma unroll
@@ -656,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
             float M = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_ml[w][r].x);
-            const float f = m[i] == -INFINITY ? 0.0f : scale2(ex2(m[i] - M), unit);
+            const float f = m[i] == -INFINITY ? 0.0f : fl_scale2(fl_ex2(m[i] - M), unit);
             float* dst = merge + (warp * kRows + r) * (HD + 4);
             constexpr int RUN = C::VP / C::ES; /* consecutive elements of a lane */
 #pragma unroll
@@ -680,13 +589,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
 #pragma unroll
             for (int w = 0; w < kWarps; w++) {
                 const float2 ml = s_ml[w][r];
-                L += ml.x == -INFINITY ? ml.y : ml.y * ex2(ml.x - M);
+                L += ml.x == -INFINITY ? ml.y : ml.y * fl_ex2(ml.x - M);
                 const float4* src = reinterpret_cast<const float4*>(merge + (w * kRows + r) * (HD + 4) + d);
                 const float4 u = src[0], v = src[1];
                 o[0] += u.x, o[1] += u.y, o[2] += u.z, o[3] += u.w, o[4] += v.x, o[5] += v.y, o[6] += v.z, o[7] += v.w;
             }
             if (whole) {
-                const int f = f0 + r, i = div_grp(a, f), h = head * a.grp + f - i * a.grp;
+                const int f = f0 + r, i = fl_div_grp(a, f), h = head * a.grp + f - i * a.grp;
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
                 for (int e = 0; e < 8; e++) o[e] *= inv;
@@ -702,66 +611,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
     }
 }
 
-/* Items that several ranges share: a warp per (row, head) adds the partials in
- * range order; a lane holds one partial's weight, and HD / 32 elements. */
+/* Items that several ranges share, a warp per (row, head). */
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const FlPaged c, const FlPagedAttn a)
 {
-    constexpr int E = HD / 32;
-    const int lane = threadIdx.x & 31;
     const int64_t pair = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
     if (pair >= (int64_t)c.n_rows * a.n_heads) return;
     const int row = (int)((uint32_t)pair / (uint32_t)a.n_heads), h = (int)(pair - (int64_t)row * a.n_heads);
     const int seq = fl_row_seq(c.row_start, c.n_seqs, row);
     if (seq < 0) return;
     const SeqWork sw = seq_work(c, a, seq);
-    const int head = div_grp(a, h), f = (row - sw.row0) * a.grp + h - head * a.grp;
-    const int item = head * sw.nrt + f / kRows, r = f % kRows;
-    const Workspace ws = workspace(a.workspace, c.n_seqs, HD);
+    const int head = fl_div_grp(a, h), f = (row - sw.row0) * a.grp + h - head * a.grp;
+    const int item = head * sw.nrt + f / kRows;
+    const FlAttnSpace ws = fl_attn_space(a.workspace, c.n_seqs, kMaxCtas, kRows, HD);
     fl_pdl_wait();
     const uint32_t per = ws.sched->per;
     const uint32_t t0 = ws.seq_unit[seq] + (uint32_t)item * sw.cost + kItemCost;
     const int c0 = (int)(t0 / per), c1 = (int)((t0 + sw.tiles - 1) / per);
-    if (c0 == c1) return; /* written by its range */
-    float M = -INFINITY, L = 0.0f, o[E] = {};
-    for (int base = c0; base <= c1; base += 32) {
-        const int i = base + lane, n = min(32, c1 - base + 1);
-        const float2 ml = i <= c1 ? ws.ml[(2 * i + (i == c0)) * kRows + r] : make_float2(-INFINITY, 0.0f);
-        float mx = ml.x;
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-        if (mx > M) {
-            const float f0 = ex2(M - mx); /* 0 the first time */
-            L *= f0;
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] *= f0;
-            M = mx;
-        }
-        const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-        L += fl_warp_sum(ml.x == -INFINITY ? ml.y : ml.y * w);
-#pragma unroll 4
-        for (int j = 0; j < n; j++) {
-            const int at = 2 * (base + j) + (base + j == c0);
-            const float wj = __shfl_sync(0xffffffffu, w, j);
-            const float* src = ws.o + ((size_t)at * kRows + r) * HD + lane * E;
-            if constexpr (E == 2) {
-                const float2 u = *reinterpret_cast<const float2*>(src);
-                o[0] = fmaf(u.x, wj, o[0]), o[1] = fmaf(u.y, wj, o[1]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e += 4) {
-                    const float4 u = *reinterpret_cast<const float4*>(src + e);
-                    o[e] = fmaf(u.x, wj, o[e]), o[e + 1] = fmaf(u.y, wj, o[e + 1]);
-                    o[e + 2] = fmaf(u.z, wj, o[e + 2]), o[e + 3] = fmaf(u.w, wj, o[e + 3]);
-                }
-            }
-        }
-    }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_stride + (int64_t)h * HD + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e++) out[e] = fl_from_float<T>(o[e] * inv);
-    if (a.lse && lane == 0) a.lse[pair] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.693147181f;
+    if (c0 != c1) fl_merge_row<T, HD>(a, ws, c0, c1, f % kRows, kRows, row, h); /* else written by its range */
 }
 
 template <typename T, int KV, int HD>

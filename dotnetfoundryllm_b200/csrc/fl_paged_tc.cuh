@@ -1,0 +1,999 @@
+/*
+ * fl_paged_tc.cuh — attention of new rows over a paged KV cache
+ * (fl_attn_paged_device) for many query rows per sequence, on the tcgen05
+ * tensor cores.  Included by one source file per head dimension.
+ *
+ * A CTA takes items (sequence, kv head, tile of NQ x 128 query rows, heads of a
+ * group folded into the rows) of BK-key tiles, in one contiguous range of the
+ * schedule that all items' tiles form, so every SM has the same number of
+ * tiles; an item cut by a range's end leaves (o, m, l) in the workspace for a
+ * second kernel.  Per key tile:
+ *  - 4 warps bring K and V from their pages to shared memory as fp16 in the
+ *    128-byte swizzled layout (8-bit elements are exact in fp16; scales stay
+ *    beside them).  V is read by the tensor core with the keys as its inner
+ *    dimension, straight from rows of 64 elements (an MN-major operand), so
+ *    nothing is transposed.
+ *  - one lane issues S = Q K^T into tensor memory and, once the weights are
+ *    there, O += P V with P read from tensor memory.
+ *  - 4 warps per 128 rows hold one row a thread: S is read from tensor memory
+ *    (no shuffles), weights go back as fp16 over the scores.
+ * Two sets of scores alternate (two row tiles, or two key tiles where the
+ * output takes the room of a second row tile), so the tensor core works on one
+ * while the other is exponentiated.  The maximum that weights refer to moves
+ * only when it grew by more than 2^8, which leaves O alone on almost every
+ * tile; weights then lie below 2^8 and are stored times 2^6, fp16's range.
+ *
+ * Sums and softmax state are fp32.  32-bit rows use two fp16 for q and for each
+ * weight (22 bits) at twice the products.
+ */
+#ifndef FL_PAGED_TC_CUH
+#define FL_PAGED_TC_CUH
+
+#include <climits>
+
+#include "fl_paged.cuh"
+
+namespace flpt {
+namespace {
+
+constexpr int kSoftWarps = 8, kLoadWarps = 4;
+constexpr int kThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr int kMaxCtas = 148;
+constexpr int kItemCost = 3; /* what starting an item costs, in key tiles */
+constexpr int kMinUnits = 2;
+constexpr float kLazy = 8.0f; /* log2 of how far weights may exceed 1 */
+constexpr int kUp = 6;        /* weights are stored times 2^kUp: below 2^15 with the values' scales below 2 */
+
+template <int KV, int HD, bool SPLIT>
+struct Cfg {
+    static constexpr int ES = KV == FL_KV_F16 ? 2 : 1;
+    static constexpr int ROW = HD * ES;
+    static constexpr int NQ = HD == 256 || (SPLIT && HD == 128) ? 1 : 2;
+    static constexpr int BK = HD == 256 ? 64 : 128;
+    static constexpr int RT = NQ * 128;                    /* query rows of an item */
+    static constexpr int STAGES = HD == 64 ? 3 : HD == 256 && SPLIT ? 1 : 2;
+    static constexpr int QTILE = 128 * HD * 2;             /* one row tile, one half of the split */
+    static constexpr int QBYTES = NQ * QTILE * (SPLIT ? 2 : 1);
+    static constexpr int TBYTES = BK * HD * 2;             /* K or V of a key tile */
+    static constexpr int PIECES = ROW / 16;                /* 16-byte pieces of a key */
+    static constexpr int NP = BK * PIECES / (kLoadWarps * 32); /* pieces of a thread */
+    static constexpr int INFO = BK * 8 + 64 + (KV == FL_KV_Q8 ? 0 : BK * (HD / 16) * 2);
+    static constexpr int SMEM = QBYTES + STAGES * (2 * TBYTES + INFO) + 1024 + 512;
+    /* tensor memory columns: two sets of scores (weights over them), the outputs, the weights' low halves */
+    static constexpr int S_COL = 0, O_COL = 2 * BK, LOW_COL = 384;
+    static_assert(O_COL + NQ * HD <= (SPLIT ? LOW_COL : 512) && SMEM <= 232448, "tensor and shared memory");
+};
+
+/* ── the schedule ───────────────────────────────────────────────────────── */
+struct SeqWork {
+    int row0, n, first, len, nrt;
+};
+struct ItemWork {
+    int f0, rows;            /* folded rows f0 .. f0 + rows - 1 */
+    int pos_min, pos_max;    /* positions of the first and the last */
+    int tile0, tiles;
+};
+template <int RT>
+__device__ __forceinline__ SeqWork seq_work(const FlPaged& c, const FlPagedAttn& a, int s)
+{
+    SeqWork w;
+    const int r0 = max(__ldg(c.row_start + s), 0), r1 = min(__ldg(c.row_start + s + 1), c.n_rows);
+    const int len = __ldg(c.seq_len + s);
+    w.row0 = r0;
+    w.n = max(r1 - r0, 0);
+    w.first = len - w.n;
+    w.len = max(0, min(len, c.cols << c.page_shift));
+    w.nrt = (w.n * a.grp + RT - 1) / RT;
+    return w;
+}
+
+template <int RT, int BK>
+__device__ __forceinline__ ItemWork item_work(const FlPagedAttn& a, const SeqWork& s, int rt)
+{
+    ItemWork w;
+    w.f0 = rt * RT;
+    w.rows = min(s.n * a.grp - w.f0, RT);
+    w.pos_min = s.first + fl_div_grp(a, w.f0);
+    w.pos_max = s.first + fl_div_grp(a, w.f0 + w.rows - 1);
+    const int lo = a.window > 0 ? max(0, w.pos_min + 1 - a.window) : 0, hi = max(0, min(s.len, w.pos_max + 1));
+    w.tile0 = lo / BK;
+    w.tiles = max(1, (hi + BK - 1) / BK - w.tile0);
+    return w;
+}
+
+/* Units of one kv head of a sequence's row tiles below `end`. */
+template <int RT, int BK>
+__device__ __forceinline__ uint32_t head_units(const FlPagedAttn& a, const SeqWork& s, int end)
+{
+    uint32_t u = 0;
+    for (int rt = 0; rt < end; rt++) u += kItemCost + item_work<RT, BK>(a, s, rt).tiles;
+    return u;
+}
+
+/* ── small helpers ──────────────────────────────────────────────────────── */
+/* One bit per half of w that is NaN or infinite. */
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w)
+{
+    return ((w & 0x7c00u) == 0x7c00u ? 1u : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 2u : 0u);
+}
+
+__device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+/* Descriptors of 128-byte swizzled tiles: rows of 128 bytes, groups of 8 rows
+ * 1024 bytes apart.  As a K-major operand (rows = M or N) the leading offset is
+ * unused; as an MN-major one (rows = K) it is the distance to the next 64
+ * elements of N. */
+__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t lbo)
+{
+    uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)((lbo >> 4) & 0x3fffu) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46; /* version */
+    d |= (uint64_t)2 << 61; /* 128-byte swizzle */
+    return d;
+}
+/* kind::f16, A and B fp16, D fp32, M = 128; bit 16: B is MN-major. */
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn)
+{
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(accum)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accum)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(accum)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(fl_smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+#define FL_R32(v) \
+    "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), \
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), \
+        "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), \
+        "r"(v[31])
+/* 32 consecutive columns of the thread's lane. */
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        FL_R32(v)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+/* Bounded wait (~2 s); false once it ran out or another role of the CTA gave up. */
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort)
+{
+    if (fl_mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = fl_globaltimer();
+    for (uint32_t it = 1;; it++) {
+        if (fl_mbar_try_wait(bar, parity)) return true;
+        if ((it & 1023u) == 0) {
+            if (*abort) return false;
+            if (fl_globaltimer() - t0 > 2000000000ull) {
+                *abort = 1;
+                return false;
+            }
+        }
+    }
+}
+
+/* The same for a whole warp, which stays together. */
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort)
+{
+    return __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
+}
+
+/* Where a range stands: iterates the segments (items cut to the range) in the
+ * same way in every role. */
+template <int RT, int BK>
+struct Segments {
+    uint32_t at, end, seq_at, head_u;
+    int seq;
+    SeqWork sw;
+    /* of the current segment */
+    ItemWork it;
+    int head, rt, j0, j1;
+
+    __device__ __forceinline__ void enter(const FlPaged& c, const FlPagedAttn& a, int s)
+    {
+        seq = s;
+        sw = seq_work<RT>(c, a, s);
+        head_u = head_units<RT, BK>(a, sw, sw.nrt);
+    }
+    __device__ __forceinline__ bool next(const FlPaged& c, const FlPagedAttn& a)
+    {
+        while (at < end) {
+            while (at - seq_at >= head_u * c.n_kv) {
+                seq_at += head_u * c.n_kv;
+                enter(c, a, seq + 1);
+            }
+            uint32_t off = at - seq_at;
+            head = (int)(off / head_u);
+            off -= head * head_u;
+            uint32_t item_at = at - off;
+            for (rt = 0;; rt++) {
+                it = item_work<RT, BK>(a, sw, rt);
+                const uint32_t n = kItemCost + it.tiles;
+                if (off < n) break;
+                off -= n;
+                item_at += n;
+            }
+            item_at += kItemCost;
+            j0 = at > item_at ? (int)(at - item_at) : 0;
+            j1 = end > item_at ? (int)min((uint32_t)it.tiles, end - item_at) : 0;
+            at = item_at + it.tiles;
+            if (at > end) at = end;
+            if (j1 > j0) return true;
+        }
+        return false;
+    }
+};
+
+template <typename T, int KV, int HD>
+__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, const FlPagedAttn a)
+{
+    constexpr bool SPLIT = sizeof(T) == 4;
+    using C = Cfg<KV, HD, SPLIT>;
+    constexpr int NQ = C::NQ, BK = C::BK, ST = C::STAGES, RT = C::RT;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = fl_smem_u32(smem_raw), s_base = (raw + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (s_base - raw);
+    const uint32_t s_q = s_base, s_k = s_base + C::QBYTES, s_v = s_k + ST * C::TBYTES;
+    uint8_t* info = smem + C::QBYTES + 2 * ST * C::TBYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(info + ST * C::INFO);
+    uint64_t *k_full = bars, *k_empty = bars + 3, *v_full = bars + 6, *v_empty = bars + 9;
+    uint64_t *s_full = bars + 12, *p_full = bars + 14, *q_full = bars + 16, *o_full = bars + 17, *pv_done = bars + 18,
+             *done = bars + 19;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 20);
+    volatile int* abort = reinterpret_cast<volatile int*>(tmem_holder + 1);
+    __shared__ uint32_t s_scan[kThreads / 32], s_at;
+    __shared__ int s_seq;
+    __shared__ float s_fr[RT];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const FlAttnSpace ws = fl_attn_space(a.workspace, c.n_seqs, kMaxCtas, RT, HD);
+    fl_pdl_trigger(); /* the merge kernel may take its place; it waits for this grid's end */
+
+    if (tid == 0) {
+        for (int s = 0; s < 3; s++) {
+            fl_mbar_init(&k_full[s], kLoadWarps * 32);
+            fl_mbar_init(&v_full[s], kLoadWarps * 32);
+            fl_mbar_init(&k_empty[s], 1);
+            /* the scales of a stage are read by the softmax warps */
+            fl_mbar_init(&v_empty[s], 1 + NQ * 4);
+        }
+        for (int b = 0; b < 2; b++) {
+            fl_mbar_init(&s_full[b], 1);
+            fl_mbar_init(&p_full[b], 4);
+        }
+        fl_mbar_init(q_full, NQ * 4);
+        fl_mbar_init(o_full, 1);
+        fl_mbar_init(pv_done, 1);
+        fl_mbar_init(done, 1);
+        *abort = 0;
+        s_seq = -1;
+        fl_fence_mbar_init();
+    }
+    if (warp == kSoftWarps + kLoadWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fl_smem_u32(tmem_holder)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+
+    /* ── this CTA's range: a scan over the sequences' units ── */
+    const int per_thread = (c.n_seqs + kThreads - 1) / kThreads;
+    const int lo = min(tid * per_thread, c.n_seqs), hi = min(lo + per_thread, c.n_seqs);
+    auto units = [&](int s) {
+        const SeqWork w = seq_work<RT>(c, a, s);
+        return head_units<RT, BK>(a, w, w.nrt) * (uint32_t)c.n_kv;
+    };
+    uint32_t mine = 0;
+    for (int s = lo; s < hi; s++) mine += units(s);
+    uint32_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += u;
+    }
+    if (lane == 31) s_scan[warp] = before;
+    fence_before();
+    __syncthreads();
+    fence_after();
+    FlSchedule sc;
+    sc.total = 0;
+    before -= mine;
+    for (int w = 0; w < kThreads / 32; w++) {
+        if (w < warp) before += s_scan[w];
+        sc.total += s_scan[w];
+    }
+    sc.per = max((uint32_t)kMinUnits, (sc.total + gridDim.x - 1) / gridDim.x);
+    const unsigned long long w0_64 = (unsigned long long)blockIdx.x * sc.per;
+    Segments<RT, BK> seg;
+    seg.at = (uint32_t)min(w0_64, (unsigned long long)sc.total);
+    seg.end = (uint32_t)min(w0_64 + sc.per, (unsigned long long)sc.total);
+    if (blockIdx.x == 0 && tid == 0) *ws.sched = sc;
+    const bool find = seg.at < seg.end && before <= seg.at && seg.at - before < mine;
+    if (find || blockIdx.x == 0) {
+        uint32_t at = before;
+        for (int s = lo; s < hi; s++) {
+            const uint32_t n = units(s);
+            if (blockIdx.x == 0) ws.seq_unit[s] = at;
+            if (find && at <= seg.at && seg.at - at < n) s_seq = s, s_at = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    const uint32_t tmem = *tmem_holder;
+    const bool work = s_seq >= 0;
+    if (work) {
+        seg.seq_at = s_at;
+        seg.enter(c, a, s_seq);
+    }
+    const int win = a.window > 0 ? a.window : INT_MAX;
+
+    if (!work) {
+    } else if (warp >= kSoftWarps && warp < kSoftWarps + kLoadWarps) {
+        /* ── K and V ── */
+        const int lt = tid - kSoftWarps * 32;
+        int n = 0; /* key tiles so far */
+        bool ok = true;
+        while (ok && seg.next(c, a)) {
+            const int32_t* table = c.table + (size_t)seg.seq * c.cols;
+            const int see_lo = a.window > 0 ? max(0, seg.it.pos_min + 1 - a.window) : 0; /* keys that some row sees */
+            const int see_hi = min(seg.sw.len, seg.it.pos_max + 1);
+            int e_run = -100;
+            for (int j = seg.j0; j < seg.j1; j++, n++) {
+                const int key0 = (seg.it.tile0 + j) * BK, st = n % ST;
+                const uint32_t par = ((n / ST) & 1) ^ 1;
+                int page = -1; /* lane i: page of keys key0 + 16 i .. */
+                if (lane < BK / 16) {
+                    const int key = key0 + 16 * lane;
+                    if (key < see_hi) page = __ldg(table + (key >> c.page_shift));
+                    if ((unsigned)page >= (unsigned)c.n_pages) page = -1;
+                }
+                auto row_of = [&](int kk) -> int64_t {
+                    const int pg = __shfl_sync(0xffffffffu, page, kk >> 4);
+                    if (pg < 0) return -1;
+                    return (((int64_t)pg * c.n_kv + seg.head) << c.page_shift) + ((key0 + kk) & ((1 << c.page_shift) - 1));
+                };
+                uint8_t* inf = info + st * C::INFO;
+                const uint32_t kd = s_k + st * C::TBYTES, vd = s_v + st * C::TBYTES;
+                const bool partial = key0 + BK - 1 > seg.it.pos_min || seg.it.pos_max - key0 >= win;
+                constexpr int KPP = kLoadWarps * 32 / C::PIECES; /* keys a pass of the warps covers */
+                const int pc = lt % C::PIECES, k_in = lt / C::PIECES;
+                if constexpr (KV == FL_KV_F16) {
+                    auto dst = [&](uint32_t base, int kk) {
+                        return base + (pc >> 3) * (BK * 128) + kk * 128 + (((pc & 7) ^ (kk & 7)) << 4);
+                    };
+                    auto bring = [&](uint32_t base, const void* src) {
+#pragma unroll
+                        for (int i = 0; i < C::NP; i++) {
+                            const int kk = i * KPP + k_in;
+                            const int64_t row = row_of(kk);
+                            if (row >= 0)
+                                fl_cp_async16(dst(base, kk), static_cast<const uint8_t*>(src) + row * C::ROW + pc * 16);
+                            else
+                                sts16(dst(base, kk), 0, 0, 0, 0);
+                        }
+                        fl_cp_async_commit();
+                    };
+                    if (!(ok = wait_warp(&k_empty[st], par, abort))) break;
+                    bring(kd, c.k);
+                    if (!(ok = wait_warp(&v_empty[st], par, abort))) break;
+                    bring(vd, c.v);
+                    fl_cp_async_wait<1>();
+                    if (lt < BK / 16) reinterpret_cast<int*>(inf + BK * 8 + 32)[lt] = page >= 0;
+                    fl_fence_proxy_async();
+                    fl_mbar_arrive(&k_full[st]);
+                    fl_cp_async_wait<0>();
+                    if (partial) {
+                        /* keys that no row sees become zero; NaN and infinities that only some rows see are noted and left out */
+                        bool any = false;
+#pragma unroll 1
+                        for (int i = 0; i < C::NP; i++) {
+                            const int kk = i * KPP + k_in;
+                            const uint32_t at = dst(vd, kk);
+                            uint32_t bits = 0;
+                            if (key0 + kk < see_lo || key0 + kk >= see_hi) {
+                                sts16(at, 0, 0, 0, 0);
+                            } else {
+                                const uint4 v = lds16(at);
+                                bits = odd_bits(v.x) | odd_bits(v.y) << 2 | odd_bits(v.z) << 4 | odd_bits(v.w) << 6;
+                                if (bits) {
+                                    auto keep = [](uint32_t w) {
+                                        const uint32_t b = odd_bits(w);
+                                        return w & ~((b & 1 ? 0xffffu : 0u) | (b & 2 ? 0xffff0000u : 0u));
+                                    };
+                                    sts16(at, keep(v.x), keep(v.y), keep(v.z), keep(v.w));
+                                    any = true;
+                                }
+                            }
+                            (inf + BK * 8 + 64)[kk * (HD / 8) + pc] = (uint8_t)bits;
+                        }
+                        any = __any_sync(0xffffffffu, any);
+                        if (lane == 0) reinterpret_cast<int*>(inf + BK * 8)[4 + (warp & 3)] = any;
+                    }
+                    fl_fence_proxy_async();
+                    fl_mbar_arrive(&v_full[st]);
+                } else {
+                    uint4 kr[C::NP], vr[C::NP];
+                    auto fetch = [&](uint4 (&r)[C::NP], const void* src) {
+#pragma unroll
+                        for (int i = 0; i < C::NP; i++) {
+                            const int64_t row = row_of(i * KPP + k_in);
+                            r[i] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(src) + row * C::ROW) + pc)
+                                            : make_uint4(0, 0, 0, 0);
+                        }
+                    };
+                    auto put = [&](uint32_t base, int kk, const uint4& r) {
+                        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+                        uint32_t h[8];
+#pragma unroll
+                        for (int x = 0; x < 4; x++) fl_widen4<KV>(w[x], h[2 * x], h[2 * x + 1]);
+                        const uint32_t at = base + (pc >> 2) * (BK * 128) + kk * 128;
+                        const uint32_t c0 = ((((pc & 3) * 2) ^ (kk & 7)) << 4), c1 = ((((pc & 3) * 2 + 1) ^ (kk & 7)) << 4);
+                        if (pc & 4) { /* the other half first: the two blocks lie on the same banks */
+                            sts16(at + c1, h[4], h[5], h[6], h[7]);
+                            sts16(at + c0, h[0], h[1], h[2], h[3]);
+                        } else {
+                            sts16(at + c0, h[0], h[1], h[2], h[3]);
+                            sts16(at + c1, h[4], h[5], h[6], h[7]);
+                        }
+                    };
+                    fetch(kr, c.k);
+                    fetch(vr, c.v);
+                    /* scales: thread lt holds those of key lt */
+                    float sk = 0.0f, sv = 0.0f;
+                    {
+                        const int64_t row = row_of(lt & (BK - 1));
+                        const int key = key0 + (lt & (BK - 1));
+                        if (lt < BK && row >= 0) {
+                            sk = __ldg(c.k_scale + row);
+                            if (key >= see_lo && key < see_hi) sv = __ldg(c.v_scale + row);
+                        }
+                    }
+                    if (!(ok = wait_warp(&k_empty[st], par, abort))) break;
+#pragma unroll
+                    for (int i = 0; i < C::NP; i++) put(kd, i * KPP + k_in, kr[i]);
+                    if (!(ok = wait_warp(&v_empty[st], par, abort))) break; /* the stage's scales go with V */
+                    /* the largest finite scale's exponent, so far in this segment */
+                    const uint32_t b = __float_as_uint(sv) & 0x7fffffffu;
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
+                    int* evs = reinterpret_cast<int*>(inf + BK * 8);
+                    if (lane == 0) evs[warp & 3] = (int)(top >> 23) - 127;
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    e_run = max(e_run, max(max(evs[0], evs[1]), max(evs[2], evs[3])));
+                    if (lt < BK) {
+                        reinterpret_cast<float*>(inf)[lt] = sk;
+                        reinterpret_cast<float*>(inf)[BK + lt] = fl_scale2(sv, kUp - e_run);
+                    }
+                    if (lt < BK / 16) reinterpret_cast<int*>(inf + BK * 8 + 32)[lt] = page >= 0;
+                    fl_fence_proxy_async();
+                    fl_mbar_arrive(&k_full[st]);
+                    bool any = false;
+#pragma unroll
+                    for (int i = 0; i < C::NP; i++) {
+                        const int kk = i * KPP + k_in;
+                        if (KV == FL_KV_F8 && partial) {
+                            /* as for F16: 0x7f is NaN */
+                            uint32_t bits = 0;
+                            if (key0 + kk < see_lo || key0 + kk >= see_hi) {
+                                vr[i] = make_uint4(0, 0, 0, 0);
+                            } else {
+                                uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+                                for (int x = 0; x < 16; x++) {
+                                    const uint32_t byte = (w[x >> 2] >> (8 * (x & 3))) & 0x7fu;
+                                    if (byte == 0x7fu) {
+                                        bits |= 1u << x;
+                                        w[x >> 2] &= ~(0xffu << (8 * (x & 3)));
+                                    }
+                                }
+                                vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                                any |= bits != 0;
+                            }
+                            reinterpret_cast<uint16_t*>(inf + BK * 8 + 64)[kk * (HD / 16) + pc] = (uint16_t)bits;
+                        }
+                        put(vd, kk, vr[i]);
+                    }
+                    if (KV == FL_KV_F8 && partial) {
+                        any = __any_sync(0xffffffffu, any);
+                        if (lane == 0) evs[4 + (warp & 3)] = any;
+                    }
+                    fl_fence_proxy_async();
+                    fl_mbar_arrive(&v_full[st]);
+                }
+            }
+        }
+    } else if (warp == kSoftWarps + kLoadWarps) {
+        /* ── the tensor core ── */
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc(BK, false), id_o = idesc(HD, true);
+            bool ok = true;
+            int n = 0, segs = 0, p_ph[2] = {0, 0};
+            auto scores = [&](int q, int buf, int st) { /* S[buf] = Q_q K^T */
+                const uint32_t d = tmem + C::S_COL + buf * BK;
+#pragma unroll
+                for (int h = SPLIT ? 1 : 0; h >= 0; h--) /* the low half first */
+#pragma unroll
+                    for (int b = 0; b < HD / 64; b++) {
+                        const uint64_t da = tile_desc(s_q + (q * (SPLIT ? 2 : 1) + h) * C::QTILE + b * 16384, 16);
+                        const uint64_t db = tile_desc(s_k + st * C::TBYTES + b * (BK * 128), 16);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) umma_ss(d, da + 2 * k, db + 2 * k, id_s, (h != (SPLIT ? 1 : 0)) | (b | k) != 0);
+                    }
+            };
+            auto values = [&](int q, int buf, int st, bool first) { /* O_q (+)= P[buf] V */
+                const uint32_t d = tmem + C::O_COL + q * HD, p = tmem + C::S_COL + buf * BK;
+                const uint64_t db = tile_desc(s_v + st * C::TBYTES, BK * 128);
+#pragma unroll
+                for (int h = SPLIT ? 1 : 0; h >= 0; h--)
+#pragma unroll
+                    for (int k = 0; k < BK / 16; k++)
+                        umma_ts(d, (h ? tmem + C::LOW_COL + buf * (BK / 2) : p) + k * 8, db + k * (2048 >> 4), id_o,
+                                !first | (h != (SPLIT ? 1 : 0)) | (k != 0));
+            };
+            while (ok && seg.next(c, a)) {
+                const int tiles = seg.j1 - seg.j0, nq = NQ == 2 && seg.it.rows > 128 ? 2 : 1;
+                if (!(ok = wait_bar(q_full, segs & 1, abort))) break;
+                fence_after();
+                if (!(ok = wait_bar(&k_full[n % ST], (n / ST) & 1, abort))) break;
+                fence_after();
+                for (int q = 0; q < nq; q++) {
+                    scores(q, q, n % ST);
+                    umma_commit(&s_full[q]);
+                }
+                umma_commit(&k_empty[n % ST]);
+                for (int j = 0; j < tiles && ok; j++) {
+                    const int sv = (n + j) % ST, sk = (n + j + 1) % ST;
+                    const bool more = j + 1 < tiles;
+                    if (NQ == 1 && ST > 1 && more) { /* the next scores while these are exponentiated */
+                        if (!(ok = wait_bar(&k_full[sk], ((n + j + 1) / ST) & 1, abort))) break;
+                        fence_after();
+                        scores(0, (j + 1) & 1, sk);
+                        umma_commit(&s_full[(j + 1) & 1]);
+                        umma_commit(&k_empty[sk]);
+                    }
+                    if (!(ok = wait_bar(&v_full[sv], ((n + j) / ST) & 1, abort))) break;
+                    for (int q = 0; q < nq; q++) {
+                        const int buf = NQ == 1 ? j & 1 : q;
+                        if (!(ok = wait_bar(&p_full[buf], p_ph[buf] & 1, abort))) break;
+                        p_ph[buf]++;
+                        fence_after();
+                        values(q, buf, sv, j == 0);
+                        if (NQ == 1) umma_commit(pv_done);
+                        if (NQ == 2 && more) {
+                            if (q == 0 && !(ok = wait_bar(&k_full[sk], ((n + j + 1) / ST) & 1, abort))) break;
+                            fence_after();
+                            scores(q, q, sk);
+                            umma_commit(&s_full[q]);
+                        }
+                    }
+                    umma_commit(&v_empty[sv]);
+                    if (NQ == 2 && more) umma_commit(&k_empty[sk]);
+                    if (NQ == 1 && ST == 1 && more) { /* one stage: the next keys come once these values are done */
+                        if (!(ok = wait_bar(&k_full[sk], ((n + j + 1) / ST) & 1, abort))) break;
+                        fence_after();
+                        scores(0, (j + 1) & 1, sk);
+                        umma_commit(&s_full[(j + 1) & 1]);
+                        umma_commit(&k_empty[sk]);
+                    }
+                }
+                if (!ok) break;
+                umma_commit(o_full);
+                n += tiles;
+                segs++;
+            }
+            /* every product issued is done before the tensor memory is freed */
+            umma_commit(done);
+            const bool dummy = fl_mbar_wait(done, 0, nullptr);
+            (void)dummy;
+        }
+    } else if (warp < NQ * 4) {
+        /* ── softmax: a row per thread ── */
+        const int q = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        int n = 0, segs = 0, s_ph[2] = {0, 0}, pv_ph = 0;
+        bool ok = true;
+        while (ok && seg.next(c, a)) {
+            const int tiles = seg.j1 - seg.j0;
+            const bool live = NQ == 1 || q == 0 || seg.it.rows > 128; /* a second row tile may be empty */
+            /* q of this warp's 32 rows, as fp16 of largest magnitude in [2^14, 2^15) */
+            {
+                constexpr int LANES = HD / 8, PER = 32 / LANES;
+                const float sign = a.score_unit < 0.0f ? -1.0f : 1.0f;
+#pragma unroll 2
+                for (int x = 0; x < 32; x += PER) {
+                    const int row = q * 128 + quarter * 32 + x + lane / LANES, e = (lane % LANES) * 8;
+                    float v[8] = {};
+                    if (row < seg.it.rows) {
+                        const int f = seg.it.f0 + row, i = fl_div_grp(a, f);
+                        fl_load8(static_cast<const T*>(a.q) + (int64_t)(seg.sw.row0 + i) * a.q_stride +
+                                     (int64_t)(seg.head * a.grp + f - i * a.grp) * HD + e, v);
+                    }
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int z = 0; z < 8; z++) top = max(top, __float_as_uint(v[z]) & 0x7fffffffu);
+#pragma unroll
+                    for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const int up = top < 0x7f800000u ? 14 + 127 - (int)(top >> 23) : 0;
+                    if (e == 0) s_fr[row] = fl_scale2(fabsf(a.score_unit), -up);
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int z = 0; z < 4; z++) {
+                        const float y0 = fl_scale2(v[2 * z], up) * sign, y1 = fl_scale2(v[2 * z + 1], up) * sign;
+                        h[z] = fl_pack_half2(y0, y1);
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[z]));
+                        l[z] = fl_pack_half2(y0 - f.x, y1 - f.y);
+                    }
+                    const int rr = quarter * 32 + x + lane / LANES;
+                    const uint32_t at = s_q + q * (SPLIT ? 2 : 1) * C::QTILE + (e >> 6) * 16384 + rr * 128 +
+                                        ((((e >> 3) & 7) ^ (rr & 7)) << 4);
+                    sts16(at, h[0], h[1], h[2], h[3]);
+                    if (SPLIT) sts16(at + C::QTILE, l[0], l[1], l[2], l[3]);
+                }
+                fl_fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) fl_mbar_arrive(q_full);
+            }
+            const int row = q * 128 + r;
+            const float fr = s_fr[row];
+            const int pos = row < seg.it.rows ? seg.sw.first + fl_div_grp(a, seg.it.f0 + row) : -1;
+            float m = -INFINITY, l = 0.0f;
+            int e_acc = -100; /* exponent of the values' scales that O counts in */
+            uint32_t nan_bits[HD / 32] = {};
+            for (int j = 0; j < tiles; j++, n++) {
+                const int st = n % ST, buf = NQ == 1 ? j & 1 : q;
+                const uint8_t* inf = info + st * C::INFO;
+                const int key0 = (seg.it.tile0 + seg.j0 + j) * BK;
+                /* the stage's scales (and what V's bring-up found) are there once V is */
+                if (!(ok = wait_warp(&v_full[st], (n / ST) & 1, abort))) break;
+                if (!live) {
+                    __syncwarp();
+                    if (lane == 0) fl_mbar_arrive(&v_empty[st]);
+                    continue;
+                }
+                if (!(ok = wait_warp(&s_full[buf], s_ph[buf] & 1, abort))) break;
+                s_ph[buf]++;
+                fence_after();
+                const uint32_t s_at = lanes + C::S_COL + buf * BK;
+                const float* sk = reinterpret_cast<const float*>(inf);
+                const float* sv = sk + BK;
+                const int* evs = reinterpret_cast<const int*>(inf + BK * 8);
+                const int* there = reinterpret_cast<const int*>(inf + BK * 8 + 32);
+                bool holes = false;
+#pragma unroll
+                for (int x = 0; x < BK / 16; x++) holes |= !there[x];
+                const bool masked = holes || key0 + BK - 1 > seg.it.pos_min || key0 + BK > seg.sw.len || seg.it.pos_max - key0 >= win;
+                /* columns the row sees: (c_lo, c_hi] */
+                const int c_hi = min(pos, seg.sw.len - 1) - key0, c_lo = pos - key0 < win ? -1 : pos - key0 - win;
+                auto hidden = [&](int col) { return col > c_hi || col <= c_lo || (holes && !there[col >> 4]); };
+
+                /* the largest score */
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int b = 0; b < BK; b += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(s_at + b, v);
+#pragma unroll
+                    for (int z = 0; z < 32; z += 4) {
+                        float x[4];
+#pragma unroll
+                        for (int y = 0; y < 4; y++) x[y] = __uint_as_float(v[z + y]);
+                        if (C::ES == 1) {
+                            const float4 k4 = *reinterpret_cast<const float4*>(sk + b + z);
+                            x[0] *= k4.x, x[1] *= k4.y, x[2] *= k4.z, x[3] *= k4.w;
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int y = 0; y < 4; y++)
+                                if (hidden(b + z + y)) x[y] = -INFINITY;
+                        }
+                        mx = fmaxf(fmaxf(mx, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+                    }
+                }
+                const float cap = a.softcap * 1.44269504f;
+                auto curve = [&](float x) { /* the score of a scaled product */
+                    x *= fr;
+                    if (a.softcap > 0.0f) {
+                        if (SPLIT) {
+                            x = tanhf(x) * cap;
+                        } else {
+                            float d;
+                            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(fl_ex2(x * 2.88539008f) + 1.0f));
+                            x = fmaf(-2.0f * cap, d, cap);
+                        }
+                    }
+                    return x;
+                };
+                if (mx > -INFINITY) mx = curve(mx);
+                /* O is rescaled when the maximum grew far, or the values' scales did */
+                float f = 1.0f;
+                bool moved = false;
+                if (mx > m + kLazy || (m == -INFINITY && mx > -INFINITY)) {
+                    f = fl_ex2(m - mx);
+                    l *= f;
+                    m = mx;
+                    moved = true;
+                }
+                if (C::ES == 1) {
+                    const int e = max(e_acc, max(max(evs[0], evs[1]), max(evs[2], evs[3])));
+                    if (e > e_acc) {
+                        f *= fl_ex2((float)(e_acc - e));
+                        e_acc = e;
+                        moved = true;
+                    }
+                }
+                const bool odd = KV != FL_KV_Q8 && (key0 + BK - 1 > seg.it.pos_min || seg.it.pos_max - key0 >= win) &&
+                                 (evs[4] | evs[5] | evs[6] | evs[7]);
+                if (j > 0 && __any_sync(0xffffffffu, moved)) {
+                    if (NQ == 1) {
+                        /* the products of the tile before are still counted up; for two row tiles S's came after them */
+                        if (!(ok = wait_warp(pv_done, (pv_ph + j - 1) & 1, abort))) break;
+                        fence_after();
+                    }
+#pragma unroll 1
+                    for (int b = 0; b < HD; b += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(lanes + C::O_COL + q * HD + b, v);
+#pragma unroll
+                        for (int z = 0; z < 32; z++) v[z] = __float_as_uint(__uint_as_float(v[z]) * f);
+                        tmem_st32(lanes + C::O_COL + q * HD + b, v);
+                    }
+                    tmem_wait_st();
+                }
+                if (odd) {
+                    /* value elements that are NaN or infinite were left out of the products of a tile that not every
+                     * row sees whole: the rows that see them have NaN there in the end */
+                    const uint32_t* bits = reinterpret_cast<const uint32_t*>(inf + BK * 8 + 64);
+                    for (int k = 0; k < BK; k++) {
+                        if (hidden(k)) continue;
+#pragma unroll
+                        for (int w = 0; w < HD / 32; w++) nan_bits[w] |= bits[k * (HD / 32) + w];
+                    }
+                }
+
+                /* weights */
+                const float ref = (m == -INFINITY ? 0.0f : m) - (C::ES == 1 ? 0.0f : (float)kUp);
+                float sum[2] = {0.0f, 0.0f};
+#pragma unroll 1
+                for (int b = 0; b < BK; b += 32) {
+                    uint32_t v[32], hi[16], low[16];
+                    tmem_ld32(s_at + b, v);
+#pragma unroll
+                    for (int z = 0; z < 32; z += 4) {
+                        float x[4], p[4];
+#pragma unroll
+                        for (int y = 0; y < 4; y++) x[y] = __uint_as_float(v[z + y]);
+                        if (C::ES == 1) {
+                            const float4 k4 = *reinterpret_cast<const float4*>(sk + b + z);
+                            x[0] *= k4.x, x[1] *= k4.y, x[2] *= k4.z, x[3] *= k4.w;
+                        }
+                        if (a.softcap > 0.0f) {
+#pragma unroll
+                            for (int y = 0; y < 4; y++) x[y] = curve(x[y]) - ref;
+                        } else {
+#pragma unroll
+                            for (int y = 0; y < 4; y++) x[y] = fmaf(x[y], fr, -ref);
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int y = 0; y < 4; y++)
+                                if (hidden(b + z + y)) x[y] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            p[y] = fl_ex2(x[y]);
+                            sum[y & 1] += p[y];
+                        }
+                        if (C::ES == 1) {
+                            const float4 v4 = *reinterpret_cast<const float4*>(sv + b + z);
+                            p[0] *= v4.x, p[1] *= v4.y, p[2] *= v4.z, p[3] *= v4.w;
+                            if (masked) {
+#pragma unroll
+                                for (int y = 0; y < 4; y++)
+                                    if (x[y] == -INFINITY) p[y] = 0.0f; /* whatever the scale */
+                            }
+                        }
+                        hi[z / 2] = fl_pack_half2(p[0], p[1]);
+                        hi[z / 2 + 1] = fl_pack_half2(p[2], p[3]);
+                        if (SPLIT) {
+                            const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[z / 2]));
+                            const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[z / 2 + 1]));
+                            low[z / 2] = fl_pack_half2(p[0] - h0.x, p[1] - h0.y);
+                            low[z / 2 + 1] = fl_pack_half2(p[2] - h1.x, p[3] - h1.y);
+                        }
+                    }
+                    tmem_st16(s_at + b / 2, hi); /* over scores that have been read */
+                    if (SPLIT) tmem_st16(lanes + C::LOW_COL + buf * (BK / 2) + b / 2, low);
+                }
+                l += sum[0] + sum[1];
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    fl_mbar_arrive(&p_full[buf]);
+                    fl_mbar_arrive(&v_empty[st]);
+                }
+            }
+            pv_ph += tiles;
+            /* ── the output ── */
+            if (live) {
+                ok = ok && wait_warp(o_full, segs & 1, abort);
+                fence_after();
+                const bool whole = seg.j0 == 0 && seg.j1 == seg.it.tiles;
+                const int slot = 2 * (int)blockIdx.x + (seg.j0 == 0 ? 1 : 0);
+                const int fold = seg.it.f0 + row, i = fl_div_grp(a, fold), h = seg.head * a.grp + fold - i * a.grp;
+                const bool mine = row < seg.it.rows;
+                if (!ok) l = __uint_as_float(0x7fffffffu); /* a wait ran out: NaN, not a number that is wrong */
+                /* o counts in 2^(e_acc - kUp); F16's weights, and their sum, in 2^-kUp */
+                const float unit = fl_scale2(1.0f, (C::ES == 1 ? e_acc : 0) - kUp);
+                if (C::ES == 2) l *= 1.0f / (1 << kUp);
+                const float inv = whole ? (l == 0.0f ? 0.0f : unit / l) : unit;
+                if (mine && !whole) ws.ml[slot * RT + row] = make_float2(m, l);
+                if (mine && whole && a.lse)
+                    a.lse[(int64_t)(seg.sw.row0 + i) * a.n_heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147181f;
+                T* out = static_cast<T*>(a.out) + (int64_t)(seg.sw.row0 + i) * a.out_stride + (int64_t)h * HD;
+                float* part = ws.o + ((size_t)slot * RT + row) * HD;
+#pragma unroll
+                for (int b = 0; b < HD; b += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(lanes + C::O_COL + q * HD + b, v);
+#pragma unroll
+                    for (int z = 0; z < 32; z += 8) {
+                        float x[8];
+#pragma unroll
+                        for (int y = 0; y < 8; y++) {
+                            x[y] = l == 0.0f ? 0.0f : __uint_as_float(v[z + y]) * inv;
+                            if ((nan_bits[b / 32] >> (z + y)) & 1u) x[y] = __uint_as_float(0x7fffffffu);
+                        }
+                        if (mine && whole) fl_store8(out + b + z, x);
+                        if (mine && !whole) fl_store8(part + b + z, x);
+                    }
+                }
+                fence_before();
+            }
+            segs++;
+        }
+    }
+
+    fence_before();
+    __syncthreads();
+    if (warp == kSoftWarps + kLoadWarps) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+/* Items that several ranges share, a warp per (row, head). */
+template <typename T, int KV, int HD>
+__global__ void __launch_bounds__(128) paged_merge_kernel(const FlPaged c, const FlPagedAttn a)
+{
+    using C = Cfg<KV, HD, sizeof(T) == 4>;
+    const int64_t pair = ((int64_t)blockIdx.x * 128 + threadIdx.x) >> 5;
+    if (pair >= (int64_t)c.n_rows * a.n_heads) return;
+    const int row = (int)((uint32_t)pair / (uint32_t)a.n_heads), h = (int)(pair - (int64_t)row * a.n_heads);
+    const int seq = fl_row_seq(c.row_start, c.n_seqs, row);
+    if (seq < 0) return;
+    const SeqWork sw = seq_work<C::RT>(c, a, seq);
+    const int head = fl_div_grp(a, h), f = (row - sw.row0) * a.grp + h - head * a.grp, rt = f / C::RT;
+    /* units of the head's row tiles, and of those before this one */
+    uint32_t all = 0, before = 0;
+    for (int x = threadIdx.x & 31; x < sw.nrt; x += 32) {
+        const uint32_t u = kItemCost + item_work<C::RT, C::BK>(a, sw, x).tiles;
+        all += u;
+        before += x < rt ? u : 0;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    before = __reduce_add_sync(0xffffffffu, before);
+    const int tiles = item_work<C::RT, C::BK>(a, sw, rt).tiles;
+    const FlAttnSpace ws = fl_attn_space(a.workspace, c.n_seqs, kMaxCtas, C::RT, HD);
+    fl_pdl_wait();
+    const uint32_t per = ws.sched->per;
+    const uint32_t t0 = ws.seq_unit[seq] + (uint32_t)head * all + before + kItemCost;
+    const int c0 = (int)(t0 / per), c1 = (int)((t0 + tiles - 1) / per);
+    if (c0 != c1) fl_merge_row<T, HD>(a, ws, c0, c1, f % C::RT, C::RT, row, h); /* else written by its range */
+}
+
+template <typename T, int KV, int HD>
+cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
+{
+    using C = Cfg<KV, HD, sizeof(T) == 4>;
+    static int sms[64] = {}; /* SMs of a device, once its kernel is configured */
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!sms[dev]) {
+        e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return e;
+        int n = 0;
+        e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+        sms[dev] = n < kMaxCtas ? n : kMaxCtas;
+    }
+    paged_tc_kernel<T, KV, HD><<<sms[dev], kThreads, C::SMEM, st>>>(c, a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(((int64_t)c.n_rows * a.n_heads + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_merge_kernel<T, KV, HD>, c, a);
+}
+
+template <typename T, int HD>
+cudaError_t launch_kv(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
+{
+    switch (c.kv_dtype) {
+    case FL_KV_F16: return launch<T, FL_KV_F16, HD>(c, a, st);
+    case FL_KV_Q8: return launch<T, FL_KV_Q8, HD>(c, a, st);
+    case FL_KV_F8: return launch<T, FL_KV_F8, HD>(c, a, st);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+template <int HD>
+cudaError_t launch_type(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
+{
+    switch (a.type) {
+    case 0: return launch_kv<float, HD>(c, a, st);
+    case 1: return launch_kv<__half, HD>(c, a, st);
+    case 30: return launch_kv<__nv_bfloat16, HD>(c, a, st);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+} // namespace
+} // namespace flpt
+
+#endif

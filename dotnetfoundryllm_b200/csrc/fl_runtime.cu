@@ -1585,7 +1585,7 @@ static int check_paged(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t n
     c.n_seqs = b->n_seqs;
     c.cols = b->table_cols;
     c.n_rows = n_rows;
-    c.max_rows = b->max_rows > 0 ? std::min(b->max_rows, n_rows) : n_rows;
+    c.max_rows = std::min(b->max_rows, n_rows);
     c.table = b->page_table;
     c.seq_len = b->seq_len;
     c.row_start = b->row_start;
