@@ -37,7 +37,10 @@ namespace flpt {
 namespace {
 
 constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr int kThreads = (kSoftWarps + kLoadWarps + 4) * 32; /* the last four: one issues to the tensor core */
+/* registers of a softmax, loading and issuing thread, from the launch's 128 each: a softmax thread holds a row of scores */
+constexpr int kSoftRegs = 184, kLoadRegs = 104, kIssueRegs = 40;
+static_assert(kSoftWarps * kSoftRegs + kLoadWarps * kLoadRegs + 4 * kIssueRegs <= kThreads / 32 * 128, "register file");
 constexpr int kMaxCtas = 148;
 constexpr int kItemCost = 3; /* what starting an item costs, in key tiles */
 constexpr int kMinUnits = 2;
@@ -57,7 +60,9 @@ struct Cfg {
     static constexpr int TBYTES = BK * HD * 2;             /* K or V of a key tile */
     static constexpr int PIECES = ROW / 16;                /* 16-byte pieces of a key */
     static constexpr int NP = BK * PIECES / (kLoadWarps * 32); /* pieces of a thread */
-    static constexpr int INFO = BK * 8 + 64 + (KV == FL_KV_Q8 ? 0 : BK * (HD / 16) * 2);
+    /* of a stage: scales of K and V, exponents and findings of the loading warps, mapped 16-key groups, values' flags:
+     * a byte a key, a bit an element */
+    static constexpr int EVS = BK * 8, THERE = EVS + 32, BAD = THERE + 32, ODD = BAD + BK, INFO = ODD + BK * HD / 8;
     static constexpr int SMEM = QBYTES + STAGES * (2 * TBYTES + INFO) + 1024 + 512;
     /* tensor memory columns: two sets of scores (weights over them), the outputs, the weights' low halves */
     static constexpr int S_COL = 0, O_COL = 2 * BK, LOW_COL = 384;
@@ -111,6 +116,27 @@ __device__ __forceinline__ uint32_t head_units(const FlPagedAttn& a, const SeqWo
 }
 
 /* ── small helpers ──────────────────────────────────────────────────────── */
+/* Two fp32 operations an instruction. */
+__device__ __forceinline__ void mul2(float& x0, float& x1, float y0, float y1)
+{
+    asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n mul.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
+        : "+f"(x0), "+f"(x1)
+        : "f"(y0), "f"(y1));
+}
+__device__ __forceinline__ void fma2(float& x0, float& x1, float y, float z)
+{
+    asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %2};\n mov.b64 c, {%3, %3};\n"
+        " fma.rn.f32x2 a, a, b, c;\n mov.b64 {%0, %1}, a;\n}\n"
+        : "+f"(x0), "+f"(x1)
+        : "f"(y), "f"(z));
+}
+__device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1)
+{
+    asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
+        : "+f"(x0), "+f"(x1)
+        : "f"(y0), "f"(y1));
+}
+
 /* One bit per half of w that is NaN or infinite. */
 __device__ __forceinline__ uint32_t odd_bits(uint32_t w)
 {
@@ -167,31 +193,30 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar)
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-#define FL_R32(v) \
-    "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), \
-        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), \
-        "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), \
-        "r"(v[31])
-/* 32 consecutive columns of the thread's lane. */
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32])
+#define FL_F32(c, v) \
+    c(v[0]), c(v[1]), c(v[2]), c(v[3]), c(v[4]), c(v[5]), c(v[6]), c(v[7]), c(v[8]), c(v[9]), c(v[10]), c(v[11]), c(v[12]), \
+        c(v[13]), c(v[14]), c(v[15]), c(v[16]), c(v[17]), c(v[18]), c(v[19]), c(v[20]), c(v[21]), c(v[22]), c(v[23]), \
+        c(v[24]), c(v[25]), c(v[26]), c(v[27]), c(v[28]), c(v[29]), c(v[30]), c(v[31])
+/* 32 consecutive columns of the thread's lane; to be used after tmem_wait_ld on them. */
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v)
 {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
         "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : FL_F32("=f", v)
         : "r"(taddr)
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32])
+__device__ __forceinline__ void tmem_wait_ld(float* v)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : FL_F32("+f", v)::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v)
 {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
         "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        FL_R32(v)
+        FL_F32("f", v)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16])
@@ -378,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     if (!work) {
     } else if (warp >= kSoftWarps && warp < kSoftWarps + kLoadWarps) {
         /* ── K and V ── */
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         const int lt = tid - kSoftWarps * 32;
         int n = 0; /* key tiles so far */
         bool ok = true;
@@ -426,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     if (!(ok = wait_warp(&v_empty[st], par, abort))) break;
                     bring(vd, c.v);
                     fl_cp_async_wait<1>();
-                    if (lt < BK / 16) reinterpret_cast<int*>(inf + BK * 8 + 32)[lt] = page >= 0;
+                    if (lt < BK / 16) reinterpret_cast<int*>(inf + C::THERE)[lt] = page >= 0;
                     fl_fence_proxy_async();
                     fl_mbar_arrive(&k_full[st]);
                     fl_cp_async_wait<0>();
@@ -452,10 +478,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                                     any = true;
                                 }
                             }
-                            (inf + BK * 8 + 64)[kk * (HD / 8) + pc] = (uint8_t)bits;
+                            (inf + C::ODD)[kk * (HD / 8) + pc] = (uint8_t)bits;
                         }
                         any = __any_sync(0xffffffffu, any);
-                        if (lane == 0) reinterpret_cast<int*>(inf + BK * 8)[4 + (warp & 3)] = any;
+                        if (lane == 0) reinterpret_cast<int*>(inf + C::EVS)[4 + (warp & 3)] = any;
                     }
                     fl_fence_proxy_async();
                     fl_mbar_arrive(&v_full[st]);
@@ -503,27 +529,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     /* the largest finite scale's exponent, so far in this segment */
                     const uint32_t b = __float_as_uint(sv) & 0x7fffffffu;
                     const uint32_t top = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
-                    int* evs = reinterpret_cast<int*>(inf + BK * 8);
+                    int* evs = reinterpret_cast<int*>(inf + C::EVS);
                     if (lane == 0) evs[warp & 3] = (int)(top >> 23) - 127;
+                    if (partial && lt < BK) { /* a scale that is no number counts as the row's elements would */
+                        const bool bad = b >= 0x7f800000u;
+                        (inf + C::BAD)[lt] = bad;
+                        if (bad) sv = 0.0f;
+                    }
                     asm volatile("bar.sync 1, 128;" ::: "memory");
                     e_run = max(e_run, max(max(evs[0], evs[1]), max(evs[2], evs[3])));
                     if (lt < BK) {
                         reinterpret_cast<float*>(inf)[lt] = sk;
                         reinterpret_cast<float*>(inf)[BK + lt] = fl_scale2(sv, kUp - e_run);
                     }
-                    if (lt < BK / 16) reinterpret_cast<int*>(inf + BK * 8 + 32)[lt] = page >= 0;
+                    if (lt < BK / 16) reinterpret_cast<int*>(inf + C::THERE)[lt] = page >= 0;
                     fl_fence_proxy_async();
                     fl_mbar_arrive(&k_full[st]);
                     bool any = false;
 #pragma unroll
                     for (int i = 0; i < C::NP; i++) {
                         const int kk = i * KPP + k_in;
-                        if (KV == FL_KV_F8 && partial) {
+                        if (partial) {
                             /* as for F16: 0x7f is NaN */
-                            uint32_t bits = 0;
+                            uint32_t bits = (inf + C::BAD)[kk] ? 0xffffu : 0u;
                             if (key0 + kk < see_lo || key0 + kk >= see_hi) {
                                 vr[i] = make_uint4(0, 0, 0, 0);
-                            } else {
+                            } else if (KV == FL_KV_F8) {
                                 uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
 #pragma unroll
                                 for (int x = 0; x < 16; x++) {
@@ -534,13 +565,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                                     }
                                 }
                                 vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                                any |= bits != 0;
                             }
-                            reinterpret_cast<uint16_t*>(inf + BK * 8 + 64)[kk * (HD / 16) + pc] = (uint16_t)bits;
+                            any |= bits != 0;
+                            reinterpret_cast<uint16_t*>(inf + C::ODD)[kk * (HD / 16) + pc] = (uint16_t)bits;
                         }
                         put(vd, kk, vr[i]);
                     }
-                    if (KV == FL_KV_F8 && partial) {
+                    if (partial) {
                         any = __any_sync(0xffffffffu, any);
                         if (lane == 0) evs[4 + (warp & 3)] = any;
                     }
@@ -549,9 +580,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 }
             }
         }
-    } else if (warp == kSoftWarps + kLoadWarps) {
+    } else if (warp >= kSoftWarps + kLoadWarps) {
         /* ── the tensor core ── */
-        if (lane == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+        if (warp == kSoftWarps + kLoadWarps && lane == 0) {
             constexpr uint32_t id_s = idesc(BK, false), id_o = idesc(HD, true);
             bool ok = true;
             int n = 0, segs = 0, p_ph[2] = {0, 0};
@@ -633,12 +665,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             const bool dummy = fl_mbar_wait(done, 0, nullptr);
             (void)dummy;
         }
-    } else if (warp < NQ * 4) {
+    } else {
         /* ── softmax: a row per thread ── */
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int q = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         int n = 0, segs = 0, s_ph[2] = {0, 0}, pv_ph = 0;
-        bool ok = true;
+        bool ok = q < NQ;
         while (ok && seg.next(c, a)) {
             const int tiles = seg.j1 - seg.j0;
             const bool live = NQ == 1 || q == 0 || seg.it.rows > 128; /* a second row tile may be empty */
@@ -703,54 +736,65 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 const uint32_t s_at = lanes + C::S_COL + buf * BK;
                 const float* sk = reinterpret_cast<const float*>(inf);
                 const float* sv = sk + BK;
-                const int* evs = reinterpret_cast<const int*>(inf + BK * 8);
-                const int* there = reinterpret_cast<const int*>(inf + BK * 8 + 32);
+                const int* evs = reinterpret_cast<const int*>(inf + C::EVS);
+                const int* there = reinterpret_cast<const int*>(inf + C::THERE);
                 bool holes = false;
 #pragma unroll
                 for (int x = 0; x < BK / 16; x++) holes |= !there[x];
                 const bool masked = holes || key0 + BK - 1 > seg.it.pos_min || key0 + BK > seg.sw.len || seg.it.pos_max - key0 >= win;
                 /* columns the row sees: (c_lo, c_hi] */
                 const int c_hi = min(pos, seg.sw.len - 1) - key0, c_lo = pos - key0 < win ? -1 : pos - key0 - win;
-                auto hidden = [&](int col) { return col > c_hi || col <= c_lo || (holes && !there[col >> 4]); };
 
-                /* the largest score */
-                float mx = -INFINITY;
-#pragma unroll 1
-                for (int b = 0; b < BK; b += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(s_at + b, v);
+                float x[BK];
 #pragma unroll
-                    for (int z = 0; z < 32; z += 4) {
-                        float x[4];
+                for (int b = 0; b < BK; b += 32) tmem_ld32(s_at + b, x + b);
 #pragma unroll
-                        for (int y = 0; y < 4; y++) x[y] = __uint_as_float(v[z + y]);
-                        if (C::ES == 1) {
-                            const float4 k4 = *reinterpret_cast<const float4*>(sk + b + z);
-                            x[0] *= k4.x, x[1] *= k4.y, x[2] *= k4.z, x[3] *= k4.w;
-                        }
-                        if (masked) {
+                for (int b = 0; b < BK; b += 32) tmem_wait_ld(x + b);
+                if (C::ES == 1) {
 #pragma unroll
-                            for (int y = 0; y < 4; y++)
-                                if (hidden(b + z + y)) x[y] = -INFINITY;
-                        }
-                        mx = fmaxf(fmaxf(mx, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+                    for (int z = 0; z < BK; z += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4*>(sk + z);
+                        mul2(x[z], x[z + 1], k4.x, k4.y);
+                        mul2(x[z + 2], x[z + 3], k4.z, k4.w);
                     }
                 }
-                const float cap = a.softcap * 1.44269504f;
-                auto curve = [&](float x) { /* the score of a scaled product */
-                    x *= fr;
-                    if (a.softcap > 0.0f) {
-                        if (SPLIT) {
-                            x = tanhf(x) * cap;
-                        } else {
-                            float d;
-                            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(fl_ex2(x * 2.88539008f) + 1.0f));
-                            x = fmaf(-2.0f * cap, d, cap);
-                        }
+                if (masked) {
+                    const uint32_t seen = (uint32_t)max(0, c_hi - c_lo);
+#pragma unroll
+                    for (int z = 0; z < BK; z++)
+                        if ((uint32_t)(z - c_lo - 1) >= seen) x[z] = -INFINITY;
+                    if (holes) {
+#pragma unroll
+                        for (int z = 0; z < BK; z += 16)
+                            if (!there[z / 16]) {
+#pragma unroll
+                                for (int y = 0; y < 16; y++) x[z + y] = -INFINITY;
+                            }
                     }
-                    return x;
-                };
-                if (mx > -INFINITY) mx = curve(mx);
+                }
+                float mx4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int z = 4; z < BK; z += 4)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) mx4[y] = fmaxf(mx4[y], x[z + y]);
+                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), unit_x = fr;
+                if (a.softcap > 0.0f) {
+                    const float cap = a.softcap * 1.44269504f;
+                    auto curve = [&](float y) {
+                        y *= fr;
+                        if (SPLIT) return tanhf(y) * cap;
+                        float d;
+                        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(fl_ex2(y * 2.88539008f) + 1.0f));
+                        return fmaf(-2.0f * cap, d, cap);
+                    };
+                    if (mx > -INFINITY) mx = curve(mx); /* the curve grows with its argument */
+#pragma unroll
+                    for (int z = 0; z < BK; z++)
+                        if (x[z] != -INFINITY) x[z] = curve(x[z]);
+                    unit_x = 1.0f;
+                } else {
+                    mx *= fr;
+                }
                 /* O is rescaled when the maximum grew far, or the values' scales did */
                 float f = 1.0f;
                 bool moved = false;
@@ -768,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         moved = true;
                     }
                 }
-                const bool odd = KV != FL_KV_Q8 && (key0 + BK - 1 > seg.it.pos_min || seg.it.pos_max - key0 >= win) &&
+                const bool odd = (key0 + BK - 1 > seg.it.pos_min || seg.it.pos_max - key0 >= win) &&
                                  (evs[4] | evs[5] | evs[6] | evs[7]);
                 if (j > 0 && __any_sync(0xffffffffu, moved)) {
                     if (NQ == 1) {
@@ -778,10 +822,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     }
 #pragma unroll 1
                     for (int b = 0; b < HD; b += 32) {
-                        uint32_t v[32];
+                        float v[32];
                         tmem_ld32(lanes + C::O_COL + q * HD + b, v);
+                        tmem_wait_ld(v);
 #pragma unroll
-                        for (int z = 0; z < 32; z++) v[z] = __float_as_uint(__uint_as_float(v[z]) * f);
+                        for (int z = 0; z < 32; z++) v[z] *= f;
                         tmem_st32(lanes + C::O_COL + q * HD + b, v);
                     }
                     tmem_wait_st();
@@ -789,9 +834,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 if (odd) {
                     /* value elements that are NaN or infinite were left out of the products of a tile that not every
                      * row sees whole: the rows that see them have NaN there in the end */
-                    const uint32_t* bits = reinterpret_cast<const uint32_t*>(inf + BK * 8 + 64);
+                    const uint32_t* bits = reinterpret_cast<const uint32_t*>(inf + C::ODD);
                     for (int k = 0; k < BK; k++) {
-                        if (hidden(k)) continue;
+                        if (k > c_hi || k <= c_lo || !there[k >> 4]) continue;
 #pragma unroll
                         for (int w = 0; w < HD / 32; w++) nan_bits[w] |= bits[k * (HD / 32) + w];
                     }
@@ -799,59 +844,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
 
                 /* weights */
                 const float ref = (m == -INFINITY ? 0.0f : m) - (C::ES == 1 ? 0.0f : (float)kUp);
-                float sum[2] = {0.0f, 0.0f};
-#pragma unroll 1
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
                 for (int b = 0; b < BK; b += 32) {
-                    uint32_t v[32], hi[16], low[16];
-                    tmem_ld32(s_at + b, v);
+                    uint32_t hi[16], low[16];
 #pragma unroll
-                    for (int z = 0; z < 32; z += 4) {
-                        float x[4], p[4];
+                    for (int z = b; z < b + 32; z += 4) {
+                        fma2(x[z], x[z + 1], unit_x, -ref);
+                        fma2(x[z + 2], x[z + 3], unit_x, -ref);
 #pragma unroll
-                        for (int y = 0; y < 4; y++) x[y] = __uint_as_float(v[z + y]);
+                        for (int y = 0; y < 4; y++) x[z + y] = fl_ex2(x[z + y]);
+                        add2(sum[0], sum[1], x[z], x[z + 1]);
+                        add2(sum[2], sum[3], x[z + 2], x[z + 3]);
                         if (C::ES == 1) {
-                            const float4 k4 = *reinterpret_cast<const float4*>(sk + b + z);
-                            x[0] *= k4.x, x[1] *= k4.y, x[2] *= k4.z, x[3] *= k4.w;
+                            const float4 v4 = *reinterpret_cast<const float4*>(sv + z);
+                            mul2(x[z], x[z + 1], v4.x, v4.y);
+                            mul2(x[z + 2], x[z + 3], v4.z, v4.w);
                         }
-                        if (a.softcap > 0.0f) {
-#pragma unroll
-                            for (int y = 0; y < 4; y++) x[y] = curve(x[y]) - ref;
-                        } else {
-#pragma unroll
-                            for (int y = 0; y < 4; y++) x[y] = fmaf(x[y], fr, -ref);
-                        }
-                        if (masked) {
-#pragma unroll
-                            for (int y = 0; y < 4; y++)
-                                if (hidden(b + z + y)) x[y] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int y = 0; y < 4; y++) {
-                            p[y] = fl_ex2(x[y]);
-                            sum[y & 1] += p[y];
-                        }
-                        if (C::ES == 1) {
-                            const float4 v4 = *reinterpret_cast<const float4*>(sv + b + z);
-                            p[0] *= v4.x, p[1] *= v4.y, p[2] *= v4.z, p[3] *= v4.w;
-                            if (masked) {
-#pragma unroll
-                                for (int y = 0; y < 4; y++)
-                                    if (x[y] == -INFINITY) p[y] = 0.0f; /* whatever the scale */
-                            }
-                        }
-                        hi[z / 2] = fl_pack_half2(p[0], p[1]);
-                        hi[z / 2 + 1] = fl_pack_half2(p[2], p[3]);
+                        const int i = (z - b) / 2;
+                        hi[i] = fl_pack_half2(x[z], x[z + 1]);
+                        hi[i + 1] = fl_pack_half2(x[z + 2], x[z + 3]);
                         if (SPLIT) {
-                            const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[z / 2]));
-                            const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[z / 2 + 1]));
-                            low[z / 2] = fl_pack_half2(p[0] - h0.x, p[1] - h0.y);
-                            low[z / 2 + 1] = fl_pack_half2(p[2] - h1.x, p[3] - h1.y);
+                            const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+                            const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[i + 1]));
+                            low[i] = fl_pack_half2(x[z] - h0.x, x[z + 1] - h0.y);
+                            low[i + 1] = fl_pack_half2(x[z + 2] - h1.x, x[z + 3] - h1.y);
                         }
                     }
-                    tmem_st16(s_at + b / 2, hi); /* over scores that have been read */
+                    tmem_st16(s_at + b / 2, hi); /* over the scores */
                     if (SPLIT) tmem_st16(lanes + C::LOW_COL + buf * (BK / 2) + b / 2, low);
                 }
-                l += sum[0] + sum[1];
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
                 fence_before();
                 __syncwarp();
@@ -881,14 +904,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 float* part = ws.o + ((size_t)slot * RT + row) * HD;
 #pragma unroll
                 for (int b = 0; b < HD; b += 32) {
-                    uint32_t v[32];
+                    float v[32];
                     tmem_ld32(lanes + C::O_COL + q * HD + b, v);
+                    tmem_wait_ld(v);
 #pragma unroll
                     for (int z = 0; z < 32; z += 8) {
                         float x[8];
 #pragma unroll
                         for (int y = 0; y < 8; y++) {
-                            x[y] = l == 0.0f ? 0.0f : __uint_as_float(v[z + y]) * inv;
+                            x[y] = l == 0.0f ? 0.0f : v[z + y] * inv;
                             if ((nan_bits[b / 32] >> (z + y)) & 1u) x[y] = __uint_as_float(0x7fffffffu);
                         }
                         if (mine && whole) fl_store8(out + b + z, x);
