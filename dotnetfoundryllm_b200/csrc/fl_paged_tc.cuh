@@ -137,12 +137,40 @@ __device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1)
         : "f"(y0), "f"(y1));
 }
 
+/* tanh y = 1 - 2 / (e^2y + 1), off by some 2^-23 absolutely.  PRECISE: below
+ * 0.35, where that is too much relatively, the Taylor series to y^11 (the next
+ * term is below 2^-26 of the value). */
+template <bool PRECISE>
+__device__ __forceinline__ float tanh_of(float y)
+{
+    float d;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(fl_ex2(y * 2.88539008f) + 1.0f));
+    float t = fmaf(-2.0f, d, 1.0f);
+    if (PRECISE) {
+        const float z = y * y;
+        float p = -1382.0f / 155925.0f;
+        p = fmaf(p, z, 62.0f / 2835.0f);
+        p = fmaf(p, z, -17.0f / 315.0f);
+        p = fmaf(p, z, 2.0f / 15.0f);
+        p = fmaf(p, z, -1.0f / 3.0f);
+        if (fabsf(y) < 0.35f) t = fmaf(p * z, y, y);
+    }
+    return t;
+}
+
 /* One bit per half of w that is NaN or infinite. */
 __device__ __forceinline__ uint32_t odd_bits(uint32_t w)
 {
     return ((w & 0x7c00u) == 0x7c00u ? 1u : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 2u : 0u);
 }
 
+/* Read once by this SM: not kept in L1. */
+__device__ __forceinline__ uint4 ldg_once(const void* p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
 {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -156,33 +184,29 @@ __device__ __forceinline__ uint4 lds16(uint32_t a)
 /* Descriptors of 128-byte swizzled tiles: rows of 128 bytes, groups of 8 rows
  * 1024 bytes apart.  As a K-major operand (rows = M or N) the leading offset is
  * unused; as an MN-major one (rows = K) it is the distance to the next 64
- * elements of N. */
-__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t lbo)
-{
-    uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)((lbo >> 4) & 0x3fffu) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46; /* version */
-    d |= (uint64_t)2 << 61; /* 128-byte swizzle */
-    return d;
-}
+ * elements of N.  The low word holds address and leading offset in 16-byte
+ * units, the high word group stride, version and swizzle. */
+constexpr uint32_t kDescHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t tile_desc(uint32_t saddr, uint32_t lbo) { return (saddr & 0x3FFFFu) >> 4 | (lbo >> 4) << 16; }
 /* kind::f16, A and B fp16, D fp32, M = 128; bit 16: B is MN-major. */
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn)
 {
     return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum)
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool accum)
 {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"(accum)
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(id), "r"((uint32_t)accum), "r"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accum)
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool accum)
 {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"(accum)
+        "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(id), "r"((uint32_t)accum), "r"(kDescHigh)
         : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar)
@@ -229,6 +253,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+/* The four warps of a role. */
+__device__ __forceinline__ void role_sync(int role) { asm volatile("bar.sync %0, 128;" ::"r"(role + 1) : "memory"); }
+
 /* Bounded wait (~2 s); false once it ran out or another role of the CTA gave up. */
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort)
 {
@@ -253,7 +280,8 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
 }
 
 /* Where a range stands: iterates the segments (items cut to the range) in the
- * same way in every role. */
+ * same way in every role.  Each role keeps one in shared memory, moved on by
+ * one of its threads, so that its state takes no registers in the loops. */
 template <int RT, int BK>
 struct Segments {
     uint32_t at, end, seq_at, head_u;
@@ -262,6 +290,7 @@ struct Segments {
     /* of the current segment */
     ItemWork it;
     int head, rt, j0, j1;
+    bool more;
 
     __device__ __forceinline__ void enter(const FlPaged& c, const FlPagedAttn& a, int s)
     {
@@ -318,6 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     __shared__ uint32_t s_scan[kThreads / 32], s_at;
     __shared__ int s_seq;
     __shared__ float s_fr[RT];
+    __shared__ Segments<RT, BK> s_seg[4];
+    __shared__ uint32_t s_nan[RT][HD / 32]; /* elements of a row's output that are NaN */
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const FlAttnSpace ws = fl_attn_space(a.workspace, c.n_seqs, kMaxCtas, RT, HD);
     fl_pdl_trigger(); /* the merge kernel may take its place; it waits for this grid's end */
@@ -377,27 +408,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     }
     sc.per = max((uint32_t)kMinUnits, (sc.total + gridDim.x - 1) / gridDim.x);
     const unsigned long long w0_64 = (unsigned long long)blockIdx.x * sc.per;
-    Segments<RT, BK> seg;
-    seg.at = (uint32_t)min(w0_64, (unsigned long long)sc.total);
-    seg.end = (uint32_t)min(w0_64 + sc.per, (unsigned long long)sc.total);
+    const uint32_t range_lo = (uint32_t)min(w0_64, (unsigned long long)sc.total);
+    const uint32_t range_hi = (uint32_t)min(w0_64 + sc.per, (unsigned long long)sc.total);
     if (blockIdx.x == 0 && tid == 0) *ws.sched = sc;
-    const bool find = seg.at < seg.end && before <= seg.at && seg.at - before < mine;
+    const bool find = range_lo < range_hi && before <= range_lo && range_lo - before < mine;
     if (find || blockIdx.x == 0) {
         uint32_t at = before;
         for (int s = lo; s < hi; s++) {
             const uint32_t n = units(s);
             if (blockIdx.x == 0) ws.seq_unit[s] = at;
-            if (find && at <= seg.at && seg.at - at < n) s_seq = s, s_at = at;
+            if (find && at <= range_lo && range_lo - at < n) s_seq = s, s_at = at;
             at += n;
         }
     }
     __syncthreads();
     const uint32_t tmem = *tmem_holder;
     const bool work = s_seq >= 0;
-    if (work) {
+    /* roles: softmax of row tile 0, of row tile 1, loading, issuing */
+    Segments<RT, BK>& seg = s_seg[warp >> 2];
+    if (work && (tid & 127) == 0) {
+        seg.at = range_lo;
+        seg.end = range_hi;
         seg.seq_at = s_at;
         seg.enter(c, a, s_seq);
     }
+    /* the next segment, for all four warps of a role */
+    auto next_segment = [&]() {
+        role_sync(warp >> 2);
+        if ((tid & 127) == 0) seg.more = seg.next(c, a);
+        role_sync(warp >> 2);
+        return seg.more;
+    };
     const int win = a.window > 0 ? a.window : INT_MAX;
 
     if (!work) {
@@ -407,13 +448,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         const int lt = tid - kSoftWarps * 32;
         int n = 0; /* key tiles so far */
         bool ok = true;
-        while (ok && seg.next(c, a)) {
+        while (ok && next_segment()) {
             const int32_t* table = c.table + (size_t)seg.seq * c.cols;
-            const int see_lo = a.window > 0 ? max(0, seg.it.pos_min + 1 - a.window) : 0; /* keys that some row sees */
-            const int see_hi = min(seg.sw.len, seg.it.pos_max + 1);
+            const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max, head = seg.head;
+            const int see_lo = a.window > 0 ? max(0, pos_min + 1 - a.window) : 0; /* keys that some row sees */
+            const int see_hi = min(seg.sw.len, pos_max + 1);
+            const int tile_lo = seg.it.tile0 + seg.j0, tile_hi = seg.it.tile0 + seg.j1;
             int e_run = -100;
-            for (int j = seg.j0; j < seg.j1; j++, n++) {
-                const int key0 = (seg.it.tile0 + j) * BK, st = n % ST;
+            for (int j = tile_lo; j < tile_hi; j++, n++) {
+                const int key0 = j * BK, st = n % ST;
                 const uint32_t par = ((n / ST) & 1) ^ 1;
                 int page = -1; /* lane i: page of keys key0 + 16 i .. */
                 if (lane < BK / 16) {
@@ -424,11 +467,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 auto row_of = [&](int kk) -> int64_t {
                     const int pg = __shfl_sync(0xffffffffu, page, kk >> 4);
                     if (pg < 0) return -1;
-                    return (((int64_t)pg * c.n_kv + seg.head) << c.page_shift) + ((key0 + kk) & ((1 << c.page_shift) - 1));
+                    return (((int64_t)pg * c.n_kv + head) << c.page_shift) + ((key0 + kk) & ((1 << c.page_shift) - 1));
                 };
                 uint8_t* inf = info + st * C::INFO;
                 const uint32_t kd = s_k + st * C::TBYTES, vd = s_v + st * C::TBYTES;
-                const bool partial = key0 + BK - 1 > seg.it.pos_min || seg.it.pos_max - key0 >= win;
+                const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
                 constexpr int KPP = kLoadWarps * 32 / C::PIECES; /* keys a pass of the warps covers */
                 const int pc = lt % C::PIECES, k_in = lt / C::PIECES;
                 if constexpr (KV == FL_KV_F16) {
@@ -491,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
 #pragma unroll
                         for (int i = 0; i < C::NP; i++) {
                             const int64_t row = row_of(i * KPP + k_in);
-                            r[i] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(src) + row * C::ROW) + pc)
+                            r[i] = row >= 0 ? ldg_once(static_cast<const uint8_t*>(src) + row * C::ROW + pc * 16)
                                             : make_uint4(0, 0, 0, 0);
                         }
                     };
@@ -536,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         (inf + C::BAD)[lt] = bad;
                         if (bad) sv = 0.0f;
                     }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    role_sync(2);
                     e_run = max(e_run, max(max(evs[0], evs[1]), max(evs[2], evs[3])));
                     if (lt < BK) {
                         reinterpret_cast<float*>(inf)[lt] = sk;
@@ -585,73 +628,70 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == kSoftWarps + kLoadWarps && lane == 0) {
             constexpr uint32_t id_s = idesc(BK, false), id_o = idesc(HD, true);
+            constexpr int H = SPLIT ? 2 : 1;
             bool ok = true;
-            int n = 0, segs = 0, p_ph[2] = {0, 0};
+            int n = 0;
+            uint32_t segs = 0, p_ph = 0; /* phases: bit b of p_ph for weights b */
             auto scores = [&](int q, int buf, int st) { /* S[buf] = Q_q K^T */
                 const uint32_t d = tmem + C::S_COL + buf * BK;
+                const uint32_t qd = tile_desc(s_q + q * H * C::QTILE, 16), kd = tile_desc(s_k + st * C::TBYTES, 16);
 #pragma unroll
-                for (int h = SPLIT ? 1 : 0; h >= 0; h--) /* the low half first */
+                for (int h = H - 1; h >= 0; h--) /* the low half first */
 #pragma unroll
-                    for (int b = 0; b < HD / 64; b++) {
-                        const uint64_t da = tile_desc(s_q + (q * (SPLIT ? 2 : 1) + h) * C::QTILE + b * 16384, 16);
-                        const uint64_t db = tile_desc(s_k + st * C::TBYTES + b * (BK * 128), 16);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) umma_ss(d, da + 2 * k, db + 2 * k, id_s, (h != (SPLIT ? 1 : 0)) | (b | k) != 0);
-                    }
+                    for (int k = 0; k < HD / 16; k++)
+                        umma_ss(d, qd + h * (C::QTILE >> 4) + (k >> 2) * (16384 >> 4) + (k & 3) * 2,
+                                kd + (k >> 2) * (BK * 128 >> 4) + (k & 3) * 2, id_s, h != H - 1 || k != 0);
+                umma_commit(&s_full[buf]);
             };
-            auto values = [&](int q, int buf, int st, bool first) { /* O_q (+)= P[buf] V */
+            auto values = [&](int q, int buf, int st, bool more) { /* O_q (+)= P[buf] V */
                 const uint32_t d = tmem + C::O_COL + q * HD, p = tmem + C::S_COL + buf * BK;
-                const uint64_t db = tile_desc(s_v + st * C::TBYTES, BK * 128);
+                const uint32_t vd = tile_desc(s_v + st * C::TBYTES, BK * 128);
 #pragma unroll
-                for (int h = SPLIT ? 1 : 0; h >= 0; h--)
+                for (int h = H - 1; h >= 0; h--)
 #pragma unroll
                     for (int k = 0; k < BK / 16; k++)
-                        umma_ts(d, (h ? tmem + C::LOW_COL + buf * (BK / 2) : p) + k * 8, db + k * (2048 >> 4), id_o,
-                                !first | (h != (SPLIT ? 1 : 0)) | (k != 0));
+                        umma_ts(d, (h ? tmem + C::LOW_COL + buf * (BK / 2) : p) + k * 8, vd + k * (2048 >> 4), id_o,
+                                more || h != H - 1 || k != 0);
             };
-            while (ok && seg.next(c, a)) {
+            for (;;) {
+                seg.more = seg.next(c, a);
+                if (!seg.more) break;
                 const int tiles = seg.j1 - seg.j0, nq = NQ == 2 && seg.it.rows > 128 ? 2 : 1;
                 if (!(ok = wait_bar(q_full, segs & 1, abort))) break;
-                fence_after();
                 if (!(ok = wait_bar(&k_full[n % ST], (n / ST) & 1, abort))) break;
                 fence_after();
-                for (int q = 0; q < nq; q++) {
-                    scores(q, q, n % ST);
-                    umma_commit(&s_full[q]);
-                }
+                for (int q = 0; q < nq; q++) scores(q, q, n % ST);
                 umma_commit(&k_empty[n % ST]);
                 for (int j = 0; j < tiles && ok; j++) {
                     const int sv = (n + j) % ST, sk = (n + j + 1) % ST;
+                    const uint32_t v_par = ((n + j) / ST) & 1, k_par = ((n + j + 1) / ST) & 1;
                     const bool more = j + 1 < tiles;
                     if (NQ == 1 && ST > 1 && more) { /* the next scores while these are exponentiated */
-                        if (!(ok = wait_bar(&k_full[sk], ((n + j + 1) / ST) & 1, abort))) break;
+                        if (!(ok = wait_bar(&k_full[sk], k_par, abort))) break;
                         fence_after();
                         scores(0, (j + 1) & 1, sk);
-                        umma_commit(&s_full[(j + 1) & 1]);
                         umma_commit(&k_empty[sk]);
                     }
-                    if (!(ok = wait_bar(&v_full[sv], ((n + j) / ST) & 1, abort))) break;
+                    if (!(ok = wait_bar(&v_full[sv], v_par, abort))) break;
                     for (int q = 0; q < nq; q++) {
                         const int buf = NQ == 1 ? j & 1 : q;
-                        if (!(ok = wait_bar(&p_full[buf], p_ph[buf] & 1, abort))) break;
-                        p_ph[buf]++;
+                        if (!(ok = wait_bar(&p_full[buf], (p_ph >> buf) & 1, abort))) break;
+                        p_ph ^= 1u << buf;
                         fence_after();
-                        values(q, buf, sv, j == 0);
+                        values(q, buf, sv, j > 0);
                         if (NQ == 1) umma_commit(pv_done);
                         if (NQ == 2 && more) {
-                            if (q == 0 && !(ok = wait_bar(&k_full[sk], ((n + j + 1) / ST) & 1, abort))) break;
+                            if (q == 0 && !(ok = wait_bar(&k_full[sk], k_par, abort))) break;
                             fence_after();
                             scores(q, q, sk);
-                            umma_commit(&s_full[q]);
                         }
                     }
                     umma_commit(&v_empty[sv]);
                     if (NQ == 2 && more) umma_commit(&k_empty[sk]);
                     if (NQ == 1 && ST == 1 && more) { /* one stage: the next keys come once these values are done */
-                        if (!(ok = wait_bar(&k_full[sk], ((n + j + 1) / ST) & 1, abort))) break;
+                        if (!(ok = wait_bar(&k_full[sk], k_par, abort))) break;
                         fence_after();
                         scores(0, (j + 1) & 1, sk);
-                        umma_commit(&s_full[(j + 1) & 1]);
                         umma_commit(&k_empty[sk]);
                     }
                 }
@@ -670,9 +710,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int q = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        int n = 0, segs = 0, s_ph[2] = {0, 0}, pv_ph = 0;
+        int n = 0;
+        uint32_t segs = 0, s_ph = 0, pv_ph = 0; /* phases: bit b of s_ph for scores b */
         bool ok = q < NQ;
-        while (ok && seg.next(c, a)) {
+        while (ok && next_segment()) {
             const int tiles = seg.j1 - seg.j0;
             const bool live = NQ == 1 || q == 0 || seg.it.rows > 128; /* a second row tile may be empty */
             /* q of this warp's 32 rows, as fp16 of largest magnitude in [2^14, 2^15) */
@@ -718,11 +759,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             const int pos = row < seg.it.rows ? seg.sw.first + fl_div_grp(a, seg.it.f0 + row) : -1;
             float m = -INFINITY, l = 0.0f;
             int e_acc = -100; /* exponent of the values' scales that O counts in */
-            uint32_t nan_bits[HD / 32] = {};
+            bool any_nan = false;
+            const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max, len = seg.sw.len, tile_lo = seg.it.tile0 + seg.j0;
             for (int j = 0; j < tiles; j++, n++) {
                 const int st = n % ST, buf = NQ == 1 ? j & 1 : q;
                 const uint8_t* inf = info + st * C::INFO;
-                const int key0 = (seg.it.tile0 + seg.j0 + j) * BK;
+                const int key0 = (tile_lo + j) * BK;
                 /* the stage's scales (and what V's bring-up found) are there once V is */
                 if (!(ok = wait_warp(&v_full[st], (n / ST) & 1, abort))) break;
                 if (!live) {
@@ -730,8 +772,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     if (lane == 0) fl_mbar_arrive(&v_empty[st]);
                     continue;
                 }
-                if (!(ok = wait_warp(&s_full[buf], s_ph[buf] & 1, abort))) break;
-                s_ph[buf]++;
+                if (!(ok = wait_warp(&s_full[buf], (s_ph >> buf) & 1, abort))) break;
+                s_ph ^= 1u << buf;
                 fence_after();
                 const uint32_t s_at = lanes + C::S_COL + buf * BK;
                 const float* sk = reinterpret_cast<const float*>(inf);
@@ -741,9 +783,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 bool holes = false;
 #pragma unroll
                 for (int x = 0; x < BK / 16; x++) holes |= !there[x];
-                const bool masked = holes || key0 + BK - 1 > seg.it.pos_min || key0 + BK > seg.sw.len || seg.it.pos_max - key0 >= win;
+                const bool masked = holes || key0 + BK - 1 > pos_min || key0 + BK > len || pos_max - key0 >= win;
                 /* columns the row sees: (c_lo, c_hi] */
-                const int c_hi = min(pos, seg.sw.len - 1) - key0, c_lo = pos - key0 < win ? -1 : pos - key0 - win;
+                const int c_hi = min(pos, len - 1) - key0, c_lo = pos - key0 < win ? -1 : pos - key0 - win;
 
                 float x[BK];
 #pragma unroll
@@ -781,11 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 if (a.softcap > 0.0f) {
                     const float cap = a.softcap * 1.44269504f;
                     auto curve = [&](float y) {
-                        y *= fr;
-                        if (SPLIT) return tanhf(y) * cap;
-                        float d;
-                        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(fl_ex2(y * 2.88539008f) + 1.0f));
-                        return fmaf(-2.0f * cap, d, cap);
+                        return tanh_of<SPLIT>(y * fr) * cap;
                     };
                     if (mx > -INFINITY) mx = curve(mx); /* the curve grows with its argument */
 #pragma unroll
@@ -812,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         moved = true;
                     }
                 }
-                const bool odd = (key0 + BK - 1 > seg.it.pos_min || seg.it.pos_max - key0 >= win) &&
+                const bool odd = (key0 + BK - 1 > pos_min || pos_max - key0 >= win) &&
                                  (evs[4] | evs[5] | evs[6] | evs[7]);
                 if (j > 0 && __any_sync(0xffffffffu, moved)) {
                     if (NQ == 1) {
@@ -835,11 +873,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     /* value elements that are NaN or infinite were left out of the products of a tile that not every
                      * row sees whole: the rows that see them have NaN there in the end */
                     const uint32_t* bits = reinterpret_cast<const uint32_t*>(inf + C::ODD);
-                    for (int k = 0; k < BK; k++) {
-                        if (k > c_hi || k <= c_lo || !there[k >> 4]) continue;
-#pragma unroll
-                        for (int w = 0; w < HD / 32; w++) nan_bits[w] |= bits[k * (HD / 32) + w];
+                    for (int w = 0; w < HD / 32; w++) {
+                        uint32_t b = any_nan ? s_nan[row][w] : 0u;
+                        for (int k = max(0, c_lo + 1); k < min(BK, c_hi + 1); k++)
+                            if (there[k >> 4]) b |= bits[k * (HD / 32) + w];
+                        s_nan[row][w] = b;
                     }
+                    any_nan = true;
                 }
 
                 /* weights */
@@ -913,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
 #pragma unroll
                         for (int y = 0; y < 8; y++) {
                             x[y] = l == 0.0f ? 0.0f : v[z + y] * inv;
-                            if ((nan_bits[b / 32] >> (z + y)) & 1u) x[y] = __uint_as_float(0x7fffffffu);
+                            if (any_nan && (s_nan[row][b / 32] >> (z + y) & 1u)) x[y] = __uint_as_float(0x7fffffffu);
                         }
                         if (mine && whole) fl_store8(out + b + z, x);
                         if (mine && !whole) fl_store8(part + b + z, x);
