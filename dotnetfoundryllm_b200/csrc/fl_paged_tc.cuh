@@ -60,10 +60,11 @@ struct Cfg {
     static constexpr int TBYTES = BK * HD * 2;             /* K or V of a key tile */
     static constexpr int PIECES = ROW / 16;                /* 16-byte pieces of a key */
     static constexpr int NP = BK * PIECES / (kLoadWarps * 32); /* pieces of a thread */
-    /* of a stage: scales of K and V, exponents and findings of the loading warps, mapped 16-key groups, values' flags:
+    /* of a key tile: scales of K and V, exponents and findings of the loading warps, mapped 16-key groups, values' flags:
      * a byte a key, a bit an element */
     static constexpr int EVS = BK * 8, THERE = EVS + 32, BAD = THERE + 32, ODD = BAD + BK, INFO = ODD + BK * HD / 8;
-    static constexpr int SMEM = QBYTES + STAGES * (2 * TBYTES + INFO) + 1024 + 512;
+    static constexpr int NI = 4;                           /* infos in flight: more than stages, so that they need no release */
+    static constexpr int SMEM = QBYTES + STAGES * 2 * TBYTES + NI * INFO + 1024 + 512;
     /* tensor memory columns: two sets of scores (weights over them), the outputs, the weights' low halves */
     static constexpr int S_COL = 0, O_COL = 2 * BK, LOW_COL = 384;
     static_assert(O_COL + NQ * HD <= (SPLIT ? LOW_COL : 512) && SMEM <= 232448, "tensor and shared memory");
@@ -116,6 +117,13 @@ __device__ __forceinline__ uint32_t head_units(const FlPagedAttn& a, const SeqWo
 }
 
 /* ── small helpers ──────────────────────────────────────────────────────── */
+/* Keeps sums of x and constants from being formed ahead of a loop and kept in registers. */
+__device__ __forceinline__ uint32_t opaque(uint32_t x)
+{
+    asm volatile("" : "+r"(x));
+    return x;
+}
+
 /* Two fp32 operations an instruction. */
 __device__ __forceinline__ void mul2(float& x0, float& x1, float y0, float y1)
 {
@@ -144,7 +152,7 @@ template <bool PRECISE>
 __device__ __forceinline__ float tanh_of(float y)
 {
     float d;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(fl_ex2(y * 2.88539008f) + 1.0f));
+    asm volatile("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(fl_ex2(y * 2.88539008f) + 1.0f));
     float t = fmaf(-2.0f, d, 1.0f);
     if (PRECISE) {
         const float z = y * y;
@@ -327,7 +335,9 @@ struct Segments {
     }
 };
 
-template <typename T, int KV, int HD>
+/* CAP: softcap > 0, a variant of its own because its 128 curves at once cost the
+ * plain kernel registers that it does not have to spare. */
+template <typename T, int KV, int HD, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, const FlPagedAttn a)
 {
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -338,11 +348,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     uint8_t* smem = smem_raw + (s_base - raw);
     const uint32_t s_q = s_base, s_k = s_base + C::QBYTES, s_v = s_k + ST * C::TBYTES;
     uint8_t* info = smem + C::QBYTES + 2 * ST * C::TBYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(info + ST * C::INFO);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(info + C::NI * C::INFO);
     uint64_t *k_full = bars, *k_empty = bars + 3, *v_full = bars + 6, *v_empty = bars + 9;
     uint64_t *s_full = bars + 12, *p_full = bars + 14, *q_full = bars + 16, *o_full = bars + 17, *pv_done = bars + 18,
-             *done = bars + 19;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 20);
+             *done = bars + 19, *i_full = bars + 20;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 24);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_holder + 1);
     __shared__ uint32_t s_scan[kThreads / 32], s_at;
     __shared__ int s_seq;
@@ -358,9 +368,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             fl_mbar_init(&k_full[s], kLoadWarps * 32);
             fl_mbar_init(&v_full[s], kLoadWarps * 32);
             fl_mbar_init(&k_empty[s], 1);
-            /* the scales of a stage are read by the softmax warps */
-            fl_mbar_init(&v_empty[s], 1 + NQ * 4);
+            fl_mbar_init(&v_empty[s], 1);
         }
+        for (int i = 0; i < C::NI; i++) fl_mbar_init(&i_full[i], kLoadWarps * 32);
         for (int b = 0; b < 2; b++) {
             fl_mbar_init(&s_full[b], 1);
             fl_mbar_init(&p_full[b], 4);
@@ -446,6 +456,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         /* ── K and V ── */
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         const int lt = tid - kSoftWarps * 32;
+        constexpr int KPP = kLoadWarps * 32 / C::PIECES; /* keys that a pass of the warps covers */
+        const int pc = lt % C::PIECES, k_in = lt / C::PIECES;
+        /* a piece's place in its tile in the first pass; pass i lies i * KPP rows on, with the same swizzle where KPP is a
+         * multiple of 8, with the other half's chunks in odd passes where it is 4 */
+        const uint32_t place = C::ES == 2 ? (pc >> 3) * (BK * 128) + k_in * 128 + (((pc & 7) ^ (k_in & 7)) << 4)
+                                          : (pc >> 2) * (BK * 128) + k_in * 128;
+        const uint32_t half0 = (((pc & 3) * 2) ^ (k_in & 7)) << 4, half1 = (((pc & 3) * 2 + 1) ^ (k_in & 7)) << 4;
+        auto at_pass = [&](uint32_t base, int i) { return (KPP == 4 && (i & 1) ? base ^ 64u : base) + i * (KPP * 128); };
+        static_assert(KPP % 8 == 0 || KPP == 4, "swizzle of a pass");
         int n = 0; /* key tiles so far */
         bool ok = true;
         while (ok && next_segment()) {
@@ -453,59 +472,70 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max, head = seg.head;
             const int see_lo = a.window > 0 ? max(0, pos_min + 1 - a.window) : 0; /* keys that some row sees */
             const int see_hi = min(seg.sw.len, pos_max + 1);
-            const int tile_lo = seg.it.tile0 + seg.j0, tile_hi = seg.it.tile0 + seg.j1;
-            int e_run = -100;
-            for (int j = tile_lo; j < tile_hi; j++, n++) {
-                const int key0 = j * BK, st = n % ST;
-                const uint32_t par = ((n / ST) & 1) ^ 1;
-                int page = -1; /* lane i: page of keys key0 + 16 i .. */
+            const int key_end = (seg.it.tile0 + seg.j1) * BK;
+            int key0 = (seg.it.tile0 + seg.j0) * BK, e_run = -100;
+            auto pages_of = [&](int k0) { /* lane i: page of keys k0 + 16 i .., or -1 */
+                int page = -1;
                 if (lane < BK / 16) {
-                    const int key = key0 + 16 * lane;
-                    if (key < see_hi) page = __ldg(table + (key >> c.page_shift));
+                    const int key = k0 + 16 * lane;
+                    if (key < see_hi && k0 < key_end) page = __ldg(table + (key >> c.page_shift));
                     if ((unsigned)page >= (unsigned)c.n_pages) page = -1;
                 }
-                auto row_of = [&](int kk) -> int64_t {
-                    const int pg = __shfl_sync(0xffffffffu, page, kk >> 4);
-                    if (pg < 0) return -1;
-                    return (((int64_t)pg * c.n_kv + head) << c.page_shift) + ((key0 + kk) & ((1 << c.page_shift) - 1));
-                };
-                uint8_t* inf = info + st * C::INFO;
-                const uint32_t kd = s_k + st * C::TBYTES, vd = s_v + st * C::TBYTES;
-                const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
-                constexpr int KPP = kLoadWarps * 32 / C::PIECES; /* keys a pass of the warps covers */
-                const int pc = lt % C::PIECES, k_in = lt / C::PIECES;
-                if constexpr (KV == FL_KV_F16) {
-                    auto dst = [&](uint32_t base, int kk) {
-                        return base + (pc >> 3) * (BK * 128) + kk * 128 + (((pc & 7) ^ (kk & 7)) << 4);
-                    };
-                    auto bring = [&](uint32_t base, const void* src) {
+                return page;
+            };
+            auto row_of = [&](int page, int kk) -> int64_t { /* cache row of key key0 + kk; -1: unmapped */
+                const int pg = __shfl_sync(0xffffffffu, page, kk >> 4);
+                if (pg < 0) return -1;
+                /* tiles start at a multiple of BK, so a key's place in its page depends on kk and the tile alone */
+                return (((int64_t)pg * c.n_kv + head) << c.page_shift);
+            };
+            const int in_page = (1 << c.page_shift) - 1;
+            int page = pages_of(key0);
+            if constexpr (KV == FL_KV_F16) {
+                auto bring = [&](uint32_t base, const void* src, int pg, int k0) {
+                    const uint32_t to = opaque(base + place);
 #pragma unroll
-                        for (int i = 0; i < C::NP; i++) {
-                            const int kk = i * KPP + k_in;
-                            const int64_t row = row_of(kk);
-                            if (row >= 0)
-                                fl_cp_async16(dst(base, kk), static_cast<const uint8_t*>(src) + row * C::ROW + pc * 16);
-                            else
-                                sts16(dst(base, kk), 0, 0, 0, 0);
-                        }
-                        fl_cp_async_commit();
-                    };
-                    if (!(ok = wait_warp(&k_empty[st], par, abort))) break;
-                    bring(kd, c.k);
-                    if (!(ok = wait_warp(&v_empty[st], par, abort))) break;
-                    bring(vd, c.v);
-                    fl_cp_async_wait<1>();
+                    for (int i = 0; i < C::NP; i++) {
+                        const int kk = i * KPP + k_in;
+                        const int64_t row = row_of(pg, kk);
+                        if (row >= 0)
+                            fl_cp_async16(at_pass(to, i), static_cast<const uint8_t*>(src) +
+                                                                  (row + ((k0 + kk) & in_page)) * C::ROW + pc * 16);
+                        else
+                            sts16(at_pass(to, i), 0, 0, 0, 0);
+                    }
+                    fl_cp_async_commit();
+                };
+                /* K of a tile is under way before V of the tile ahead of it has come */
+                if (!(ok = wait_warp(&k_empty[n % ST], ((n / ST) & 1) ^ 1, abort))) break;
+                bring(s_k + (n % ST) * C::TBYTES, c.k, page, key0);
+                for (; key0 < key_end; key0 += BK, n++) {
+                    const int st = n % ST, st1 = (n + 1) % ST;
+                    uint8_t* inf = info + (n % C::NI) * C::INFO;
+                    const uint32_t vd = s_v + st * C::TBYTES;
+                    const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
                     if (lt < BK / 16) reinterpret_cast<int*>(inf + C::THERE)[lt] = page >= 0;
+                    fl_mbar_arrive(&i_full[n % C::NI]);
+                    if (!(ok = wait_warp(&v_empty[st], ((n / ST) & 1) ^ 1, abort))) break;
+                    bring(vd, c.v, page, key0);
+                    page = pages_of(key0 + BK);
+                    fl_cp_async_wait<1>();
                     fl_fence_proxy_async();
                     fl_mbar_arrive(&k_full[st]);
-                    fl_cp_async_wait<0>();
+                    if (key0 + BK < key_end) {
+                        if (!(ok = wait_warp(&k_empty[st1], (((n + 1) / ST) & 1) ^ 1, abort))) break;
+                        bring(s_k + st1 * C::TBYTES, c.k, page, key0 + BK);
+                    } else {
+                        fl_cp_async_commit();
+                    }
+                    fl_cp_async_wait<1>();
                     if (partial) {
                         /* keys that no row sees become zero; NaN and infinities that only some rows see are noted and left out */
                         bool any = false;
 #pragma unroll 1
                         for (int i = 0; i < C::NP; i++) {
                             const int kk = i * KPP + k_in;
-                            const uint32_t at = dst(vd, kk);
+                            const uint32_t at = at_pass(vd + place, i);
                             uint32_t bits = 0;
                             if (key0 + kk < see_lo || key0 + kk >= see_hi) {
                                 sts16(at, 0, 0, 0, 0);
@@ -528,51 +558,53 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     }
                     fl_fence_proxy_async();
                     fl_mbar_arrive(&v_full[st]);
-                } else {
-                    uint4 kr[C::NP], vr[C::NP];
-                    auto fetch = [&](uint4 (&r)[C::NP], const void* src) {
+                }
+                fl_cp_async_wait<0>();
+            } else {
+                uint4 kr[C::NP], vr[C::NP];
+                float sk = 0.0f, sv = 0.0f; /* scales of key lt */
+                auto fetch = [&](uint4 (&r)[C::NP], const void* src, int pg, int k0) {
 #pragma unroll
-                        for (int i = 0; i < C::NP; i++) {
-                            const int64_t row = row_of(i * KPP + k_in);
-                            r[i] = row >= 0 ? ldg_once(static_cast<const uint8_t*>(src) + row * C::ROW + pc * 16)
-                                            : make_uint4(0, 0, 0, 0);
-                        }
-                    };
-                    auto put = [&](uint32_t base, int kk, const uint4& r) {
-                        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-                        uint32_t h[8];
-#pragma unroll
-                        for (int x = 0; x < 4; x++) fl_widen4<KV>(w[x], h[2 * x], h[2 * x + 1]);
-                        const uint32_t at = base + (pc >> 2) * (BK * 128) + kk * 128;
-                        const uint32_t c0 = ((((pc & 3) * 2) ^ (kk & 7)) << 4), c1 = ((((pc & 3) * 2 + 1) ^ (kk & 7)) << 4);
-                        if (pc & 4) { /* the other half first: the two blocks lie on the same banks */
-                            sts16(at + c1, h[4], h[5], h[6], h[7]);
-                            sts16(at + c0, h[0], h[1], h[2], h[3]);
-                        } else {
-                            sts16(at + c0, h[0], h[1], h[2], h[3]);
-                            sts16(at + c1, h[4], h[5], h[6], h[7]);
-                        }
-                    };
-                    fetch(kr, c.k);
-                    fetch(vr, c.v);
-                    /* scales: thread lt holds those of key lt */
-                    float sk = 0.0f, sv = 0.0f;
-                    {
-                        const int64_t row = row_of(lt & (BK - 1));
-                        const int key = key0 + (lt & (BK - 1));
-                        if (lt < BK && row >= 0) {
-                            sk = __ldg(c.k_scale + row);
-                            if (key >= see_lo && key < see_hi) sv = __ldg(c.v_scale + row);
-                        }
+                    for (int i = 0; i < C::NP; i++) {
+                        const int kk = i * KPP + k_in;
+                        const int64_t row = row_of(pg, kk);
+                        r[i] = row >= 0 ? ldg_once(static_cast<const uint8_t*>(src) + (row + ((k0 + kk) & in_page)) * C::ROW + pc * 16)
+                                        : make_uint4(0, 0, 0, 0);
                     }
-                    if (!(ok = wait_warp(&k_empty[st], par, abort))) break;
+                };
+                auto fetch_scales = [&](int pg, int k0) {
+                    const int key = k0 + (lt & (BK - 1));
+                    const int64_t row = row_of(pg, lt & (BK - 1));
+                    sk = sv = 0.0f;
+                    if (lt < BK && row >= 0) {
+                        sk = __ldg(c.k_scale + row + (key & in_page));
+                        if (key >= see_lo && key < see_hi) sv = __ldg(c.v_scale + row + (key & in_page));
+                    }
+                };
+                auto put = [&](uint32_t to, const uint4& r) {
+                    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+                    uint32_t h[8];
 #pragma unroll
-                    for (int i = 0; i < C::NP; i++) put(kd, i * KPP + k_in, kr[i]);
-                    if (!(ok = wait_warp(&v_empty[st], par, abort))) break; /* the stage's scales go with V */
-                    /* the largest finite scale's exponent, so far in this segment */
+                    for (int x = 0; x < 4; x++) fl_widen4<KV>(w[x], h[2 * x], h[2 * x + 1]);
+                    /* lanes of odd blocks store their other half first: both blocks lie on the same banks */
+                    const bool swap = pc & 4;
+                    sts16(to + (swap ? half1 : half0), swap ? h[4] : h[0], swap ? h[5] : h[1], swap ? h[6] : h[2], swap ? h[7] : h[3]);
+                    sts16(to + (swap ? half0 : half1), swap ? h[0] : h[4], swap ? h[1] : h[5], swap ? h[2] : h[6], swap ? h[3] : h[7]);
+                };
+                fetch(kr, c.k, page, key0);
+                fetch_scales(page, key0);
+                for (; key0 < key_end; key0 += BK, n++) {
+                    const int st = n % ST;
+                    const uint32_t par = ((n / ST) & 1) ^ 1;
+                    uint8_t* inf = info + (n % C::NI) * C::INFO;
+                    int* evs = reinterpret_cast<int*>(inf + C::EVS);
+                    const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
+                    fetch(vr, c.v, page, key0);
+                    const int page1 = pages_of(key0 + BK);
+                    if (!(ok = wait_warp(&k_empty[st], par, abort))) break;
+                    /* scales; the largest finite one's exponent, so far in this segment */
                     const uint32_t b = __float_as_uint(sv) & 0x7fffffffu;
                     const uint32_t top = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
-                    int* evs = reinterpret_cast<int*>(inf + C::EVS);
                     if (lane == 0) evs[warp & 3] = (int)(top >> 23) - 127;
                     if (partial && lt < BK) { /* a scale that is no number counts as the row's elements would */
                         const bool bad = b >= 0x7f800000u;
@@ -586,14 +618,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         reinterpret_cast<float*>(inf)[BK + lt] = fl_scale2(sv, kUp - e_run);
                     }
                     if (lt < BK / 16) reinterpret_cast<int*>(inf + C::THERE)[lt] = page >= 0;
+                    fl_mbar_arrive(&i_full[n % C::NI]);
+                    {
+                        const uint32_t to = opaque(s_k + st * C::TBYTES + place);
+#pragma unroll
+                        for (int i = 0; i < C::NP; i++) put(at_pass(to, i), kr[i]);
+                    }
                     fl_fence_proxy_async();
                     fl_mbar_arrive(&k_full[st]);
-                    bool any = false;
+                    page = page1;
+                    if (key0 + BK < key_end) {
+                        fetch(kr, c.k, page, key0 + BK);
+                        fetch_scales(page, key0 + BK);
+                    }
+                    if (!(ok = wait_warp(&v_empty[st], par, abort))) break;
+                    const uint32_t to = opaque(s_v + st * C::TBYTES + place);
+                    if (partial) {
+                        bool any = false;
 #pragma unroll
-                    for (int i = 0; i < C::NP; i++) {
-                        const int kk = i * KPP + k_in;
-                        if (partial) {
-                            /* as for F16: 0x7f is NaN */
+                        for (int i = 0; i < C::NP; i++) {
+                            const int kk = i * KPP + k_in;
+                            /* as for F16: 0x7f is e4m3's NaN */
                             uint32_t bits = (inf + C::BAD)[kk] ? 0xffffu : 0u;
                             if (key0 + kk < see_lo || key0 + kk >= see_hi) {
                                 vr[i] = make_uint4(0, 0, 0, 0);
@@ -612,12 +657,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                             any |= bits != 0;
                             reinterpret_cast<uint16_t*>(inf + C::ODD)[kk * (HD / 16) + pc] = (uint16_t)bits;
                         }
-                        put(vd, kk, vr[i]);
-                    }
-                    if (partial) {
                         any = __any_sync(0xffffffffu, any);
                         if (lane == 0) evs[4 + (warp & 3)] = any;
                     }
+#pragma unroll
+                    for (int i = 0; i < C::NP; i++) put(at_pass(to, i), vr[i]);
                     fl_fence_proxy_async();
                     fl_mbar_arrive(&v_full[st]);
                 }
@@ -633,8 +677,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             int n = 0;
             uint32_t segs = 0, p_ph = 0; /* phases: bit b of p_ph for weights b */
             auto scores = [&](int q, int buf, int st) { /* S[buf] = Q_q K^T */
-                const uint32_t d = tmem + C::S_COL + buf * BK;
-                const uint32_t qd = tile_desc(s_q + q * H * C::QTILE, 16), kd = tile_desc(s_k + st * C::TBYTES, 16);
+                const uint32_t d = opaque(tmem + C::S_COL + buf * BK);
+                const uint32_t qd = opaque(tile_desc(s_q + q * H * C::QTILE, 16)), kd = opaque(tile_desc(s_k + st * C::TBYTES, 16));
 #pragma unroll
                 for (int h = H - 1; h >= 0; h--) /* the low half first */
 #pragma unroll
@@ -644,13 +688,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 umma_commit(&s_full[buf]);
             };
             auto values = [&](int q, int buf, int st, bool more) { /* O_q (+)= P[buf] V */
-                const uint32_t d = tmem + C::O_COL + q * HD, p = tmem + C::S_COL + buf * BK;
-                const uint32_t vd = tile_desc(s_v + st * C::TBYTES, BK * 128);
+                const uint32_t d = opaque(tmem + C::O_COL + q * HD), p = opaque(tmem + C::S_COL + buf * BK);
+                const uint32_t vd = opaque(tile_desc(s_v + st * C::TBYTES, BK * 128)), low = opaque(tmem + C::LOW_COL + buf * (BK / 2));
 #pragma unroll
                 for (int h = H - 1; h >= 0; h--)
 #pragma unroll
                     for (int k = 0; k < BK / 16; k++)
-                        umma_ts(d, (h ? tmem + C::LOW_COL + buf * (BK / 2) : p) + k * 8, vd + k * (2048 >> 4), id_o,
+                        umma_ts(d, (h ? low : p) + k * 8, vd + k * (2048 >> 4), id_o,
                                 more || h != H - 1 || k != 0);
             };
             for (;;) {
@@ -763,15 +807,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max, len = seg.sw.len, tile_lo = seg.it.tile0 + seg.j0;
             for (int j = 0; j < tiles; j++, n++) {
                 const int st = n % ST, buf = NQ == 1 ? j & 1 : q;
-                const uint8_t* inf = info + st * C::INFO;
+                const uint8_t* inf = info + (n % C::NI) * C::INFO;
                 const int key0 = (tile_lo + j) * BK;
-                /* the stage's scales (and what V's bring-up found) are there once V is */
-                if (!(ok = wait_warp(&v_full[st], (n / ST) & 1, abort))) break;
-                if (!live) {
-                    __syncwarp();
-                    if (lane == 0) fl_mbar_arrive(&v_empty[st]);
-                    continue;
-                }
+                if (!live) continue;
+                if (!(ok = wait_warp(&i_full[n % C::NI], (n / C::NI) & 1, abort))) break;
                 if (!(ok = wait_warp(&s_full[buf], (s_ph >> buf) & 1, abort))) break;
                 s_ph ^= 1u << buf;
                 fence_after();
@@ -820,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
 #pragma unroll
                     for (int y = 0; y < 4; y++) mx4[y] = fmaxf(mx4[y], x[z + y]);
                 float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), unit_x = fr;
-                if (a.softcap > 0.0f) {
+                if constexpr (CAP) {
                     const float cap = a.softcap * 1.44269504f;
                     auto curve = [&](float y) {
                         return tanh_of<SPLIT>(y * fr) * cap;
@@ -850,8 +889,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         moved = true;
                     }
                 }
-                const bool odd = (key0 + BK - 1 > pos_min || pos_max - key0 >= win) &&
-                                 (evs[4] | evs[5] | evs[6] | evs[7]);
+                bool odd = false;
+                if (key0 + BK - 1 > pos_min || pos_max - key0 >= win) {
+                    /* what bringing up V found is there once V is */
+                    if (!(ok = wait_warp(&v_full[st], (n / ST) & 1, abort))) break;
+                    odd = evs[4] | evs[5] | evs[6] | evs[7];
+                }
                 if (j > 0 && __any_sync(0xffffffffu, moved)) {
                     if (NQ == 1) {
                         /* the products of the tile before are still counted up; for two row tiles S's came after them */
@@ -918,10 +961,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 tmem_wait_st();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    fl_mbar_arrive(&p_full[buf]);
-                    fl_mbar_arrive(&v_empty[st]);
-                }
+                if (lane == 0) fl_mbar_arrive(&p_full[buf]);
             }
             pv_ph += tiles;
             /* ── the output ── */
@@ -1013,14 +1053,19 @@ cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!sms[dev]) {
-        e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return e;
         int n = 0;
         e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess) return e;
         sms[dev] = n < kMaxCtas ? n : kMaxCtas;
     }
-    paged_tc_kernel<T, KV, HD><<<sms[dev], kThreads, C::SMEM, st>>>(c, a);
+    if (a.softcap > 0.0f)
+        paged_tc_kernel<T, KV, HD, true><<<sms[dev], kThreads, C::SMEM, st>>>(c, a);
+    else
+        paged_tc_kernel<T, KV, HD, false><<<sms[dev], kThreads, C::SMEM, st>>>(c, a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
