@@ -39,7 +39,7 @@ namespace {
 constexpr int kSoftWarps = 8, kLoadWarps = 4;
 constexpr int kThreads = (kSoftWarps + kLoadWarps + 4) * 32; /* the last four: one issues to the tensor core */
 /* registers of a softmax, loading and issuing thread, from the launch's 128 each: a softmax thread holds a row of scores */
-constexpr int kSoftRegs = 184, kLoadRegs = 104, kIssueRegs = 40;
+constexpr int kSoftRegs = 200, kLoadRegs = 64, kIssueRegs = 48;
 static_assert(kSoftWarps * kSoftRegs + kLoadWarps * kLoadRegs + 4 * kIssueRegs <= kThreads / 32 * 128, "register file");
 constexpr int kMaxCtas = 148;
 constexpr int kItemCost = 3; /* what starting an item costs, in key tiles */
@@ -172,13 +172,6 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t w)
     return ((w & 0x7c00u) == 0x7c00u ? 1u : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 2u : 0u);
 }
 
-/* Read once by this SM: not kept in L1. */
-__device__ __forceinline__ uint4 ldg_once(const void* p)
-{
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
 __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
 {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -356,7 +349,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_holder + 1);
     __shared__ uint32_t s_scan[kThreads / 32], s_at;
     __shared__ int s_seq;
-    __shared__ float s_fr[RT];
+    __shared__ float s_fr[RT];                    /* score units of a row's scaled q */
+    __shared__ int s_pos[RT];
     __shared__ Segments<RT, BK> s_seg[4];
     __shared__ uint32_t s_nan[RT][HD / 32]; /* elements of a row's output that are NaN */
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -457,12 +451,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         const int lt = tid - kSoftWarps * 32;
         constexpr int KPP = kLoadWarps * 32 / C::PIECES; /* keys that a pass of the warps covers */
-        const int pc = lt % C::PIECES, k_in = lt / C::PIECES;
+        /* 8-bit: eight lanes hold four pieces of two keys, whose stores of 32 bytes a piece then lie on different banks */
+        const int pc = C::ES == 2 ? lt % C::PIECES : (lane & 3) | ((lane >> 3) * 4) % C::PIECES;
+        const int k_in = C::ES == 2 ? lt / C::PIECES : (warp & 3) * (32 / C::PIECES) + (lane >> 3) * 4 / C::PIECES * 2 + ((lane >> 2) & 1);
         /* a piece's place in its tile in the first pass; pass i lies i * KPP rows on, with the same swizzle where KPP is a
-         * multiple of 8, with the other half's chunks in odd passes where it is 4 */
+         * multiple of 8, with the other half's chunks in odd passes where it is 4.  An 8-bit piece arrives in the first of
+         * the two chunks that it widens to, which its own thread writes: no other storage, no barrier. */
         const uint32_t place = C::ES == 2 ? (pc >> 3) * (BK * 128) + k_in * 128 + (((pc & 7) ^ (k_in & 7)) << 4)
-                                          : (pc >> 2) * (BK * 128) + k_in * 128;
-        const uint32_t half0 = (((pc & 3) * 2) ^ (k_in & 7)) << 4, half1 = (((pc & 3) * 2 + 1) ^ (k_in & 7)) << 4;
+                                          : (pc >> 2) * (BK * 128) + k_in * 128 + (((pc & 3) * 2 ^ (k_in & 7)) << 4);
         auto at_pass = [&](uint32_t base, int i) { return (KPP == 4 && (i & 1) ? base ^ 64u : base) + i * (KPP * 128); };
         static_assert(KPP % 8 == 0 || KPP == 4, "swizzle of a pass");
         int n = 0; /* key tiles so far */
@@ -474,105 +470,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             const int see_hi = min(seg.sw.len, pos_max + 1);
             const int key_end = (seg.it.tile0 + seg.j1) * BK;
             int key0 = (seg.it.tile0 + seg.j0) * BK, e_run = -100;
-            auto pages_of = [&](int k0) { /* lane i: page of keys k0 + 16 i .., or -1 */
+            auto pages_of = [&](int k0) { /* lane i: the table's entry for keys k0 + 16 i .., unchecked so that nothing waits for it */
                 int page = -1;
-                if (lane < BK / 16) {
-                    const int key = k0 + 16 * lane;
-                    if (key < see_hi && k0 < key_end) page = __ldg(table + (key >> c.page_shift));
-                    if ((unsigned)page >= (unsigned)c.n_pages) page = -1;
-                }
+                const int key = k0 + 16 * lane;
+                if (lane < BK / 16 && key < see_hi && k0 < key_end) page = __ldg(table + (key >> c.page_shift));
                 return page;
             };
             auto row_of = [&](int page, int kk) -> int64_t { /* cache row of key key0 + kk; -1: unmapped */
                 const int pg = __shfl_sync(0xffffffffu, page, kk >> 4);
-                if (pg < 0) return -1;
+                if ((unsigned)pg >= (unsigned)c.n_pages) return -1;
                 /* tiles start at a multiple of BK, so a key's place in its page depends on kk and the tile alone */
                 return (((int64_t)pg * c.n_kv + head) << c.page_shift);
             };
             const int in_page = (1 << c.page_shift) - 1;
-            int page = pages_of(key0);
-            if constexpr (KV == FL_KV_F16) {
-                auto bring = [&](uint32_t base, const void* src, int pg, int k0) {
-                    const uint32_t to = opaque(base + place);
+            auto bring = [&](uint32_t base, const void* src, int pg, int k0) { /* one copy group of this thread */
+                const uint32_t to = opaque(base + place);
 #pragma unroll
-                    for (int i = 0; i < C::NP; i++) {
-                        const int kk = i * KPP + k_in;
-                        const int64_t row = row_of(pg, kk);
-                        if (row >= 0)
-                            fl_cp_async16(at_pass(to, i), static_cast<const uint8_t*>(src) +
-                                                                  (row + ((k0 + kk) & in_page)) * C::ROW + pc * 16);
-                        else
-                            sts16(at_pass(to, i), 0, 0, 0, 0);
-                    }
-                    fl_cp_async_commit();
-                };
-                /* K of a tile is under way before V of the tile ahead of it has come */
-                if (!(ok = wait_warp(&k_empty[n % ST], ((n / ST) & 1) ^ 1, abort))) break;
-                bring(s_k + (n % ST) * C::TBYTES, c.k, page, key0);
-                for (; key0 < key_end; key0 += BK, n++) {
-                    const int st = n % ST, st1 = (n + 1) % ST;
-                    uint8_t* inf = info + (n % C::NI) * C::INFO;
-                    const uint32_t vd = s_v + st * C::TBYTES;
-                    const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
-                    if (lt < BK / 16) reinterpret_cast<int*>(inf + C::THERE)[lt] = page >= 0;
-                    fl_mbar_arrive(&i_full[n % C::NI]);
-                    if (!(ok = wait_warp(&v_empty[st], ((n / ST) & 1) ^ 1, abort))) break;
-                    bring(vd, c.v, page, key0);
-                    page = pages_of(key0 + BK);
-                    fl_cp_async_wait<1>();
-                    fl_fence_proxy_async();
-                    fl_mbar_arrive(&k_full[st]);
-                    if (key0 + BK < key_end) {
-                        if (!(ok = wait_warp(&k_empty[st1], (((n + 1) / ST) & 1) ^ 1, abort))) break;
-                        bring(s_k + st1 * C::TBYTES, c.k, page, key0 + BK);
-                    } else {
-                        fl_cp_async_commit();
-                    }
-                    fl_cp_async_wait<1>();
-                    if (partial) {
-                        /* keys that no row sees become zero; NaN and infinities that only some rows see are noted and left out */
-                        bool any = false;
-#pragma unroll 1
-                        for (int i = 0; i < C::NP; i++) {
-                            const int kk = i * KPP + k_in;
-                            const uint32_t at = at_pass(vd + place, i);
-                            uint32_t bits = 0;
-                            if (key0 + kk < see_lo || key0 + kk >= see_hi) {
-                                sts16(at, 0, 0, 0, 0);
-                            } else {
-                                const uint4 v = lds16(at);
-                                bits = odd_bits(v.x) | odd_bits(v.y) << 2 | odd_bits(v.z) << 4 | odd_bits(v.w) << 6;
-                                if (bits) {
-                                    auto keep = [](uint32_t w) {
-                                        const uint32_t b = odd_bits(w);
-                                        return w & ~((b & 1 ? 0xffffu : 0u) | (b & 2 ? 0xffff0000u : 0u));
-                                    };
-                                    sts16(at, keep(v.x), keep(v.y), keep(v.z), keep(v.w));
-                                    any = true;
-                                }
-                            }
-                            (inf + C::ODD)[kk * (HD / 8) + pc] = (uint8_t)bits;
-                        }
-                        any = __any_sync(0xffffffffu, any);
-                        if (lane == 0) reinterpret_cast<int*>(inf + C::EVS)[4 + (warp & 3)] = any;
-                    }
-                    fl_fence_proxy_async();
-                    fl_mbar_arrive(&v_full[st]);
+                for (int i = 0; i < C::NP; i++) {
+                    const int kk = i * KPP + k_in;
+                    const int64_t row = row_of(pg, kk);
+                    if (row >= 0)
+                        fl_cp_async16(at_pass(to, i), static_cast<const uint8_t*>(src) +
+                                                          (row + ((k0 + kk) & in_page)) * C::ROW + pc * 16);
+                    else
+                        sts16(at_pass(to, i), 0, 0, 0, 0);
                 }
-                fl_cp_async_wait<0>();
-            } else {
-                uint4 kr[C::NP], vr[C::NP];
-                float sk = 0.0f, sv = 0.0f; /* scales of key lt */
-                auto fetch = [&](uint4 (&r)[C::NP], const void* src, int pg, int k0) {
-#pragma unroll
-                    for (int i = 0; i < C::NP; i++) {
-                        const int kk = i * KPP + k_in;
-                        const int64_t row = row_of(pg, kk);
-                        r[i] = row >= 0 ? ldg_once(static_cast<const uint8_t*>(src) + (row + ((k0 + kk) & in_page)) * C::ROW + pc * 16)
-                                        : make_uint4(0, 0, 0, 0);
-                    }
-                };
-                auto fetch_scales = [&](int pg, int k0) {
+                fl_cp_async_commit();
+            };
+            float sk = 0.0f, sv = 0.0f; /* 8 bits: scales of key lt */
+            auto fetch_scales = [&](int pg, int k0) {
+                if constexpr (C::ES == 1) {
                     const int key = k0 + (lt & (BK - 1));
                     const int64_t row = row_of(pg, lt & (BK - 1));
                     sk = sv = 0.0f;
@@ -580,28 +507,39 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         sk = __ldg(c.k_scale + row + (key & in_page));
                         if (key >= see_lo && key < see_hi) sv = __ldg(c.v_scale + row + (key & in_page));
                     }
-                };
-                auto put = [&](uint32_t to, const uint4& r) {
-                    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-                    uint32_t h[8];
+                }
+            };
+            auto widen = [&](uint32_t base) { /* this thread's pieces of a tile, in place */
+                if constexpr (C::ES == 1) {
+                    const uint32_t to = opaque(base + place);
 #pragma unroll
-                    for (int x = 0; x < 4; x++) fl_widen4<KV>(w[x], h[2 * x], h[2 * x + 1]);
-                    /* lanes of odd blocks store their other half first: both blocks lie on the same banks */
-                    const bool swap = pc & 4;
-                    sts16(to + (swap ? half1 : half0), swap ? h[4] : h[0], swap ? h[5] : h[1], swap ? h[6] : h[2], swap ? h[7] : h[3]);
-                    sts16(to + (swap ? half0 : half1), swap ? h[0] : h[4], swap ? h[1] : h[5], swap ? h[2] : h[6], swap ? h[3] : h[7]);
-                };
-                fetch(kr, c.k, page, key0);
-                fetch_scales(page, key0);
-                for (; key0 < key_end; key0 += BK, n++) {
-                    const int st = n % ST;
-                    const uint32_t par = ((n / ST) & 1) ^ 1;
-                    uint8_t* inf = info + (n % C::NI) * C::INFO;
-                    int* evs = reinterpret_cast<int*>(inf + C::EVS);
-                    const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
-                    fetch(vr, c.v, page, key0);
-                    const int page1 = pages_of(key0 + BK);
-                    if (!(ok = wait_warp(&k_empty[st], par, abort))) break;
+                    for (int i = 0; i < C::NP; i++) {
+                        const uint4 r = lds16(at_pass(to, i));
+                        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+                        uint32_t h[8];
+#pragma unroll
+                        for (int x = 0; x < 4; x++) fl_widen4<KV>(w[x], h[2 * x], h[2 * x + 1]);
+                        sts16(at_pass(to, i), h[0], h[1], h[2], h[3]);
+                        sts16(at_pass(to, i) ^ 16u, h[4], h[5], h[6], h[7]);
+                    }
+                }
+            };
+            /* K of a tile is under way before V of the tile ahead of it has come */
+            int page = pages_of(key0);
+            if (!(ok = wait_warp(&k_empty[n % ST], ((n / ST) & 1) ^ 1, abort))) break;
+            bring(s_k + (n % ST) * C::TBYTES, c.k, page, key0);
+            fetch_scales(page, key0);
+            for (; key0 < key_end; key0 += BK, n++) {
+                const int st = n % ST, st1 = (n + 1) % ST;
+                uint8_t* inf = info + (n % C::NI) * C::INFO;
+                int* evs = reinterpret_cast<int*>(inf + C::EVS);
+                const uint32_t kd = s_k + st * C::TBYTES, vd = s_v + st * C::TBYTES;
+                const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
+                if (!(ok = wait_warp(&v_empty[st], ((n / ST) & 1) ^ 1, abort))) break;
+                bring(vd, c.v, page, key0);
+                if (lt < BK / 16) reinterpret_cast<int*>(inf + C::THERE)[lt] = (unsigned)page < (unsigned)c.n_pages;
+                page = pages_of(key0 + BK);
+                if constexpr (C::ES == 1) {
                     /* scales; the largest finite one's exponent, so far in this segment */
                     const uint32_t b = __float_as_uint(sv) & 0x7fffffffu;
                     const uint32_t top = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
@@ -617,55 +555,64 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         reinterpret_cast<float*>(inf)[lt] = sk;
                         reinterpret_cast<float*>(inf)[BK + lt] = fl_scale2(sv, kUp - e_run);
                     }
-                    if (lt < BK / 16) reinterpret_cast<int*>(inf + C::THERE)[lt] = page >= 0;
-                    fl_mbar_arrive(&i_full[n % C::NI]);
-                    {
-                        const uint32_t to = opaque(s_k + st * C::TBYTES + place);
-#pragma unroll
-                        for (int i = 0; i < C::NP; i++) put(at_pass(to, i), kr[i]);
-                    }
-                    fl_fence_proxy_async();
-                    fl_mbar_arrive(&k_full[st]);
-                    page = page1;
-                    if (key0 + BK < key_end) {
-                        fetch(kr, c.k, page, key0 + BK);
-                        fetch_scales(page, key0 + BK);
-                    }
-                    if (!(ok = wait_warp(&v_empty[st], par, abort))) break;
-                    const uint32_t to = opaque(s_v + st * C::TBYTES + place);
-                    if (partial) {
-                        bool any = false;
-#pragma unroll
-                        for (int i = 0; i < C::NP; i++) {
-                            const int kk = i * KPP + k_in;
-                            /* as for F16: 0x7f is e4m3's NaN */
-                            uint32_t bits = (inf + C::BAD)[kk] ? 0xffffu : 0u;
-                            if (key0 + kk < see_lo || key0 + kk >= see_hi) {
-                                vr[i] = make_uint4(0, 0, 0, 0);
-                            } else if (KV == FL_KV_F8) {
-                                uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-                                for (int x = 0; x < 16; x++) {
-                                    const uint32_t byte = (w[x >> 2] >> (8 * (x & 3))) & 0x7fu;
-                                    if (byte == 0x7fu) {
-                                        bits |= 1u << x;
-                                        w[x >> 2] &= ~(0xffu << (8 * (x & 3)));
-                                    }
-                                }
-                                vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                            any |= bits != 0;
-                            reinterpret_cast<uint16_t*>(inf + C::ODD)[kk * (HD / 16) + pc] = (uint16_t)bits;
-                        }
-                        any = __any_sync(0xffffffffu, any);
-                        if (lane == 0) evs[4 + (warp & 3)] = any;
-                    }
-#pragma unroll
-                    for (int i = 0; i < C::NP; i++) put(at_pass(to, i), vr[i]);
-                    fl_fence_proxy_async();
-                    fl_mbar_arrive(&v_full[st]);
                 }
+                fl_mbar_arrive(&i_full[n % C::NI]);
+                fl_cp_async_wait<1>();
+                widen(kd);
+                fl_fence_proxy_async();
+                fl_mbar_arrive(&k_full[st]);
+                if (key0 + BK < key_end) {
+                    if (!(ok = wait_warp(&k_empty[st1], (((n + 1) / ST) & 1) ^ 1, abort))) break;
+                    bring(s_k + st1 * C::TBYTES, c.k, page, key0 + BK);
+                    fetch_scales(page, key0 + BK);
+                } else {
+                    fl_cp_async_commit();
+                }
+                fl_cp_async_wait<1>();
+                if (partial) {
+                    /* keys that no row sees become zero; NaN and infinities that only some rows see are noted and left out */
+                    bool any = false;
+#pragma unroll 1
+                    for (int i = 0; i < C::NP; i++) {
+                        const int kk = i * KPP + k_in;
+                        const uint32_t at = at_pass(vd + place, i);
+                        uint32_t bits = 0;
+                        if (key0 + kk < see_lo || key0 + kk >= see_hi) {
+                            sts16(at, 0, 0, 0, 0);
+                        } else if (KV != FL_KV_Q8) {
+                            const uint4 v = lds16(at);
+                            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int x = 0; x < 4; x++) {
+                                uint32_t b, gone;
+                                if (KV == FL_KV_F16) {
+                                    b = odd_bits(w[x]);
+                                    gone = (b & 1 ? 0xffffu : 0u) | (b & 2 ? 0xffff0000u : 0u);
+                                } else { /* 0x7f is e4m3's NaN */
+                                    gone = __vcmpeq4(w[x] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                                    b = (gone & 1u) | (gone >> 8 & 1u) << 1 | (gone >> 16 & 1u) << 2 | (gone >> 24 & 1u) << 3;
+                                }
+                                bits |= b << (x * (16 / C::ES / 4));
+                                w[x] &= ~gone;
+                            }
+                            if (bits) sts16(at, w[0], w[1], w[2], w[3]);
+                        }
+                        if (C::ES == 1) {
+                            if ((inf + C::BAD)[kk]) bits = 0xffffu;
+                            reinterpret_cast<uint16_t*>(inf + C::ODD)[kk * (HD / 16) + pc] = (uint16_t)bits;
+                        } else {
+                            (inf + C::ODD)[kk * (HD / 8) + pc] = (uint8_t)bits;
+                        }
+                        any |= bits != 0;
+                    }
+                    any = __any_sync(0xffffffffu, any);
+                    if (lane == 0) evs[4 + (warp & 3)] = any;
+                }
+                widen(vd);
+                fl_fence_proxy_async();
+                fl_mbar_arrive(&v_full[st]);
             }
+            fl_cp_async_wait<0>();
         }
     } else if (warp >= kSoftWarps + kLoadWarps) {
         /* ── the tensor core ── */
@@ -799,16 +746,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 if (lane == 0) fl_mbar_arrive(q_full);
             }
             const int row = q * 128 + r;
-            const float fr = s_fr[row];
-            const int pos = row < seg.it.rows ? seg.sw.first + fl_div_grp(a, seg.it.f0 + row) : -1;
+            s_pos[row] = row < seg.it.rows ? seg.sw.first + fl_div_grp(a, seg.it.f0 + row) : -1;
+            /* what a row and its segment are stays in shared memory: the scores need the registers */
             float m = -INFINITY, l = 0.0f;
             int e_acc = -100; /* exponent of the values' scales that O counts in */
             bool any_nan = false;
-            const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max, len = seg.sw.len, tile_lo = seg.it.tile0 + seg.j0;
             for (int j = 0; j < tiles; j++, n++) {
                 const int st = n % ST, buf = NQ == 1 ? j & 1 : q;
                 const uint8_t* inf = info + (n % C::NI) * C::INFO;
-                const int key0 = (tile_lo + j) * BK;
+                const int key0 = (seg.it.tile0 + seg.j0 + j) * BK;
                 if (!live) continue;
                 if (!(ok = wait_warp(&i_full[n % C::NI], (n / C::NI) & 1, abort))) break;
                 if (!(ok = wait_warp(&s_full[buf], (s_ph >> buf) & 1, abort))) break;
@@ -822,10 +768,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 bool holes = false;
 #pragma unroll
                 for (int x = 0; x < BK / 16; x++) holes |= !there[x];
-                const bool masked = holes || key0 + BK - 1 > pos_min || key0 + BK > len || pos_max - key0 >= win;
+                const bool masked = holes || key0 + BK - 1 > seg.it.pos_min || key0 + BK > seg.sw.len || seg.it.pos_max - key0 >= win;
                 /* columns the row sees: (c_lo, c_hi] */
-                const int c_hi = min(pos, len - 1) - key0, c_lo = pos - key0 < win ? -1 : pos - key0 - win;
+                const int pos = s_pos[row];
+                const int c_hi = min(pos, seg.sw.len - 1) - key0, c_lo = pos - key0 < win ? -1 : pos - key0 - win;
 
+                const float fr = s_fr[row];
                 float x[BK];
 #pragma unroll
                 for (int b = 0; b < BK; b += 32) tmem_ld32(s_at + b, x + b);
@@ -890,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     }
                 }
                 bool odd = false;
-                if (key0 + BK - 1 > pos_min || pos_max - key0 >= win) {
+                if (key0 + BK - 1 > seg.it.pos_min || seg.it.pos_max - key0 >= win) {
                     /* what bringing up V found is there once V is */
                     if (!(ok = wait_warp(&v_full[st], (n / ST) & 1, abort))) break;
                     odd = evs[4] | evs[5] | evs[6] | evs[7];
