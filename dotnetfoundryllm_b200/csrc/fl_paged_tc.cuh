@@ -30,6 +30,7 @@
 #define FL_PAGED_TC_CUH
 
 #include <climits>
+#include <type_traits>
 
 #include "fl_paged.cuh"
 
@@ -47,7 +48,7 @@ constexpr int kMinUnits = 2;
 constexpr float kLazy = 8.0f; /* log2 of how far weights may exceed 1 */
 constexpr int kUp = 6;        /* weights are stored times 2^kUp: below 2^15 with the values' scales below 2 */
 
-template <int KV, int HD, bool SPLIT>
+template <int KV, int HD, bool SPLIT, bool BF16>
 struct Cfg {
     static constexpr int ES = KV == FL_KV_F16 ? 2 : 1;
     static constexpr int ROW = HD * ES;
@@ -60,9 +61,12 @@ struct Cfg {
     static constexpr int TBYTES = BK * HD * 2;             /* K or V of a key tile */
     static constexpr int PIECES = ROW / 16;                /* 16-byte pieces of a key */
     static constexpr int NP = BK * PIECES / (kLoadWarps * 32); /* pieces of a thread */
-    /* of a key tile: scales of K and V, exponents and findings of the loading warps, mapped 16-key groups, values' flags:
-     * a byte a key, a bit an element */
-    static constexpr int EVS = BK * 8, THERE = EVS + 32, BAD = THERE + 32, ODD = BAD + BK, INFO = ODD + BK * HD / 8;
+    /* bf16 rows: V's scales multiply weights that are already fp16, two at a time; each is rounded to 11 bits once more,
+     * far below the output's 8, for half the shared-memory reads (its lanes' reads of a scale are what bounds 8 bits) */
+    static constexpr bool HALF_V = ES == 1 && BF16;
+    /* of a key tile: scales of K, of V; (exponent that V's count in, mapped 16-key groups); exponents and findings of the
+     * loading warps; values' flags: a byte a key, a bit an element */
+    static constexpr int HEAD = BK * 8, EVS = HEAD + 16, BAD = EVS + 32, ODD = BAD + BK, INFO = ODD + BK * HD / 8;
     static constexpr int NI = 4;                           /* infos in flight: more than stages, so that they need no release */
     static constexpr int SMEM = QBYTES + STAGES * 2 * TBYTES + NI * INFO + 1024 + 512;
     /* tensor memory columns: two sets of scores (weights over them), the outputs, the weights' low halves */
@@ -334,7 +338,7 @@ template <typename T, int KV, int HD, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, const FlPagedAttn a)
 {
     constexpr bool SPLIT = sizeof(T) == 4;
-    using C = Cfg<KV, HD, SPLIT>;
+    using C = Cfg<KV, HD, SPLIT, std::is_same<T, __nv_bfloat16>::value>;
     constexpr int NQ = C::NQ, BK = C::BK, ST = C::STAGES, RT = C::RT;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = fl_smem_u32(smem_raw), s_base = (raw + 1023u) & ~1023u;
@@ -350,7 +354,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     __shared__ uint32_t s_scan[kThreads / 32], s_at;
     __shared__ int s_seq;
     __shared__ float s_fr[RT];                    /* score units of a row's scaled q */
-    __shared__ int s_pos[RT];
     __shared__ Segments<RT, BK> s_seg[4];
     __shared__ uint32_t s_nan[RT][HD / 32]; /* elements of a row's output that are NaN */
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -537,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
                 if (!(ok = wait_warp(&v_empty[st], ((n / ST) & 1) ^ 1, abort))) break;
                 bring(vd, c.v, page, key0);
-                if (lt < BK / 16) reinterpret_cast<int*>(inf + C::THERE)[lt] = (unsigned)page < (unsigned)c.n_pages;
+                const uint32_t mapped = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)c.n_pages) & ((1u << (BK / 16)) - 1);
                 page = pages_of(key0 + BK);
                 if constexpr (C::ES == 1) {
                     /* scales; the largest finite one's exponent, so far in this segment */
@@ -553,9 +556,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     e_run = max(e_run, max(max(evs[0], evs[1]), max(evs[2], evs[3])));
                     if (lt < BK) {
                         reinterpret_cast<float*>(inf)[lt] = sk;
-                        reinterpret_cast<float*>(inf)[BK + lt] = fl_scale2(sv, kUp - e_run);
+                        const float v = fl_scale2(sv, kUp - e_run);
+                        if (C::HALF_V)
+                            reinterpret_cast<__half*>(inf + BK * 4)[lt] = __float2half_rn(v);
+                        else
+                            reinterpret_cast<float*>(inf)[BK + lt] = v;
                     }
                 }
+                if (lt == 0) *reinterpret_cast<int2*>(inf + C::HEAD) = make_int2(e_run, (int)mapped);
                 fl_mbar_arrive(&i_full[n % C::NI]);
                 fl_cp_async_wait<1>();
                 widen(kd);
@@ -746,15 +754,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 if (lane == 0) fl_mbar_arrive(q_full);
             }
             const int row = q * 128 + r;
-            s_pos[row] = row < seg.it.rows ? seg.sw.first + fl_div_grp(a, seg.it.f0 + row) : -1;
-            /* what a row and its segment are stays in shared memory: the scores need the registers */
+            const float fr = s_fr[row];
+            const int pos = row < seg.it.rows ? seg.sw.first + fl_div_grp(a, seg.it.f0 + row) : -1;
+            const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max, len = seg.sw.len;
+            int key0 = (seg.it.tile0 + seg.j0) * BK;
             float m = -INFINITY, l = 0.0f;
             int e_acc = -100; /* exponent of the values' scales that O counts in */
             bool any_nan = false;
-            for (int j = 0; j < tiles; j++, n++) {
+            for (int j = 0; j < tiles; j++, n++, key0 += BK) {
                 const int st = n % ST, buf = NQ == 1 ? j & 1 : q;
                 const uint8_t* inf = info + (n % C::NI) * C::INFO;
-                const int key0 = (seg.it.tile0 + seg.j0 + j) * BK;
                 if (!live) continue;
                 if (!(ok = wait_warp(&i_full[n % C::NI], (n / C::NI) & 1, abort))) break;
                 if (!(ok = wait_warp(&s_full[buf], (s_ph >> buf) & 1, abort))) break;
@@ -764,16 +773,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 const float* sk = reinterpret_cast<const float*>(inf);
                 const float* sv = sk + BK;
                 const int* evs = reinterpret_cast<const int*>(inf + C::EVS);
-                const int* there = reinterpret_cast<const int*>(inf + C::THERE);
-                bool holes = false;
-#pragma unroll
-                for (int x = 0; x < BK / 16; x++) holes |= !there[x];
-                const bool masked = holes || key0 + BK - 1 > seg.it.pos_min || key0 + BK > seg.sw.len || seg.it.pos_max - key0 >= win;
+                const int2 head = *reinterpret_cast<const int2*>(inf + C::HEAD);
+                const bool holes = head.y != (1 << (BK / 16)) - 1;
+                const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
                 /* columns the row sees: (c_lo, c_hi] */
-                const int pos = s_pos[row];
-                const int c_hi = min(pos, seg.sw.len - 1) - key0, c_lo = pos - key0 < win ? -1 : pos - key0 - win;
-
-                const float fr = s_fr[row];
+                const int c_hi = min(pos, len - 1) - key0, c_lo = pos - key0 < win ? -1 : pos - key0 - win;
                 float x[BK];
 #pragma unroll
                 for (int b = 0; b < BK; b += 32) tmem_ld32(s_at + b, x + b);
@@ -787,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         mul2(x[z + 2], x[z + 3], k4.z, k4.w);
                     }
                 }
-                if (masked) {
+                if (holes || partial || key0 + BK > len) {
                     const uint32_t seen = (uint32_t)max(0, c_hi - c_lo);
 #pragma unroll
                     for (int z = 0; z < BK; z++)
@@ -795,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     if (holes) {
 #pragma unroll
                         for (int z = 0; z < BK; z += 16)
-                            if (!there[z / 16]) {
+                            if (!(head.y >> (z / 16) & 1)) {
 #pragma unroll
                                 for (int y = 0; y < 16; y++) x[z + y] = -INFINITY;
                             }
@@ -830,15 +834,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     moved = true;
                 }
                 if (C::ES == 1) {
-                    const int e = max(e_acc, max(max(evs[0], evs[1]), max(evs[2], evs[3])));
-                    if (e > e_acc) {
-                        f *= fl_ex2((float)(e_acc - e));
-                        e_acc = e;
+                    if (head.x > e_acc) {
+                        f *= fl_ex2((float)(e_acc - head.x));
+                        e_acc = head.x;
                         moved = true;
                     }
                 }
                 bool odd = false;
-                if (key0 + BK - 1 > seg.it.pos_min || seg.it.pos_max - key0 >= win) {
+                if (partial) {
                     /* what bringing up V found is there once V is */
                     if (!(ok = wait_warp(&v_full[st], (n / ST) & 1, abort))) break;
                     odd = evs[4] | evs[5] | evs[6] | evs[7];
@@ -867,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     for (int w = 0; w < HD / 32; w++) {
                         uint32_t b = any_nan ? s_nan[row][w] : 0u;
                         for (int k = max(0, c_lo + 1); k < min(BK, c_hi + 1); k++)
-                            if (there[k >> 4]) b |= bits[k * (HD / 32) + w];
+                            if (head.y >> (k >> 4) & 1) b |= bits[k * (HD / 32) + w];
                         s_nan[row][w] = b;
                     }
                     any_nan = true;
@@ -887,7 +890,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         for (int y = 0; y < 4; y++) x[z + y] = fl_ex2(x[z + y]);
                         add2(sum[0], sum[1], x[z], x[z + 1]);
                         add2(sum[2], sum[3], x[z + 2], x[z + 3]);
-                        if (C::ES == 1) {
+                        if (C::ES == 1 && !C::HALF_V) {
                             const float4 v4 = *reinterpret_cast<const float4*>(sv + z);
                             mul2(x[z], x[z + 1], v4.x, v4.y);
                             mul2(x[z + 2], x[z + 3], v4.z, v4.w);
@@ -895,6 +898,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         const int i = (z - b) / 2;
                         hi[i] = fl_pack_half2(x[z], x[z + 1]);
                         hi[i + 1] = fl_pack_half2(x[z + 2], x[z + 3]);
+                        if (C::HALF_V && (z & 4)) { /* eight scales at a time */
+                            const uint4 v8 = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(sv) + z - 4);
+                            const uint32_t w[4] = {v8.x, v8.y, v8.z, v8.w};
+#pragma unroll
+                            for (int y = 0; y < 4; y++) {
+                                uint32_t& h = hi[i - 2 + y];
+                                h = fl_half2_bits(__hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&w[y])));
+                            }
+                        }
                         if (SPLIT) {
                             const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
                             const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[i + 1]));
@@ -965,7 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
 template <typename T, int KV, int HD>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const FlPaged c, const FlPagedAttn a)
 {
-    using C = Cfg<KV, HD, sizeof(T) == 4>;
+    using C = Cfg<KV, HD, sizeof(T) == 4, std::is_same<T, __nv_bfloat16>::value>;
     const int64_t pair = ((int64_t)blockIdx.x * 128 + threadIdx.x) >> 5;
     if (pair >= (int64_t)c.n_rows * a.n_heads) return;
     const int row = (int)((uint32_t)pair / (uint32_t)a.n_heads), h = (int)(pair - (int64_t)row * a.n_heads);
@@ -994,7 +1006,7 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const FlPaged c, const
 template <typename T, int KV, int HD>
 cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
 {
-    using C = Cfg<KV, HD, sizeof(T) == 4>;
+    using C = Cfg<KV, HD, sizeof(T) == 4, std::is_same<T, __nv_bfloat16>::value>;
     static int sms[64] = {}; /* SMs of a device, once its kernel is configured */
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
