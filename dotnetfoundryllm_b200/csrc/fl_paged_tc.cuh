@@ -8,9 +8,12 @@
  * schedule that all items' tiles form, so every SM has the same number of
  * tiles; an item cut by a range's end leaves (o, m, l) in the workspace for a
  * second kernel.  Per key tile:
- *  - 4 warps bring K and V from their pages to shared memory as fp16 in the
- *    128-byte swizzled layout (8-bit elements are exact in fp16; scales stay
- *    beside them).  V is read by the tensor core with the keys as its inner
+ *  - 3 warps copy K and V from their pages to shared memory (cp.async); 4 more
+ *    make them fp16 in the 128-byte swizzled layout, in place (8-bit elements
+ *    are exact in fp16; scales stay beside them), and hand them to the tensor
+ *    core.  The two are apart because the fence that hands over waits for every
+ *    copy its thread has under way: with both in one thread no tile's copies
+ *    overlapped another's work (2048 rows at 16384 keys: 828 us).  V is read by the tensor core with the keys as its inner
  *    dimension, straight from rows of 64 elements (an MN-major operand), so
  *    nothing is transposed.
  *  - one lane issues S = Q K^T into tensor memory and, once the weights are
@@ -37,9 +40,9 @@
 namespace flpt {
 namespace {
 
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kThreads = (kSoftWarps + kLoadWarps + 4) * 32; /* the last four: one issues to the tensor core */
-/* registers of a softmax, loading and issuing thread, from the launch's 128 each: a softmax thread holds a row of scores */
+constexpr int kSoftWarps = 8, kLoadWarps = 4, kCopyWarps = 3;
+constexpr int kThreads = (kSoftWarps + kLoadWarps + 4) * 32; /* the last four: one issues to the tensor core, three copy */
+/* registers of a softmax, widening and issuing thread, from the launch's 128 each: a softmax thread holds a row of scores */
 constexpr int kSoftRegs = 200, kLoadRegs = 64, kIssueRegs = 48;
 static_assert(kSoftWarps * kSoftRegs + kLoadWarps * kLoadRegs + 4 * kIssueRegs <= kThreads / 32 * 128, "register file");
 constexpr int kMaxCtas = 148;
@@ -60,7 +63,13 @@ struct Cfg {
     static constexpr int QBYTES = NQ * QTILE * (SPLIT ? 2 : 1);
     static constexpr int TBYTES = BK * HD * 2;             /* K or V of a key tile */
     static constexpr int PIECES = ROW / 16;                /* 16-byte pieces of a key */
-    static constexpr int NP = BK * PIECES / (kLoadWarps * 32); /* pieces of a thread */
+    static constexpr int NP = BK * PIECES / (kLoadWarps * 32); /* pieces of a widening thread */
+    /* a piece's place in its tile; an 8-bit one arrives in the first of the two chunks that it widens to */
+    static __device__ __forceinline__ uint32_t place(int key, int pc)
+    {
+        return ES == 2 ? (pc >> 3) * (BK * 128) + key * 128 + (((pc & 7) ^ (key & 7)) << 4)
+                       : (pc >> 2) * (BK * 128) + key * 128 + (((pc & 3) * 2 ^ (key & 7)) << 4);
+    }
     /* bf16 rows: V's scales multiply weights that are already fp16, two at a time; each is rounded to 11 bits once more,
      * far below the output's 8, for half the shared-memory reads (its lanes' reads of a scale are what bounds 8 bits) */
     static constexpr bool HALF_V = ES == 1 && BF16;
@@ -214,6 +223,11 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint
         "r"(a), "r"(b), "r"(id), "r"((uint32_t)accum), "r"(kDescHigh)
         : "memory");
 }
+/* Arrives on `bar` once this thread's copies so far have landed. */
+__device__ __forceinline__ void copies_arrive(uint64_t* bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(fl_smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void umma_commit(uint64_t* bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(fl_smem_u32(bar))
@@ -258,8 +272,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-/* The four warps of a role. */
-__device__ __forceinline__ void role_sync(int role) { asm volatile("bar.sync %0, 128;" ::"r"(role + 1) : "memory"); }
+/* The warps of a role. */
+__device__ __forceinline__ void role_sync(int role)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(role + 1), "r"(role == 4 ? kCopyWarps * 32 : 128) : "memory");
+}
 
 /* Bounded wait (~2 s); false once it ran out or another role of the CTA gave up. */
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort)
@@ -348,13 +365,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     uint64_t* bars = reinterpret_cast<uint64_t*>(info + C::NI * C::INFO);
     uint64_t *k_full = bars, *k_empty = bars + 3, *v_full = bars + 6, *v_empty = bars + 9;
     uint64_t *s_full = bars + 12, *p_full = bars + 14, *q_full = bars + 16, *o_full = bars + 17, *pv_done = bars + 18,
-             *done = bars + 19, *i_full = bars + 20;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 24);
+             *done = bars + 19, *i_full = bars + 20,
+             *k_raw = bars + 24, *v_raw = bars + 27;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 30);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_holder + 1);
     __shared__ uint32_t s_scan[kThreads / 32], s_at;
     __shared__ int s_seq;
     __shared__ float s_fr[RT];                    /* score units of a row's scaled q */
-    __shared__ Segments<RT, BK> s_seg[4];
+    __shared__ Segments<RT, BK> s_seg[5];
     __shared__ uint32_t s_nan[RT][HD / 32]; /* elements of a row's output that are NaN */
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const FlAttnSpace ws = fl_attn_space(a.workspace, c.n_seqs, kMaxCtas, RT, HD);
@@ -366,6 +384,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             fl_mbar_init(&v_full[s], kLoadWarps * 32);
             fl_mbar_init(&k_empty[s], 1);
             fl_mbar_init(&v_empty[s], 1);
+            /* each copying thread arrives twice: by its copies, and for its own stores */
+            fl_mbar_init(&k_raw[s], 2 * kCopyWarps * 32);
+            fl_mbar_init(&v_raw[s], 2 * kCopyWarps * 32);
         }
         for (int i = 0; i < C::NI; i++) fl_mbar_init(&i_full[i], kLoadWarps * 32);
         for (int b = 0; b < 2; b++) {
@@ -431,119 +452,70 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     __syncthreads();
     const uint32_t tmem = *tmem_holder;
     const bool work = s_seq >= 0;
-    /* roles: softmax of row tile 0, of row tile 1, loading, issuing */
-    Segments<RT, BK>& seg = s_seg[warp >> 2];
-    if (work && (tid & 127) == 0) {
+    /* roles: softmax of row tile 0, of row tile 1, widening, issuing, copying */
+    const int role = warp <= kSoftWarps + kLoadWarps ? warp >> 2 : 4;
+    const bool leads = role == 4 ? tid == kThreads - kCopyWarps * 32 : (tid & 127) == 0;
+    Segments<RT, BK>& seg = s_seg[role];
+    if (work && leads) {
         seg.at = range_lo;
         seg.end = range_hi;
         seg.seq_at = s_at;
         seg.enter(c, a, s_seq);
     }
-    /* the next segment, for all four warps of a role */
+    /* the next segment, for all warps of a role */
     auto next_segment = [&]() {
-        role_sync(warp >> 2);
-        if ((tid & 127) == 0) seg.more = seg.next(c, a);
-        role_sync(warp >> 2);
+        role_sync(role);
+        if (leads) seg.more = seg.next(c, a);
+        role_sync(role);
         return seg.more;
     };
     const int win = a.window > 0 ? a.window : INT_MAX;
 
     if (!work) {
     } else if (warp >= kSoftWarps && warp < kSoftWarps + kLoadWarps) {
-        /* ── K and V ── */
+        /* ── K and V as the tensor core reads them ── */
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         const int lt = tid - kSoftWarps * 32;
         constexpr int KPP = kLoadWarps * 32 / C::PIECES; /* keys that a pass of the warps covers */
         /* 8-bit: eight lanes hold four pieces of two keys, whose stores of 32 bytes a piece then lie on different banks */
         const int pc = C::ES == 2 ? lt % C::PIECES : (lane & 3) | ((lane >> 3) * 4) % C::PIECES;
         const int k_in = C::ES == 2 ? lt / C::PIECES : (warp & 3) * (32 / C::PIECES) + (lane >> 3) * 4 / C::PIECES * 2 + ((lane >> 2) & 1);
-        /* a piece's place in its tile in the first pass; pass i lies i * KPP rows on, with the same swizzle where KPP is a
-         * multiple of 8, with the other half's chunks in odd passes where it is 4.  An 8-bit piece arrives in the first of
-         * the two chunks that it widens to, which its own thread writes: no other storage, no barrier. */
-        const uint32_t place = C::ES == 2 ? (pc >> 3) * (BK * 128) + k_in * 128 + (((pc & 7) ^ (k_in & 7)) << 4)
-                                          : (pc >> 2) * (BK * 128) + k_in * 128 + (((pc & 3) * 2 ^ (k_in & 7)) << 4);
-        auto at_pass = [&](uint32_t base, int i) { return (KPP == 4 && (i & 1) ? base ^ 64u : base) + i * (KPP * 128); };
-        static_assert(KPP % 8 == 0 || KPP == 4, "swizzle of a pass");
         int n = 0; /* key tiles so far */
         bool ok = true;
         while (ok && next_segment()) {
-            const int32_t* table = c.table + (size_t)seg.seq * c.cols;
-            const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max, head = seg.head;
+            const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max;
             const int see_lo = a.window > 0 ? max(0, pos_min + 1 - a.window) : 0; /* keys that some row sees */
             const int see_hi = min(seg.sw.len, pos_max + 1);
             const int key_end = (seg.it.tile0 + seg.j1) * BK;
-            int key0 = (seg.it.tile0 + seg.j0) * BK, e_run = -100;
-            auto pages_of = [&](int k0) { /* lane i: the table's entry for keys k0 + 16 i .., unchecked so that nothing waits for it */
-                int page = -1;
-                const int key = k0 + 16 * lane;
-                if (lane < BK / 16 && key < see_hi && k0 < key_end) page = __ldg(table + (key >> c.page_shift));
-                return page;
-            };
-            auto row_of = [&](int page, int kk) -> int64_t { /* cache row of key key0 + kk; -1: unmapped */
-                const int pg = __shfl_sync(0xffffffffu, page, kk >> 4);
-                if ((unsigned)pg >= (unsigned)c.n_pages) return -1;
-                /* tiles start at a multiple of BK, so a key's place in its page depends on kk and the tile alone */
-                return (((int64_t)pg * c.n_kv + head) << c.page_shift);
-            };
-            const int in_page = (1 << c.page_shift) - 1;
-            auto bring = [&](uint32_t base, const void* src, int pg, int k0) { /* one copy group of this thread */
-                const uint32_t to = opaque(base + place);
-#pragma unroll
-                for (int i = 0; i < C::NP; i++) {
-                    const int kk = i * KPP + k_in;
-                    const int64_t row = row_of(pg, kk);
-                    if (row >= 0)
-                        fl_cp_async16(at_pass(to, i), static_cast<const uint8_t*>(src) +
-                                                          (row + ((k0 + kk) & in_page)) * C::ROW + pc * 16);
-                    else
-                        sts16(at_pass(to, i), 0, 0, 0, 0);
-                }
-                fl_cp_async_commit();
-            };
-            float sk = 0.0f, sv = 0.0f; /* 8 bits: scales of key lt */
-            auto fetch_scales = [&](int pg, int k0) {
+            int e_run = -100;
+            auto widen = [&](uint32_t base) { /* this thread's pieces of a tile, each in the two chunks that are its own */
                 if constexpr (C::ES == 1) {
-                    const int key = k0 + (lt & (BK - 1));
-                    const int64_t row = row_of(pg, lt & (BK - 1));
-                    sk = sv = 0.0f;
-                    if (lt < BK && row >= 0) {
-                        sk = __ldg(c.k_scale + row + (key & in_page));
-                        if (key >= see_lo && key < see_hi) sv = __ldg(c.v_scale + row + (key & in_page));
-                    }
-                }
-            };
-            auto widen = [&](uint32_t base) { /* this thread's pieces of a tile, in place */
-                if constexpr (C::ES == 1) {
-                    const uint32_t to = opaque(base + place);
+                    const uint32_t to = opaque(base + C::place(k_in, pc));
 #pragma unroll
                     for (int i = 0; i < C::NP; i++) {
-                        const uint4 r = lds16(at_pass(to, i));
+                        const uint32_t at = to + i * (KPP * 128);
+                        const uint4 r = lds16(at);
                         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
                         uint32_t h[8];
 #pragma unroll
                         for (int x = 0; x < 4; x++) fl_widen4<KV>(w[x], h[2 * x], h[2 * x + 1]);
-                        sts16(at_pass(to, i), h[0], h[1], h[2], h[3]);
-                        sts16(at_pass(to, i) ^ 16u, h[4], h[5], h[6], h[7]);
+                        sts16(at, h[0], h[1], h[2], h[3]);
+                        sts16(at ^ 16u, h[4], h[5], h[6], h[7]);
                     }
                 }
             };
-            /* K of a tile is under way before V of the tile ahead of it has come */
-            int page = pages_of(key0);
-            if (!(ok = wait_warp(&k_empty[n % ST], ((n / ST) & 1) ^ 1, abort))) break;
-            bring(s_k + (n % ST) * C::TBYTES, c.k, page, key0);
-            fetch_scales(page, key0);
-            for (; key0 < key_end; key0 += BK, n++) {
-                const int st = n % ST, st1 = (n + 1) % ST;
+            for (int key0 = (seg.it.tile0 + seg.j0) * BK; key0 < key_end; key0 += BK, n++) {
+                const int st = n % ST;
+                const uint32_t par = (n / ST) & 1;
                 uint8_t* inf = info + (n % C::NI) * C::INFO;
                 int* evs = reinterpret_cast<int*>(inf + C::EVS);
-                const uint32_t kd = s_k + st * C::TBYTES, vd = s_v + st * C::TBYTES;
+                const uint32_t vd = s_v + st * C::TBYTES;
                 const bool partial = key0 + BK - 1 > pos_min || pos_max - key0 >= win;
-                if (!(ok = wait_warp(&v_empty[st], ((n / ST) & 1) ^ 1, abort))) break;
-                bring(vd, c.v, page, key0);
-                const uint32_t mapped = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)c.n_pages) & ((1u << (BK / 16)) - 1);
-                page = pages_of(key0 + BK);
+                if (!(ok = wait_warp(&k_raw[st], par, abort))) break;
                 if constexpr (C::ES == 1) {
-                    /* scales; the largest finite one's exponent, so far in this segment */
+                    /* V's scales; the largest finite one's exponent, so far in this segment */
+                    float sv = 0.0f;
+                    if (lt < BK && key0 + lt >= see_lo && key0 + lt < see_hi) sv = reinterpret_cast<const float*>(inf)[BK + lt];
                     const uint32_t b = __float_as_uint(sv) & 0x7fffffffu;
                     const uint32_t top = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
                     if (lane == 0) evs[warp & 3] = (int)(top >> 23) - 127;
@@ -555,7 +527,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     role_sync(2);
                     e_run = max(e_run, max(max(evs[0], evs[1]), max(evs[2], evs[3])));
                     if (lt < BK) {
-                        reinterpret_cast<float*>(inf)[lt] = sk;
                         const float v = fl_scale2(sv, kUp - e_run);
                         if (C::HALF_V)
                             reinterpret_cast<__half*>(inf + BK * 4)[lt] = __float2half_rn(v);
@@ -563,27 +534,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                             reinterpret_cast<float*>(inf)[BK + lt] = v;
                     }
                 }
-                if (lt == 0) *reinterpret_cast<int2*>(inf + C::HEAD) = make_int2(e_run, (int)mapped);
+                if (lt == 0) *reinterpret_cast<int*>(inf + C::HEAD) = e_run;
                 fl_mbar_arrive(&i_full[n % C::NI]);
-                fl_cp_async_wait<1>();
-                widen(kd);
+                widen(s_k + st * C::TBYTES);
                 fl_fence_proxy_async();
                 fl_mbar_arrive(&k_full[st]);
-                if (key0 + BK < key_end) {
-                    if (!(ok = wait_warp(&k_empty[st1], (((n + 1) / ST) & 1) ^ 1, abort))) break;
-                    bring(s_k + st1 * C::TBYTES, c.k, page, key0 + BK);
-                    fetch_scales(page, key0 + BK);
-                } else {
-                    fl_cp_async_commit();
-                }
-                fl_cp_async_wait<1>();
+                if (!(ok = wait_warp(&v_raw[st], par, abort))) break;
                 if (partial) {
                     /* keys that no row sees become zero; NaN and infinities that only some rows see are noted and left out */
                     bool any = false;
 #pragma unroll 1
                     for (int i = 0; i < C::NP; i++) {
                         const int kk = i * KPP + k_in;
-                        const uint32_t at = at_pass(vd + place, i);
+                        const uint32_t at = vd + C::place(kk, pc);
                         uint32_t bits = 0;
                         if (key0 + kk < see_lo || key0 + kk >= see_hi) {
                             sts16(at, 0, 0, 0, 0);
@@ -620,12 +583,79 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 fl_fence_proxy_async();
                 fl_mbar_arrive(&v_full[st]);
             }
-            fl_cp_async_wait<0>();
         }
     } else if (warp >= kSoftWarps + kLoadWarps) {
         /* ── the tensor core ── */
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        if (warp == kSoftWarps + kLoadWarps && lane == 0) {
+        if (role == 4) {
+            /* ── copies out of the pages ── */
+            constexpr int KI = 32 / C::PIECES; /* keys that a warp copies at once */
+            const int ct = tid - (kThreads - kCopyWarps * 32);
+            const uint32_t mine = C::place(lane / C::PIECES, lane % C::PIECES);
+            int n = 0;
+            bool ok = true;
+            while (ok && next_segment()) {
+                const int32_t* table = c.table + (size_t)seg.seq * c.cols;
+                const int see_hi = min(seg.sw.len, seg.it.pos_max + 1), head = seg.head, in_page = (1 << c.page_shift) - 1;
+                const int key_end = (seg.it.tile0 + seg.j1) * BK;
+                auto pages_of = [&](int k0) { /* lane i: the table's entry for keys k0 + 16 i .., unchecked so that nothing waits for it */
+                    int page = -1;
+                    const int key = k0 + 16 * lane;
+                    if (lane < BK / 16 && key < see_hi && k0 < key_end) page = __ldg(table + (key >> c.page_shift));
+                    return page;
+                };
+                int key0 = (seg.it.tile0 + seg.j0) * BK, next_page = pages_of(key0);
+                for (; key0 < key_end; key0 += BK, n++) {
+                    const int page = next_page, st = n % ST;
+                    const uint32_t par = ((n / ST) & 1) ^ 1;
+                    uint8_t* inf = info + (n % C::NI) * C::INFO;
+                    next_page = pages_of(key0 + BK);
+                    auto row_of = [&](int kk) -> int64_t { /* cache row of key key0 + kk; -1: unmapped */
+                        const int pg = __shfl_sync(0xffffffffu, page, kk >> 4);
+                        if ((unsigned)pg >= (unsigned)c.n_pages) return -1;
+                        return (((int64_t)pg * c.n_kv + head) << c.page_shift) + ((key0 + kk) & in_page);
+                    };
+                    auto bring = [&](uint32_t base, const void* src, uint64_t* bar) {
+                        /* a warp takes 16 keys, which lie in one page and in a row, lane by lane 16 bytes */
+                        for (int grp = ct >> 5; grp < BK / 16; grp += kCopyWarps) {
+                            const int64_t row = row_of(grp * 16);
+                            const uint8_t* from = static_cast<const uint8_t*>(src) + row * C::ROW + lane * 16;
+                            const uint32_t to = base + grp * (16 * 128);
+                            if (row >= 0) {
+#pragma unroll
+                                for (int i = 0; i < C::PIECES / 2; i++)
+                                    fl_cp_async16(to + i * KI * 128 + (mine ^ ((i * KI & 7) << 4)), from + i * 512);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < C::PIECES / 2; i++)
+                                    sts16(to + i * KI * 128 + (mine ^ ((i * KI & 7) << 4)), 0, 0, 0, 0);
+                            }
+                        }
+                        copies_arrive(bar);
+                        fl_mbar_arrive(bar);
+                    };
+                    if (!(ok = wait_warp(&k_empty[st], par, abort))) break;
+                    const uint32_t mapped = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)c.n_pages) & ((1u << (BK / 16)) - 1);
+                    if (ct == 0) *reinterpret_cast<int*>(inf + C::HEAD + 4) = (int)mapped;
+                    if constexpr (C::ES == 1) { /* scales of K, then of V: four a piece */
+                        const int kk = (ct & (BK / 4 - 1)) * 4;
+                        const int64_t row = row_of(kk);
+                        if (ct < BK / 2) {
+                            const bool v = ct >= BK / 4;
+                            const uint32_t to = fl_smem_u32(inf) + (v ? BK * 4 : 0) + kk * 4;
+                            if (row >= 0)
+                                fl_cp_async16(to, (v ? c.v_scale : c.k_scale) + row);
+                            else
+                                sts16(to, 0, 0, 0, 0);
+                        }
+                    }
+                    bring(s_k + st * C::TBYTES, c.k, &k_raw[st]);
+                    if (!(ok = wait_warp(&v_empty[st], par, abort))) break;
+                    bring(s_v + st * C::TBYTES, c.v, &v_raw[st]);
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else if (lane == 0) {
             constexpr uint32_t id_s = idesc(BK, false), id_o = idesc(HD, true);
             constexpr int H = SPLIT ? 2 : 1;
             bool ok = true;
