@@ -492,15 +492,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 if constexpr (C::ES == 1) {
                     const uint32_t to = opaque(base + C::place(k_in, pc));
 #pragma unroll
-                    for (int i = 0; i < C::NP; i++) {
-                        const uint32_t at = to + i * (KPP * 128);
-                        const uint4 r = lds16(at);
-                        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-                        uint32_t h[8];
+                    for (int i0 = 0; i0 < C::NP; i0 += 4) { /* four loads under way at once */
+                        uint4 r[4];
 #pragma unroll
-                        for (int x = 0; x < 4; x++) fl_widen4<KV>(w[x], h[2 * x], h[2 * x + 1]);
-                        sts16(at, h[0], h[1], h[2], h[3]);
-                        sts16(at ^ 16u, h[4], h[5], h[6], h[7]);
+                        for (int i = 0; i < 4; i++) r[i] = lds16(to + (i0 + i) * (KPP * 128));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t at = to + (i0 + i) * (KPP * 128), w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+                            uint32_t h[8];
+#pragma unroll
+                            for (int x = 0; x < 4; x++) fl_widen4<KV>(w[x], h[2 * x], h[2 * x + 1]);
+                            sts16(at, h[0], h[1], h[2], h[3]);
+                            sts16(at ^ 16u, h[4], h[5], h[6], h[7]);
+                        }
                     }
                 }
             };
