@@ -2,9 +2,21 @@
  * fl_verify.cu — verification of drafted tokens against the target's logits
  * (fl_verify_device).
  *
- * rows: one CTA per logits row takes its maximum (first index) and the sum of
- * exp((l - max) / T).  draw: one CTA per sequence walks the acceptance tests,
- * then draws from the row that stopped it by cumulative sums in 64 bits.
+ * Bound by reading the logits once; four kernels, each started early and
+ * waiting for the one before (programmatic dependent launch), over chunks of
+ * 4096 vocabulary entries so that one sequence and sixty-four both spread over
+ * the SMs:
+ *  rows: per (row, chunk) the maximum with its first index and the sum of
+ *        exp((l - max) / T), exponentials in fp32;
+ *  stop: per (sequence, chunk) first the acceptance tests, which every chunk's
+ *        CTA repeats (a few rows of a few partials), then the chunk's sum over
+ *        the row that the sequence stopped at, exponentials and sums in 64 bits;
+ *  rest: the same for max(p - q, 0), which needs that sum's total first;
+ *  draw: per sequence the chunk that the draw falls into, and the entry in it.
+ * The draw compares with cumulative sums of up to 2^24 entries, whose borders
+ * lie closer than fp32 resolves, hence the 64 bits there; the acceptance tests
+ * compare single probabilities, for which the fp32 exponentials' 2^-22 is
+ * enough.
  */
 #include <cfloat>
 #include <climits>
@@ -13,199 +25,452 @@
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 128, kChunk = 4096;
+constexpr int kDrawThreads = 512;
 
-struct RowStat {
-    double z;   /* sum of exp((l - m) / T) */
-    float m;    /* largest logit; -infinity: everything masked */
-    int32_t best;
+struct RowPart { /* of a row's chunk */
+    float m, z;
+    int32_t best, pad;
+};
+struct Decision { /* of a sequence */
+    double z;    /* sum of exp((l - m) / T) over the row, exponentials in fp32 */
+    float m;
+    int32_t row; /* that it stopped at; -1: no rows */
+    int32_t rej, best;
+};
+struct Sums { /* of a chunk of that row */
+    double e;    /* of exp((l - m) / T), less the draft's where it was rejected and certain */
+    double rest; /* of max(exp - q Z, 0) */
 };
 
-/* NaN is masked, +infinity is the largest finite value. */
-template <typename T>
-__device__ __forceinline__ float logit(const T* row, int x)
+struct Space {
+    RowPart* part;   /* [n_rows][chunks] */
+    Decision* dec;   /* [n_seqs] */
+    Sums* sums;      /* [n_seqs][chunks] */
+};
+__host__ __device__ __forceinline__ int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
+__host__ __device__ __forceinline__ Space space(void* p, int n_rows, int n_seqs, int vocab, size_t* bytes = nullptr)
 {
-    const float l = fl_to_float(row[x]);
-    return l != l ? -INFINITY : fminf(l, FLT_MAX);
-}
-
-__device__ __forceinline__ double weight(float l, float m, double inv_t) { return exp(((double)l - (double)m) * inv_t); }
-
-__device__ __forceinline__ double block_sum(double v, double* scratch)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < kThreads / 32; w++) s += scratch[w];
+    uint8_t* b = static_cast<uint8_t*>(p);
+    const size_t c = (size_t)chunks_of(vocab);
+    Space s;
+    size_t at = 0;
+    s.part = reinterpret_cast<RowPart*>(b);
+    at += fl_align256(n_rows * c * sizeof(RowPart));
+    s.dec = reinterpret_cast<Decision*>(b + at);
+    at += fl_align256(n_seqs * sizeof(Decision));
+    s.sums = reinterpret_cast<Sums*>(b + at);
+    at += n_seqs * c * sizeof(Sums);
+    if (bytes) *bytes = at;
     return s;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g, RowStat* __restrict__ stat)
+/* NaN is masked, +infinity is the largest finite value. */
+__device__ __forceinline__ float clean(float l) { return l != l ? -INFINITY : fminf(l, FLT_MAX); }
+
+/* e^x for x <= 0 in 64 bits: x = n ln 2 + y, |y| <= 0.35; the Taylor series of
+ * e^y to y^11 (the next term is below 2^-47), times 2^n. */
+__device__ __forceinline__ double exp64(double x)
 {
-    __shared__ double s_d[kThreads / 32];
-    __shared__ float s_m[kThreads / 32];
+    if (!(x > -708.0)) return 0.0; /* below 2^-1021 */
+    const double n = rint(x * 1.4426950408889634);
+    const double y = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, x)); /* ln 2 in two parts */
+    double p = 1.0 / 39916800.0;
+    p = fma(p, y, 1.0 / 3628800.0);
+    p = fma(p, y, 1.0 / 362880.0);
+    p = fma(p, y, 1.0 / 40320.0);
+    p = fma(p, y, 1.0 / 5040.0);
+    p = fma(p, y, 1.0 / 720.0);
+    p = fma(p, y, 1.0 / 120.0);
+    p = fma(p, y, 1.0 / 24.0);
+    p = fma(p, y, 1.0 / 6.0);
+    p = fma(p, y, 0.5);
+    p = fma(p, y, 1.0);
+    p = fma(p, y, 1.0);
+    return __hiloint2double(__double2hiint(p) + ((int)n << 20), __double2loint(p)); /* p in [0.7, 1.42] */
+}
+
+__device__ __forceinline__ double weight(float l, float m, double inv_t) { return exp64(((double)l - (double)m) * inv_t); }
+
+__device__ __forceinline__ double warp_sum(double v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+/* f(x, l) for this thread's entries of [x0, x1), ascending: ends that are not
+ * 16-byte aligned one by one, the rest 16 bytes at a time. */
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void each(const T* __restrict__ row, int x0, int x1, F f)
+{
+    constexpr int VE = 16 / sizeof(T);
+    const int n = x1 - x0;
+    const int head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(row + x0) % 16) % 16 / sizeof(T)));
+    const int nv = (n - head) / VE;
+    if ((int)threadIdx.x < head) f(x0 + threadIdx.x, clean(fl_to_float(row[x0 + threadIdx.x])));
+    const uint4* v = reinterpret_cast<const uint4*>(row + x0 + head);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += NT) {
+        const uint4 u = __ldg(v + i);
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int j = 0; j < VE; j++) f(x0 + head + i * VE + j, clean(fl_to_float(e[j])));
+    }
+    const int tail = x0 + head + nv * VE + threadIdx.x;
+    if (tail < x1) f(tail, clean(fl_to_float(row[tail])));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g)
+{
+    constexpr int VE = 16 / sizeof(T), NV = kChunk / (VE * kThreads);
+    __shared__ float s_m[kThreads / 32], s_z[kThreads / 32];
     __shared__ int s_i[kThreads / 32];
-    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int chunk = blockIdx.y, row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    fl_pdl_trigger();
     const int s = fl_row_seq(g.row_start, g.n_seqs, row);
     if (s < 0) return;
     const T* l = static_cast<const T*>(g.logits) + row * g.logits_stride;
-    float m = -INFINITY;
-    int best = 0;
-    for (int x = threadIdx.x; x < g.vocab; x += kThreads) {
-        const float v = logit(l, x);
-        if (v > m) m = v, best = x;
+    const int x0 = chunk * kChunk, x1 = min(g.vocab, x0 + kChunk), n = x1 - x0;
+    const float t = g.temperature[s];
+    /* the thread's entries, all loaded before any is used: an unaligned start, then 16 bytes at a time, then the end */
+    const int head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(l + x0) % 16) % 16 / sizeof(T)));
+    const int nv = (n - head) / VE, tail = head + nv * VE + threadIdx.x;
+    const uint4* v = reinterpret_cast<const uint4*>(l + x0 + head);
+    uint4 u[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int at = threadIdx.x + i * kThreads;
+        if (at < nv) u[i] = __ldg(v + at);
     }
+    float ends[2] = {-INFINITY, -INFINITY};
+    if ((int)threadIdx.x < head) ends[0] = clean(fl_to_float(l[x0 + threadIdx.x]));
+    if (tail < n) ends[1] = clean(fl_to_float(l[x0 + tail]));
+    float m = ends[0];
+    int best = m > -INFINITY ? x0 + (int)threadIdx.x : INT_MAX;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int at = threadIdx.x + i * kThreads;
+        if (at >= nv) continue;
+        const T* e = reinterpret_cast<const T*>(&u[i]);
+#pragma unroll
+        for (int j = 0; j < VE; j++) {
+            const float x = clean(fl_to_float(e[j]));
+            if (x > m) m = x, best = x0 + head + at * VE + j;
+        }
+    }
+    if (ends[1] > m) m = ends[1], best = x0 + tail;
+    const float mine = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
         const int b2 = __shfl_xor_sync(0xffffffffu, best, o);
         if (m2 > m || (m2 == m && b2 < best)) m = m2, best = b2;
     }
-    if (lane == 0) s_m[warp] = m, s_i[warp] = best;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 32; w++)
-        if (s_m[w] > m || (s_m[w] == m && s_i[w] < best)) m = s_m[w], best = s_i[w];
-    const float t = g.temperature[s];
-    double z = 0.0;
-    if (t > 0.0f && m > -INFINITY) {
-        const double inv_t = 1.0 / (double)t;
-        for (int x = threadIdx.x; x < g.vocab; x += kThreads) z += weight(logit(l, x), m, inv_t);
+    /* the thread's sum against its own maximum, brought to the warp's, then to the chunk's */
+    float z = 0.0f;
+    if (t > 0.0f && mine > -INFINITY) {
+        const float c = fminf(1.44269504f / t, FLT_MAX);
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if ((int)threadIdx.x + i * kThreads >= nv) continue;
+            const T* e = reinterpret_cast<const T*>(&u[i]);
+#pragma unroll
+            for (int j = 0; j < VE; j++) z += fl_ex2((clean(fl_to_float(e[j])) - mine) * c);
+        }
+        z += fl_ex2((ends[0] - mine) * c) + fl_ex2((ends[1] - mine) * c);
+        z *= fl_ex2((mine - m) * c);
     }
-    z = block_sum(z, s_d);
-    if (threadIdx.x == 0) stat[row] = RowStat{z, m, best};
+    z = fl_warp_sum(z);
+    if (lane == 0) s_m[warp] = m, s_z[warp] = z, s_i[warp] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float M = -INFINITY, Z = 0.0f;
+        int B = INT_MAX;
+        for (int w = 0; w < kThreads / 32; w++)
+            if (s_m[w] > M || (s_m[w] == M && s_i[w] < B)) M = s_m[w], B = s_i[w];
+        for (int w = 0; w < kThreads / 32; w++)
+            if (s_m[w] > -INFINITY && t > 0.0f) Z += s_z[w] * fl_ex2((s_m[w] - M) * fminf(1.44269504f / t, FLT_MAX));
+        const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
+        sp.part[(size_t)row * gridDim.y + chunk] = RowPart{M, Z, B, 0};
+    }
+}
+
+/* A row's maximum, first index of it and sum, by a warp from its chunks. */
+__device__ __forceinline__ Decision merge_row(const RowPart* __restrict__ part, int chunks, double inv_t)
+{
+    const int lane = threadIdx.x & 31;
+    Decision d{0.0, -INFINITY, 0, 0, INT_MAX};
+    for (int c = lane; c < chunks; c += 32) {
+        const RowPart p = part[c];
+        if (p.m > d.m || (p.m == d.m && p.best < d.best)) d.m = p.m, d.best = p.best;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, d.m, o);
+        const int b2 = __shfl_xor_sync(0xffffffffu, d.best, o);
+        if (m2 > d.m || (m2 == d.m && b2 < d.best)) d.m = m2, d.best = b2;
+    }
+    for (int c = lane; c < chunks; c += 32) {
+        const RowPart p = part[c];
+        if (p.m > -INFINITY) d.z += (double)p.z * exp64(((double)p.m - (double)d.m) * inv_t);
+    }
+    d.z = warp_sum(d.z);
+    return d;
+}
+
+__device__ __forceinline__ float prob(const float* q, int x)
+{
+    const float v = q[x];
+    return v > 0.0f ? v : 0.0f;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_draw_kernel(const FlVerify g, const RowStat* __restrict__ stat)
+__global__ void __launch_bounds__(kThreads) verify_stop_kernel(const FlVerify g)
 {
+    __shared__ Decision s_row[kThreads / 32];
+    __shared__ int s_ok[kThreads / 32];
     __shared__ double s_d[kThreads / 32];
-    __shared__ double s_run[2];
-    __shared__ int s_stop, s_rej, s_tok;
-    const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int chunk = blockIdx.y, s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = gridDim.y;
+    fl_pdl_trigger();
+    const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
     const int r0 = max(g.row_start[s], 0), r1 = min(g.row_start[s + 1], g.n_rows);
-    if (r1 <= r0) {
-        if (threadIdx.x == 0) g.accepted[s] = 0;
-        return;
-    }
     const float t = g.temperature[s];
     const bool greedy = !(t > 0.0f);
     const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
-    if (warp == 0) {
-        int stop = r1 - 1, rej = 0;
-        for (int base = r0; base < r1 - 1; base += 32) {
-            const int row = base + lane;
-            bool ok = true;
-            if (row < r1 - 1) {
-                const RowStat st = stat[row];
-                const int d = g.draft[row];
-                ok = d >= 0 && d < g.vocab && st.m > -INFINITY;
-                if (ok && greedy) {
-                    ok = d == st.best;
-                } else if (ok) {
-                    float q = 1.0f;
-                    if (g.probs) q = g.probs[row * g.probs_stride + d];
-                    q = q > 0.0f ? q : 0.0f;
-                    const float l = logit(static_cast<const T*>(g.logits) + row * g.logits_stride, d);
-                    ok = (double)g.u_accept[row] * (double)q * st.z < weight(l, st.m, inv_t);
-                }
-            }
-            const unsigned bad = __ballot_sync(0xffffffffu, !ok);
-            if (bad) {
-                stop = base + __ffs(bad) - 1;
-                rej = 1;
-                break;
-            }
-        }
-        if (lane == 0) s_stop = stop, s_rej = rej, s_tok = -1;
+    fl_pdl_wait();
+    if (r1 <= r0) {
+        if (chunk == 0 && threadIdx.x == 0) sp.dec[s] = Decision{0.0, -INFINITY, -1, 0, -1};
+        return;
     }
-    __syncthreads();
-    const int r = s_stop;
-    const bool rej = s_rej;
-    const RowStat st = stat[r];
-    int token = -1;
-    if (st.m > -INFINITY) {
-        if (greedy) {
-            token = st.best;
-        } else {
-            const T* l = static_cast<const T*>(g.logits) + r * g.logits_stride;
-            const float* q = g.probs ? g.probs + r * g.probs_stride : nullptr;
-            const int d = g.draft[r];
-            bool rest = rej;
-            auto w_of = [&](int x) -> double {
-                const double e = weight(logit(l, x), st.m, inv_t);
-                if (!rest) return e;
-                if (!q) return x == d ? 0.0 : e;
-                const float qx = q[x] > 0.0f ? q[x] : 0.0f;
-                return fmax(e - (double)qx * st.z, 0.0);
-            };
-            double total = 0.0;
-            for (int x = threadIdx.x; x < g.vocab; x += kThreads) total += w_of(x);
-            total = block_sum(total, s_d);
-            if (rest && !(total > 0.0)) {
-                rest = false;
-                total = st.z;
+    /* the acceptance tests, a row per warp, in order */
+    Decision d{};
+    for (int base = r0;; base += kThreads / 32) {
+        const int row = base + warp;
+        if (row < r1) {
+            Decision w = merge_row(sp.part + (size_t)row * chunks, chunks, inv_t);
+            w.row = row;
+            bool ok = false;
+            if (row < r1 - 1) {
+                const int x = g.draft[row];
+                if (x >= 0 && x < g.vocab && w.m > -INFINITY) {
+                    if (greedy) {
+                        ok = x == w.best;
+                    } else {
+                        const float q = g.probs ? prob(g.probs + row * g.probs_stride, x) : 1.0f;
+                        const float l = clean(fl_to_float(static_cast<const T*>(g.logits)[row * g.logits_stride + x]));
+                        ok = (double)g.u_accept[row] * (double)q * w.z < weight(l, w.m, inv_t);
+                    }
+                }
+                w.rej = 1;
             }
-            const double goal = (double)g.u_sample[s] * total;
-            double run = 0.0;
-            int last = -1; /* the last x with weight, should rounding leave the goal above every sum */
-            for (int base = 0; base < g.vocab; base += kThreads) {
-                const int x = base + threadIdx.x;
-                const double w = x < g.vocab ? w_of(x) : 0.0;
-                double c = w; /* inclusive scan over the block */
+            if (lane == 0) s_row[warp] = w, s_ok[warp] = ok;
+        } else if (lane == 0) {
+            s_ok[warp] = 1; /* behind the last row, which always stops */
+        }
+        __syncthreads();
+        int stop = 0;
+        while (stop < kThreads / 32 && s_ok[stop]) stop++;
+        if (stop < kThreads / 32) {
+            d = s_row[stop];
+            break;
+        }
+        __syncthreads();
+    }
+    if (chunk == 0 && threadIdx.x == 0) sp.dec[s] = d;
+    if (greedy || !(d.m > -INFINITY)) return;
+    /* the chunk's sum over the row that it stopped at */
+    const int skip = d.rej && !g.probs ? g.draft[d.row] : -1;
+    double sum = 0.0;
+    each<T, kThreads>(static_cast<const T*>(g.logits) + d.row * g.logits_stride, chunk * kChunk,
+                      min(g.vocab, (chunk + 1) * kChunk), [&](int x, float l) {
+                          if (x != skip) sum += weight(l, d.m, inv_t);
+                      });
+    sum = warp_sum(sum);
+    if (lane == 0) s_d[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kThreads / 32; w++) sum += s_d[w];
+        sp.sums[(size_t)s * chunks + chunk].e = sum;
+    }
+}
+
+/* The sum of a sequence's chunks, the same in every thread of a warp. */
+template <bool REST>
+__device__ __forceinline__ double total_of(const Sums* __restrict__ s, int chunks)
+{
+    double v = 0.0;
+    for (int c = threadIdx.x & 31; c < chunks; c += 32) v += REST ? s[c].rest : s[c].e;
+    return warp_sum(v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_rest_kernel(const FlVerify g)
+{
+    __shared__ double s_d[kThreads / 32];
+    const int chunk = blockIdx.y, s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = gridDim.y;
+    fl_pdl_trigger();
+    const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
+    const float t = g.temperature[s];
+    fl_pdl_wait();
+    const Decision d = sp.dec[s];
+    if (d.row < 0 || !d.rej || !(t > 0.0f) || !(d.m > -INFINITY)) return;
+    const double inv_t = 1.0 / (double)t, z = total_of<false>(sp.sums + (size_t)s * chunks, chunks);
+    const float* q = g.probs + d.row * g.probs_stride;
+    double sum = 0.0;
+    each<T, kThreads>(static_cast<const T*>(g.logits) + d.row * g.logits_stride, chunk * kChunk,
+                      min(g.vocab, (chunk + 1) * kChunk),
+                      [&](int x, float l) { sum += fmax(weight(l, d.m, inv_t) - (double)prob(q, x) * z, 0.0); });
+    sum = warp_sum(sum);
+    if (lane == 0) s_d[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kThreads / 32; w++) sum += s_d[w];
+        sp.sums[(size_t)s * chunks + chunk].rest = sum;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const FlVerify g)
+{
+    constexpr int PER = kChunk / kDrawThreads; /* consecutive entries of a thread */
+    __shared__ double s_w[kDrawThreads / 32];
+    __shared__ double s_before;
+    __shared__ int s_chunk, s_tok, s_last;
+    const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = chunks_of(g.vocab);
+    const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
+    const int r0 = max(g.row_start[s], 0), r1 = min(g.row_start[s + 1], g.n_rows);
+    const float t = g.temperature[s];
+    fl_pdl_wait();
+    const Decision d = sp.dec[s];
+    if (d.row < 0) {
+        if (threadIdx.x == 0) g.accepted[s] = 0;
+        return;
+    }
+    int token = -1;
+    const Sums* sums = sp.sums + (size_t)s * chunks;
+    const bool greedy = !(t > 0.0f);
+    const double z = greedy || !(d.m > -INFINITY) ? 0.0 : total_of<false>(sums, chunks);
+    const int skip = d.rej && !g.probs ? g.draft[d.row] : -1;
+    if (d.m > -INFINITY && greedy) {
+        token = d.best;
+    } else if (d.m > -INFINITY && !(z > 0.0)) {
+        token = skip; /* the draft is all of p */
+    } else if (d.m > -INFINITY) {
+        const double inv_t = 1.0 / (double)t;
+        bool rest = d.rej && g.probs;
+        double all = z;
+        if (rest) {
+            all = total_of<true>(sums, chunks);
+            if (!(all > 0.0)) rest = false, all = z; /* nothing is left of p - q: p itself */
+        }
+        const double goal = (double)g.u_sample[s] * all;
+        /* the first chunk whose running sum exceeds the goal; else the last that has any weight */
+        if (warp == 0) {
+            double before = 0.0, before_last = 0.0;
+            int hit = -1, last = 0;
+            for (int c0 = 0; c0 < chunks && hit < 0; c0 += 32) {
+                const int c = c0 + lane;
+                const double w = c < chunks ? (rest ? sums[c].rest : sums[c].e) : 0.0;
+                double run = w;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const double u = __shfl_up_sync(0xffffffffu, c, o);
-                    if (lane >= o) c += u;
+                    const double u = __shfl_up_sync(0xffffffffu, run, o);
+                    if (lane >= o) run += u;
                 }
-                __syncthreads();
-                if (lane == 31) s_d[warp] = c;
-                __syncthreads();
-                double before = run, all = run;
-                for (int i = 0; i < kThreads / 32; i++) {
-                    if (i < warp) before += s_d[i];
-                    all += s_d[i];
+                const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
+                const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && before + run > goal);
+                const int at = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : -1;
+                if (at >= 0) {
+                    last = c0 + at;
+                    before_last = before + __shfl_sync(0xffffffffu, run - w, at);
                 }
-                if (w > 0.0) last = x;
-                const bool hit = w > 0.0 && before + c > goal;
-                if (threadIdx.x == 0) s_tok = INT_MAX;
-                __syncthreads();
-                if (hit) atomicMin(&s_tok, x);
-                __syncthreads();
-                if (s_tok != INT_MAX) break;
-                run = all;
+                if (over) hit = last;
+                before += __shfl_sync(0xffffffffu, run, 31);
             }
-            __syncthreads();
-            if (s_tok == INT_MAX) {
-                __syncthreads();
-                if (threadIdx.x == 0) s_tok = -1;
-                __syncthreads();
-                if (last >= 0) atomicMax(&s_tok, last);
-                __syncthreads();
-            }
-            token = s_tok;
+            if (lane == 0) s_chunk = last, s_before = before_last, s_tok = INT_MAX, s_last = -1;
         }
+        __syncthreads();
+        /* the entry in it */
+        const int x0 = s_chunk * kChunk + threadIdx.x * PER;
+        const T* l = static_cast<const T*>(g.logits) + d.row * g.logits_stride;
+        const float* q = rest ? g.probs + d.row * g.probs_stride : nullptr;
+        double w[PER], mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int x = x0 + i;
+            w[i] = 0.0;
+            if (x < g.vocab && x != skip) {
+                w[i] = weight(clean(fl_to_float(l[x])), d.m, inv_t);
+                if (rest) w[i] = fmax(w[i] - (double)prob(q, x) * z, 0.0);
+            }
+            mine += w[i];
+        }
+        double run = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double u = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += u;
+        }
+        if (lane == 31) s_w[warp] = run;
+        __syncthreads();
+        double c = s_before + run - mine;
+        for (int i = 0; i < warp; i++) c += s_w[i];
+        int last = -1, hit = INT_MAX;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            c += w[i];
+            if (w[i] > 0.0) {
+                last = x0 + i;
+                if (c > goal && hit == INT_MAX) hit = x0 + i;
+            }
+        }
+        if (hit != INT_MAX) atomicMin(&s_tok, hit);
+        if (last >= 0) atomicMax(&s_last, last);
+        __syncthreads();
+        token = s_tok != INT_MAX ? s_tok : s_last;
     }
-    for (int row = r0 + threadIdx.x; row < r1; row += kThreads)
-        g.tokens[row] = row < r ? g.draft[row] : row == r ? token : -1;
-    if (threadIdx.x == 0) g.accepted[s] = r - r0;
+    for (int row = r0 + threadIdx.x; row < r1; row += kDrawThreads)
+        g.tokens[row] = row < d.row ? g.draft[row] : row == d.row ? token : -1;
+    if (threadIdx.x == 0) g.accepted[s] = d.row - r0;
+}
+
+template <typename K>
+cudaError_t after(K kernel, dim3 grid, int threads, const FlVerify& v, cudaStream_t st)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, v);
 }
 
 template <typename T>
 cudaError_t launch(const FlVerify& v, cudaStream_t st)
 {
-    RowStat* stat = static_cast<RowStat*>(v.workspace);
-    if (v.n_rows > 0) verify_rows_kernel<T><<<v.n_rows, kThreads, 0, st>>>(v, stat);
-    verify_draw_kernel<T><<<v.n_seqs, kThreads, 0, st>>>(v, stat);
-    return cudaGetLastError();
+    const unsigned chunks = chunks_of(v.vocab);
+    if (v.n_rows > 0) verify_rows_kernel<T><<<dim3(v.n_rows, chunks), kThreads, 0, st>>>(v);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = after(verify_stop_kernel<T>, dim3(v.n_seqs, chunks), kThreads, v, st);
+    if (e == cudaSuccess && v.probs) e = after(verify_rest_kernel<T>, dim3(v.n_seqs, chunks), kThreads, v, st);
+    if (e == cudaSuccess) e = after(verify_draw_kernel<T>, dim3(v.n_seqs), kDrawThreads, v, st);
+    return e;
 }
 
 } // namespace
 
-size_t fl_verify_workspace_bytes(int n_rows, int, int) { return (size_t)n_rows * sizeof(RowStat); }
+size_t fl_verify_workspace_bytes(int n_rows, int n_seqs, int vocab)
+{
+    size_t bytes;
+    space(nullptr, n_rows, n_seqs, vocab, &bytes);
+    return bytes;
+}
 
 cudaError_t fl_launch_verify(const FlVerify& v, cudaStream_t st)
 {
