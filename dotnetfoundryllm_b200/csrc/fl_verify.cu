@@ -25,7 +25,7 @@
 
 namespace {
 
-constexpr int kThreads = 128, kChunk = 4096;
+constexpr int kThreads = 128, kStopThreads = 256, kChunk = 4096;
 constexpr int kDrawThreads = 512;
 
 struct RowPart { /* of a row's chunk */
@@ -68,29 +68,45 @@ __host__ __device__ __forceinline__ Space space(void* p, int n_rows, int n_seqs,
 /* NaN is masked, +infinity is the largest finite value. */
 __device__ __forceinline__ float clean(float l) { return l != l ? -INFINITY : fminf(l, FLT_MAX); }
 
-/* e^x for x <= 0 in 64 bits: x = n ln 2 + y, |y| <= 0.35; the Taylor series of
- * e^y to y^11 (the next term is below 2^-47), times 2^n. */
-__device__ __forceinline__ double exp64(double x)
+/* e^((l - m) / T) in 64 bits as 2^(k / 32), k = (l - m) A with A = 32 log2(e) /
+ * T: k = n + f, |f| <= 1/2; 2^(n / 32) from a table of 32 and an exponent,
+ * 2^(f / 32) by its Taylor series to f^5 (the next term is below 2^-48). */
+constexpr double kL = 0.69314718055994531 / 32.0;
+struct Exp64 {
+    double a, m;
+    const double* table; /* 2^(i / 32), i < 32, in shared memory */
+    __device__ __forceinline__ double operator()(float l) const
+    {
+        const double k = ((double)l - m) * a;
+        if (!(k > -32.0 * 1021.0)) return 0.0; /* below 2^-1021; masked */
+        const double magic = 6755399441055744.0; /* 1.5 * 2^52: the sum's low word is k rounded */
+        const double t = k + magic;
+        const int n = __double2loint(t);
+        const double f = k - (t - magic);
+        double p = kL * kL * kL * kL * kL / 120.0;
+        p = fma(p, f, kL * kL * kL * kL / 24.0);
+        p = fma(p, f, kL * kL * kL / 6.0);
+        p = fma(p, f, kL * kL / 2.0);
+        p = fma(p, f, kL);
+        p = fma(p, f, 1.0);
+        p *= table[n & 31];
+        return __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+    }
+};
+__device__ __forceinline__ void exp64_table(double* table)
 {
-    if (!(x > -708.0)) return 0.0; /* below 2^-1021 */
-    const double n = rint(x * 1.4426950408889634);
-    const double y = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, x)); /* ln 2 in two parts */
-    double p = 1.0 / 39916800.0;
-    p = fma(p, y, 1.0 / 3628800.0);
-    p = fma(p, y, 1.0 / 362880.0);
-    p = fma(p, y, 1.0 / 40320.0);
-    p = fma(p, y, 1.0 / 5040.0);
-    p = fma(p, y, 1.0 / 720.0);
-    p = fma(p, y, 1.0 / 120.0);
-    p = fma(p, y, 1.0 / 24.0);
-    p = fma(p, y, 1.0 / 6.0);
-    p = fma(p, y, 0.5);
-    p = fma(p, y, 1.0);
-    p = fma(p, y, 1.0);
-    return __hiloint2double(__double2hiint(p) + ((int)n << 20), __double2loint(p)); /* p in [0.7, 1.42] */
+    if (threadIdx.x < 32) {
+        /* e^(i kL) by its series; i kL < 0.7 */
+        const double y = kL * (double)(int)threadIdx.x;
+        double p = 1.0;
+        for (int i = 20; i > 0; i--) p = fma(p, y / (double)i, 1.0);
+        table[threadIdx.x] = p;
+    }
 }
-
-__device__ __forceinline__ double weight(float l, float m, double inv_t) { return exp64(((double)l - (double)m) * inv_t); }
+__device__ __forceinline__ Exp64 exp64_of(float m, float t, const double* table)
+{
+    return Exp64{46.166241308446828 / (double)t, (double)m, table}; /* 32 log2(e) */
+}
 
 __device__ __forceinline__ double warp_sum(double v)
 {
@@ -99,26 +115,83 @@ __device__ __forceinline__ double warp_sum(double v)
     return v;
 }
 
-/* f(x, l) for this thread's entries of [x0, x1), ascending: ends that are not
- * 16-byte aligned one by one, the rest 16 bytes at a time. */
-template <typename T, int NT, typename F>
+/* f(x, n, l): n of this thread's entries of [x0, x1) from x on, by threads and
+ * ascending: ends that are not 16-byte aligned one by one, the rest 16 bytes
+ * at a time. */
+template <int NT, typename T, typename F>
 __device__ __forceinline__ void each(const T* __restrict__ row, int x0, int x1, F f)
 {
     constexpr int VE = 16 / sizeof(T);
     const int n = x1 - x0;
     const int head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(row + x0) % 16) % 16 / sizeof(T)));
     const int nv = (n - head) / VE;
-    if ((int)threadIdx.x < head) f(x0 + threadIdx.x, clean(fl_to_float(row[x0 + threadIdx.x])));
+    float l[VE] = {};
+    if ((int)threadIdx.x < head) {
+        l[0] = clean(fl_to_float(row[x0 + threadIdx.x]));
+        f(x0 + (int)threadIdx.x, 1, l);
+    }
     const uint4* v = reinterpret_cast<const uint4*>(row + x0 + head);
-#pragma unroll 4
+#pragma unroll 2
     for (int i = threadIdx.x; i < nv; i += NT) {
         const uint4 u = __ldg(v + i);
         const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-        for (int j = 0; j < VE; j++) f(x0 + head + i * VE + j, clean(fl_to_float(e[j])));
+        for (int j = 0; j < VE; j++) l[j] = clean(fl_to_float(e[j]));
+        f(x0 + head + i * VE, VE, l);
     }
     const int tail = x0 + head + nv * VE + threadIdx.x;
-    if (tail < x1) f(tail, clean(fl_to_float(row[tail])));
+    if (tail < x1) {
+        l[0] = clean(fl_to_float(row[tail]));
+        f(tail, 1, l);
+    }
+}
+
+/* The larger of each half's two numbers, NaN losing. */
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __half)
+{
+    const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __nv_bfloat16)
+{
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ float2 halves(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+__device__ __forceinline__ float2 halves(uint32_t w, __nv_bfloat16)
+{
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+/* The largest of 16 bytes of logits, NaN losing; -infinity if there is no other. */
+template <typename T>
+__device__ __forceinline__ float max_of(const uint4& u)
+{
+    if constexpr (sizeof(T) == 4) {
+        return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                     fmaxf(__uint_as_float(u.z), fmaxf(__uint_as_float(u.w), -INFINITY)));
+    } else {
+        const float2 f = halves(max2(max2(u.x, u.y, T()), max2(u.z, u.w, T()), T()), T());
+        return fmaxf(fmaxf(f.x, f.y), -INFINITY);
+    }
+}
+
+/* Sum of 2^((l - m) c) over 16 bytes of logits; NaN if one is NaN or infinite. */
+template <typename T>
+__device__ __forceinline__ float sum_of(const uint4& u, float m, float c)
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    float z = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            z += fl_ex2((__uint_as_float(w[i]) - m) * c);
+        } else {
+            const float2 f = halves(w[i], T());
+            z += fl_ex2((f.x - m) * c) + fl_ex2((f.y - m) * c);
+        }
+    }
+    return z;
 }
 
 template <typename T>
@@ -129,11 +202,8 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g)
     __shared__ int s_i[kThreads / 32];
     const int chunk = blockIdx.y, row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     fl_pdl_trigger();
-    const int s = fl_row_seq(g.row_start, g.n_seqs, row);
-    if (s < 0) return;
     const T* l = static_cast<const T*>(g.logits) + row * g.logits_stride;
     const int x0 = chunk * kChunk, x1 = min(g.vocab, x0 + kChunk), n = x1 - x0;
-    const float t = g.temperature[s];
     /* the thread's entries, all loaded before any is used: an unaligned start, then 16 bytes at a time, then the end */
     const int head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(l + x0) % 16) % 16 / sizeof(T)));
     const int nv = (n - head) / VE, tail = head + nv * VE + threadIdx.x;
@@ -147,37 +217,47 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g)
     float ends[2] = {-INFINITY, -INFINITY};
     if ((int)threadIdx.x < head) ends[0] = clean(fl_to_float(l[x0 + threadIdx.x]));
     if (tail < n) ends[1] = clean(fl_to_float(l[x0 + tail]));
-    float m = ends[0];
-    int best = m > -INFINITY ? x0 + (int)threadIdx.x : INT_MAX;
+    const int s = fl_row_seq(g.row_start, g.n_seqs, row); /* while they are under way */
+    if (s < 0) return;
+    const float t = g.temperature[s];
+    float m = fmaxf(ends[0], ends[1]);
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int at = threadIdx.x + i * kThreads;
-        if (at >= nv) continue;
-        const T* e = reinterpret_cast<const T*>(&u[i]);
-#pragma unroll
-        for (int j = 0; j < VE; j++) {
-            const float x = clean(fl_to_float(e[j]));
-            if (x > m) m = x, best = x0 + head + at * VE + j;
-        }
-    }
-    if (ends[1] > m) m = ends[1], best = x0 + tail;
+    for (int i = 0; i < NV; i++)
+        if ((int)threadIdx.x + i * kThreads < nv) m = fmaxf(m, max_of<T>(u[i]));
+    m = fminf(m, FLT_MAX);
     const float mine = m;
+    m = fl_warp_max(m);
+    /* its first index, looked for by the threads that hold it */
+    int best = INT_MAX;
+    if (mine == m && m > -INFINITY) {
+        if (ends[1] == m) best = x0 + tail;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-        const int b2 = __shfl_xor_sync(0xffffffffu, best, o);
-        if (m2 > m || (m2 == m && b2 < best)) m = m2, best = b2;
+        for (int i = NV - 1; i >= 0; i--) {
+            if ((int)threadIdx.x + i * kThreads >= nv) continue;
+            const T* e = reinterpret_cast<const T*>(&u[i]);
+#pragma unroll
+            for (int j = VE - 1; j >= 0; j--)
+                if (clean(fl_to_float(e[j])) == m) best = x0 + head + (threadIdx.x + i * kThreads) * VE + j;
+        }
+        if (ends[0] == m) best = x0 + threadIdx.x;
     }
+    best = __reduce_min_sync(0xffffffffu, best);
     /* the thread's sum against its own maximum, brought to the warp's, then to the chunk's */
     float z = 0.0f;
     if (t > 0.0f && mine > -INFINITY) {
         const float c = fminf(1.44269504f / t, FLT_MAX);
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            if ((int)threadIdx.x + i * kThreads >= nv) continue;
-            const T* e = reinterpret_cast<const T*>(&u[i]);
+        for (int i = 0; i < NV; i++)
+            if ((int)threadIdx.x + i * kThreads < nv) z += sum_of<T>(u[i], mine, c);
+        if (z != z || mine == FLT_MAX) { /* a NaN or an infinity among them: one by one */
+            z = 0.0f;
 #pragma unroll
-            for (int j = 0; j < VE; j++) z += fl_ex2((clean(fl_to_float(e[j])) - mine) * c);
+            for (int i = 0; i < NV; i++) {
+                if ((int)threadIdx.x + i * kThreads >= nv) continue;
+                const T* e = reinterpret_cast<const T*>(&u[i]);
+#pragma unroll
+                for (int j = 0; j < VE; j++) z += fl_ex2((clean(fl_to_float(e[j])) - mine) * c);
+            }
         }
         z += fl_ex2((ends[0] - mine) * c) + fl_ex2((ends[1] - mine) * c);
         z *= fl_ex2((mine - m) * c);
@@ -197,24 +277,37 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g)
     }
 }
 
-/* A row's maximum, first index of it and sum, by a warp from its chunks. */
-__device__ __forceinline__ Decision merge_row(const RowPart* __restrict__ part, int chunks, double inv_t)
+/* A row's maximum, first index of it and sum, by a warp from its chunks: up to
+ * 128 of them are loaded at once, more a second time. */
+__device__ __forceinline__ Decision merge_row(const RowPart* __restrict__ part, int chunks, float t, const double* table)
 {
     const int lane = threadIdx.x & 31;
     Decision d{0.0, -INFINITY, 0, 0, INT_MAX};
-    for (int c = lane; c < chunks; c += 32) {
-        const RowPart p = part[c];
-        if (p.m > d.m || (p.m == d.m && p.best < d.best)) d.m = p.m, d.best = p.best;
+    RowPart p[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int c = lane + 32 * i;
+        p[i] = c < chunks ? part[c] : RowPart{-INFINITY, 0.0f, INT_MAX, 0};
     }
+    auto take = [&](const RowPart& r) {
+        if (r.m > d.m || (r.m == d.m && r.best < d.best)) d.m = r.m, d.best = r.best;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; i++) take(p[i]);
+    for (int c = lane + 128; c < chunks; c += 32) take(part[c]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float m2 = __shfl_xor_sync(0xffffffffu, d.m, o);
         const int b2 = __shfl_xor_sync(0xffffffffu, d.best, o);
         if (m2 > d.m || (m2 == d.m && b2 < d.best)) d.m = m2, d.best = b2;
     }
-    for (int c = lane; c < chunks; c += 32) {
-        const RowPart p = part[c];
-        if (p.m > -INFINITY) d.z += (double)p.z * exp64(((double)p.m - (double)d.m) * inv_t);
+    if (t > 0.0f && d.m > -INFINITY) {
+        const Exp64 e = exp64_of(d.m, t, table);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (p[i].m > -INFINITY) d.z += (double)p[i].z * e(p[i].m);
+        for (int c = lane + 128; c < chunks; c += 32)
+            if (part[c].m > -INFINITY) d.z += (double)part[c].z * e(part[c].m);
     }
     d.z = warp_sum(d.z);
     return d;
@@ -227,18 +320,33 @@ __device__ __forceinline__ float prob(const float* q, int x)
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_stop_kernel(const FlVerify g)
+__global__ void __launch_bounds__(kStopThreads) verify_stop_kernel(const FlVerify g)
 {
-    __shared__ Decision s_row[kThreads / 32];
-    __shared__ int s_ok[kThreads / 32];
-    __shared__ double s_d[kThreads / 32];
+    __shared__ Decision s_row[kStopThreads / 32];
+    __shared__ int s_ok[kStopThreads / 32];
+    __shared__ double s_d[kStopThreads / 32], s_table[32];
     const int chunk = blockIdx.y, s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = gridDim.y;
     fl_pdl_trigger();
     const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
     const int r0 = max(g.row_start[s], 0), r1 = min(g.row_start[s + 1], g.n_rows);
     const float t = g.temperature[s];
     const bool greedy = !(t > 0.0f);
-    const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
+    exp64_table(s_table);
+    /* what a row's test compares; the first rows' before the wait */
+    int x = -1;
+    float q = 1.0f, l = -INFINITY, u = 0.0f;
+    auto draft_of = [&](int row) {
+        x = -1;
+        if (row >= r1 - 1) return;
+        x = g.draft[row];
+        if (x < 0 || x >= g.vocab) x = -1;
+        if (x < 0 || greedy) return;
+        if (g.probs) q = prob(g.probs + row * g.probs_stride, x);
+        l = clean(fl_to_float(static_cast<const T*>(g.logits)[row * g.logits_stride + x]));
+        u = g.u_accept[row];
+    };
+    draft_of(r0 + warp);
+    __syncthreads();
     fl_pdl_wait();
     if (r1 <= r0) {
         if (chunk == 0 && threadIdx.x == 0) sp.dec[s] = Decision{0.0, -INFINITY, -1, 0, -1};
@@ -246,33 +354,24 @@ __global__ void __launch_bounds__(kThreads) verify_stop_kernel(const FlVerify g)
     }
     /* the acceptance tests, a row per warp, in order */
     Decision d{};
-    for (int base = r0;; base += kThreads / 32) {
+    for (int base = r0;; base += kStopThreads / 32) {
         const int row = base + warp;
         if (row < r1) {
-            Decision w = merge_row(sp.part + (size_t)row * chunks, chunks, inv_t);
+            Decision w = merge_row(sp.part + (size_t)row * chunks, chunks, t, s_table);
             w.row = row;
             bool ok = false;
-            if (row < r1 - 1) {
-                const int x = g.draft[row];
-                if (x >= 0 && x < g.vocab && w.m > -INFINITY) {
-                    if (greedy) {
-                        ok = x == w.best;
-                    } else {
-                        const float q = g.probs ? prob(g.probs + row * g.probs_stride, x) : 1.0f;
-                        const float l = clean(fl_to_float(static_cast<const T*>(g.logits)[row * g.logits_stride + x]));
-                        ok = (double)g.u_accept[row] * (double)q * w.z < weight(l, w.m, inv_t);
-                    }
-                }
-                w.rej = 1;
-            }
+            if (base > r0) draft_of(row);
+            if (x >= 0 && w.m > -INFINITY)
+                ok = greedy ? x == w.best : (double)u * (double)q * w.z < exp64_of(w.m, t, s_table)(l);
+            w.rej = row < r1 - 1;
             if (lane == 0) s_row[warp] = w, s_ok[warp] = ok;
         } else if (lane == 0) {
             s_ok[warp] = 1; /* behind the last row, which always stops */
         }
         __syncthreads();
         int stop = 0;
-        while (stop < kThreads / 32 && s_ok[stop]) stop++;
-        if (stop < kThreads / 32) {
+        while (stop < kStopThreads / 32 && s_ok[stop]) stop++;
+        if (stop < kStopThreads / 32) {
             d = s_row[stop];
             break;
         }
@@ -282,16 +381,19 @@ __global__ void __launch_bounds__(kThreads) verify_stop_kernel(const FlVerify g)
     if (greedy || !(d.m > -INFINITY)) return;
     /* the chunk's sum over the row that it stopped at */
     const int skip = d.rej && !g.probs ? g.draft[d.row] : -1;
+    const Exp64 ew = exp64_of(d.m, t, s_table);
     double sum = 0.0;
-    each<T, kThreads>(static_cast<const T*>(g.logits) + d.row * g.logits_stride, chunk * kChunk,
-                      min(g.vocab, (chunk + 1) * kChunk), [&](int x, float l) {
-                          if (x != skip) sum += weight(l, d.m, inv_t);
-                      });
+    each<kStopThreads>(static_cast<const T*>(g.logits) + d.row * g.logits_stride, chunk * kChunk, min(g.vocab, (chunk + 1) * kChunk),
+         [&](int x, int n, const float* l) {
+#pragma unroll
+             for (int j = 0; j < 16 / (int)sizeof(T); j++)
+                 if (j < n && x + j != skip) sum += ew(l[j]);
+         });
     sum = warp_sum(sum);
     if (lane == 0) s_d[warp] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 32; w++) sum += s_d[w];
+        for (int w = 1; w < kStopThreads / 32; w++) sum += s_d[w];
         sp.sums[(size_t)s * chunks + chunk].e = sum;
     }
 }
@@ -308,20 +410,39 @@ __device__ __forceinline__ double total_of(const Sums* __restrict__ s, int chunk
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_rest_kernel(const FlVerify g)
 {
-    __shared__ double s_d[kThreads / 32];
+    __shared__ double s_d[kThreads / 32], s_table[32];
     const int chunk = blockIdx.y, s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = gridDim.y;
     fl_pdl_trigger();
     const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
     const float t = g.temperature[s];
+    exp64_table(s_table);
+    __syncthreads();
     fl_pdl_wait();
     const Decision d = sp.dec[s];
     if (d.row < 0 || !d.rej || !(t > 0.0f) || !(d.m > -INFINITY)) return;
-    const double inv_t = 1.0 / (double)t, z = total_of<false>(sp.sums + (size_t)s * chunks, chunks);
+    const double z = total_of<false>(sp.sums + (size_t)s * chunks, chunks);
+    const Exp64 ew = exp64_of(d.m, t, s_table);
     const float* q = g.probs + d.row * g.probs_stride;
     double sum = 0.0;
-    each<T, kThreads>(static_cast<const T*>(g.logits) + d.row * g.logits_stride, chunk * kChunk,
-                      min(g.vocab, (chunk + 1) * kChunk),
-                      [&](int x, float l) { sum += fmax(weight(l, d.m, inv_t) - (double)prob(q, x) * z, 0.0); });
+    each<kThreads>(static_cast<const T*>(g.logits) + d.row * g.logits_stride, chunk * kChunk,
+                   min(g.vocab, (chunk + 1) * kChunk), [&](int x, int n, const float* l) {
+             constexpr int VE = 16 / (int)sizeof(T);
+             float p[VE] = {};
+             if (n == VE && reinterpret_cast<uintptr_t>(q + x) % 16 == 0) {
+#pragma unroll
+                 for (int j = 0; j < VE; j += 4) {
+                     const float4 v = __ldg(reinterpret_cast<const float4*>(q + x + j));
+                     p[j] = v.x, p[j + 1] = v.y, p[j + 2] = v.z, p[j + 3] = v.w;
+                 }
+             } else {
+#pragma unroll
+                 for (int j = 0; j < VE; j++)
+                     if (j < n) p[j] = q[x + j];
+             }
+#pragma unroll
+             for (int j = 0; j < VE; j++)
+                 if (j < n) sum += fmax(ew(l[j]) - (double)(p[j] > 0.0f ? p[j] : 0.0f) * z, 0.0);
+         });
     sum = warp_sum(sum);
     if (lane == 0) s_d[warp] = sum;
     __syncthreads();
@@ -335,13 +456,15 @@ template <typename T>
 __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const FlVerify g)
 {
     constexpr int PER = kChunk / kDrawThreads; /* consecutive entries of a thread */
-    __shared__ double s_w[kDrawThreads / 32];
+    __shared__ double s_w[kDrawThreads / 32], s_table[32];
     __shared__ double s_before;
     __shared__ int s_chunk, s_tok, s_last;
     const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = chunks_of(g.vocab);
     const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
     const int r0 = max(g.row_start[s], 0), r1 = min(g.row_start[s + 1], g.n_rows);
     const float t = g.temperature[s];
+    exp64_table(s_table);
+    __syncthreads();
     fl_pdl_wait();
     const Decision d = sp.dec[s];
     if (d.row < 0) {
@@ -358,7 +481,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const FlVerif
     } else if (d.m > -INFINITY && !(z > 0.0)) {
         token = skip; /* the draft is all of p */
     } else if (d.m > -INFINITY) {
-        const double inv_t = 1.0 / (double)t;
+        const Exp64 ew = exp64_of(d.m, t, s_table);
         bool rest = d.rej && g.probs;
         double all = z;
         if (rest) {
@@ -402,7 +525,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const FlVerif
             const int x = x0 + i;
             w[i] = 0.0;
             if (x < g.vocab && x != skip) {
-                w[i] = weight(clean(fl_to_float(l[x])), d.m, inv_t);
+                w[i] = ew(clean(fl_to_float(l[x])));
                 if (rest) w[i] = fmax(w[i] - (double)prob(q, x) * z, 0.0);
             }
             mine += w[i];
@@ -457,7 +580,7 @@ cudaError_t launch(const FlVerify& v, cudaStream_t st)
     const unsigned chunks = chunks_of(v.vocab);
     if (v.n_rows > 0) verify_rows_kernel<T><<<dim3(v.n_rows, chunks), kThreads, 0, st>>>(v);
     cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) e = after(verify_stop_kernel<T>, dim3(v.n_seqs, chunks), kThreads, v, st);
+    if (e == cudaSuccess) e = after(verify_stop_kernel<T>, dim3(v.n_seqs, chunks), kStopThreads, v, st);
     if (e == cudaSuccess && v.probs) e = after(verify_rest_kernel<T>, dim3(v.n_seqs, chunks), kThreads, v, st);
     if (e == cudaSuccess) e = after(verify_draw_kernel<T>, dim3(v.n_seqs), kDrawThreads, v, st);
     return e;
