@@ -2,22 +2,25 @@
  * fl_verify.cu — verification of drafted tokens against the target's logits
  * (fl_verify_device).
  *
- * Bound by reading the logits once; four kernels, each started early and
- * waiting for the one before (programmatic dependent launch), over chunks of
- * 4096 vocabulary entries so that one sequence and sixty-four both spread over
- * the SMs:
- *  rows: per (row, chunk) the maximum with its first index and the sum of
- *        exp((l - max) / T), exponentials in fp32;
- *  stop: per (sequence, chunk) first the acceptance tests, which every chunk's
- *        CTA repeats (a few rows of a few partials), then the chunk's sum over
- *        the row that the sequence stopped at, exponentials and sums in 64 bits;
- *  rest: the same for max(p - q, 0), which needs that sum's total first;
- *  draw: per sequence the chunk that the draw falls into, and the entry in it.
+ * Bound by reading the logits once; two kernels, the second started early and
+ * waiting for the first (programmatic dependent launch):
+ *  rows:   per (row, chunk of 4096 entries) the maximum and the sum of exp((l -
+ *          max) / T), exponentials in fp32; the first index of the maximum where
+ *          the sequence is greedy;
+ *  finish: a cluster of 8 CTAs per sequence, each of whose 64 warps has a
+ *          contiguous range of the vocabulary.  Every CTA repeats the acceptance
+ *          tests (a few rows of a few partials); then over the row that the
+ *          sequence stopped at: the sum of the exponentials, the sum of
+ *          max(p - q, 0), which needs the first one's total, and the entry that
+ *          the draw falls into, looked for by the warp whose range holds it.
+ *          Sums go around by distributed shared memory.
  * The draw compares with cumulative sums of up to 2^24 entries, whose borders
- * lie closer than fp32 resolves, hence the 64 bits there; the acceptance tests
- * compare single probabilities, for which the fp32 exponentials' 2^-22 is
- * enough.
+ * lie closer than fp32 resolves: the second kernel's exponentials and sums are
+ * in 64 bits.  The acceptance tests compare single probabilities, for which the
+ * fp32 exponentials' 2^-22 is enough.
  */
+#include <cooperative_groups.h>
+
 #include <cfloat>
 #include <climits>
 
@@ -25,8 +28,8 @@
 
 namespace {
 
-constexpr int kThreads = 128, kStopThreads = 256, kChunk = 4096;
-constexpr int kDrawThreads = 512;
+constexpr int kThreads = 128, kChunk = 4096;
+constexpr int kCluster = 8, kFinThreads = 256, kFinWarps = kFinThreads / 32;
 
 struct RowPart { /* of a row's chunk */
     float m, z;
@@ -35,35 +38,11 @@ struct RowPart { /* of a row's chunk */
 struct Decision { /* of a sequence */
     double z;    /* sum of exp((l - m) / T) over the row, exponentials in fp32 */
     float m;
-    int32_t row; /* that it stopped at; -1: no rows */
+    int32_t row; /* that it stopped at */
     int32_t rej, best;
 };
-struct Sums { /* of a chunk of that row */
-    double e;    /* of exp((l - m) / T), less the draft's where it was rejected and certain */
-    double rest; /* of max(exp - q Z, 0) */
-};
 
-struct Space {
-    RowPart* part;   /* [n_rows][chunks] */
-    Decision* dec;   /* [n_seqs] */
-    Sums* sums;      /* [n_seqs][chunks] */
-};
 __host__ __device__ __forceinline__ int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
-__host__ __device__ __forceinline__ Space space(void* p, int n_rows, int n_seqs, int vocab, size_t* bytes = nullptr)
-{
-    uint8_t* b = static_cast<uint8_t*>(p);
-    const size_t c = (size_t)chunks_of(vocab);
-    Space s;
-    size_t at = 0;
-    s.part = reinterpret_cast<RowPart*>(b);
-    at += fl_align256(n_rows * c * sizeof(RowPart));
-    s.dec = reinterpret_cast<Decision*>(b + at);
-    at += fl_align256(n_seqs * sizeof(Decision));
-    s.sums = reinterpret_cast<Sums*>(b + at);
-    at += n_seqs * c * sizeof(Sums);
-    if (bytes) *bytes = at;
-    return s;
-}
 
 /* NaN is masked, +infinity is the largest finite value. */
 __device__ __forceinline__ float clean(float l) { return l != l ? -INFINITY : fminf(l, FLT_MAX); }
@@ -115,37 +94,6 @@ __device__ __forceinline__ double warp_sum(double v)
     return v;
 }
 
-/* f(x, n, l): n of this thread's entries of [x0, x1) from x on, by threads and
- * ascending: ends that are not 16-byte aligned one by one, the rest 16 bytes
- * at a time. */
-template <int NT, typename T, typename F>
-__device__ __forceinline__ void each(const T* __restrict__ row, int x0, int x1, F f)
-{
-    constexpr int VE = 16 / sizeof(T);
-    const int n = x1 - x0;
-    const int head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(row + x0) % 16) % 16 / sizeof(T)));
-    const int nv = (n - head) / VE;
-    float l[VE] = {};
-    if ((int)threadIdx.x < head) {
-        l[0] = clean(fl_to_float(row[x0 + threadIdx.x]));
-        f(x0 + (int)threadIdx.x, 1, l);
-    }
-    const uint4* v = reinterpret_cast<const uint4*>(row + x0 + head);
-#pragma unroll 2
-    for (int i = threadIdx.x; i < nv; i += NT) {
-        const uint4 u = __ldg(v + i);
-        const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int j = 0; j < VE; j++) l[j] = clean(fl_to_float(e[j]));
-        f(x0 + head + i * VE, VE, l);
-    }
-    const int tail = x0 + head + nv * VE + threadIdx.x;
-    if (tail < x1) {
-        l[0] = clean(fl_to_float(row[tail]));
-        f(tail, 1, l);
-    }
-}
-
 /* The larger of each half's two numbers, NaN losing. */
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __half)
 {
@@ -181,17 +129,18 @@ template <typename T>
 __device__ __forceinline__ float sum_of(const uint4& u, float m, float c)
 {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    float z = 0.0f;
+    float z = 0.0f, z1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if constexpr (sizeof(T) == 4) {
             z += fl_ex2((__uint_as_float(w[i]) - m) * c);
         } else {
             const float2 f = halves(w[i], T());
-            z += fl_ex2((f.x - m) * c) + fl_ex2((f.y - m) * c);
+            z += fl_ex2((f.x - m) * c);
+            z1 += fl_ex2((f.y - m) * c);
         }
     }
-    return z;
+    return z + z1;
 }
 
 template <typename T>
@@ -229,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g)
     m = fl_warp_max(m);
     /* its first index, looked for by the threads that hold it */
     int best = INT_MAX;
-    if (mine == m && m > -INFINITY) {
+    if (!(t > 0.0f) && mine == m && m > -INFINITY) {
         if (ends[1] == m) best = x0 + tail;
 #pragma unroll
         for (int i = NV - 1; i >= 0; i--) {
@@ -272,8 +221,7 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g)
             if (s_m[w] > M || (s_m[w] == M && s_i[w] < B)) M = s_m[w], B = s_i[w];
         for (int w = 0; w < kThreads / 32; w++)
             if (s_m[w] > -INFINITY && t > 0.0f) Z += s_z[w] * fl_ex2((s_m[w] - M) * fminf(1.44269504f / t, FLT_MAX));
-        const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
-        sp.part[(size_t)row * gridDim.y + chunk] = RowPart{M, Z, B, 0};
+        static_cast<RowPart*>(g.workspace)[(size_t)row * gridDim.y + chunk] = RowPart{M, Z, B, 0};
     }
 }
 
@@ -319,15 +267,82 @@ __device__ __forceinline__ float prob(const float* q, int x)
     return v > 0.0f ? v : 0.0f;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kStopThreads) verify_stop_kernel(const FlVerify g)
+/* f(x, n, l): n of this lane's entries of [x0, x1) from x on: ends that are not
+ * 16-byte aligned one by one, the rest 16 bytes at a time. */
+template <typename T, typename F>
+__device__ __forceinline__ void each(const T* __restrict__ row, int x0, int x1, F f)
 {
-    __shared__ Decision s_row[kStopThreads / 32];
-    __shared__ int s_ok[kStopThreads / 32];
-    __shared__ double s_d[kStopThreads / 32], s_table[32];
-    const int chunk = blockIdx.y, s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = gridDim.y;
-    fl_pdl_trigger();
-    const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
+    constexpr int VE = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31, n = max(0, x1 - x0);
+    const int head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(row + x0) % 16) % 16 / sizeof(T)));
+    const int nv = (n - head) / VE;
+    float l[VE] = {};
+    if (lane < head) {
+        l[0] = clean(fl_to_float(row[x0 + lane]));
+        f(x0 + lane, 1, l);
+    }
+    const uint4* v = reinterpret_cast<const uint4*>(row + x0 + head);
+#pragma unroll 2
+    for (int i = lane; i < nv; i += 32) {
+        const uint4 u = __ldg(v + i);
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int j = 0; j < VE; j++) l[j] = clean(fl_to_float(e[j]));
+        f(x0 + head + i * VE, VE, l);
+    }
+    const int tail = x0 + head + nv * VE + lane;
+    if (tail < x1) {
+        l[0] = clean(fl_to_float(row[tail]));
+        f(tail, 1, l);
+    }
+}
+
+/* This warp's sum, put beside the other warps'; the CTA's sum at its rank in
+ * every CTA of the cluster; returns the total, the same everywhere. */
+__device__ __forceinline__ double share(double v, double* warps, double* ranks)
+{
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cl = cg::this_cluster();
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x < kCluster) {
+        double sum = 0.0;
+        for (int w = 0; w < kFinWarps; w++) sum += warps[w];
+        cl.map_shared_rank(ranks, threadIdx.x)[cl.block_rank()] = sum;
+    }
+    cl.sync();
+    double all = 0.0;
+    for (int r = 0; r < kCluster; r++) all += ranks[r];
+    return all;
+}
+
+/* The first of n parts whose running sum exceeds the goal, else the last with
+ * any weight; `before` becomes the sum of those ahead of it. */
+__device__ __forceinline__ int part_of(const double* parts, int n, double goal, double& before)
+{
+    double run = before;
+    int at = -1;
+    for (int i = 0; i < n; i++) {
+        if (parts[i] > 0.0) {
+            at = i;
+            before = run;
+            if (run + parts[i] > goal) break;
+        }
+        run += parts[i];
+    }
+    return at;
+}
+
+template <typename T>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) verify_finish_kernel(const FlVerify g)
+{
+    __shared__ Decision s_row[kFinWarps];
+    __shared__ int s_ok[kFinWarps];
+    __shared__ double s_table[32], s_warps[2][kFinWarps], s_ranks[2][kCluster];
+    const int s = blockIdx.x / kCluster, rank = blockIdx.x % kCluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int chunks = chunks_of(g.vocab);
+    const RowPart* part = static_cast<const RowPart*>(g.workspace);
     const int r0 = max(g.row_start[s], 0), r1 = min(g.row_start[s + 1], g.n_rows);
     const float t = g.temperature[s];
     const bool greedy = !(t > 0.0f);
@@ -348,16 +363,16 @@ __global__ void __launch_bounds__(kStopThreads) verify_stop_kernel(const FlVerif
     draft_of(r0 + warp);
     __syncthreads();
     fl_pdl_wait();
-    if (r1 <= r0) {
-        if (chunk == 0 && threadIdx.x == 0) sp.dec[s] = Decision{0.0, -INFINITY, -1, 0, -1};
+    if (r1 <= r0) { /* this and every later return: alike in the whole cluster */
+        if (rank == 0 && threadIdx.x == 0) g.accepted[s] = 0;
         return;
     }
     /* the acceptance tests, a row per warp, in order */
     Decision d{};
-    for (int base = r0;; base += kStopThreads / 32) {
+    for (int base = r0;; base += kFinWarps) {
         const int row = base + warp;
         if (row < r1) {
-            Decision w = merge_row(sp.part + (size_t)row * chunks, chunks, t, s_table);
+            Decision w = merge_row(part + (size_t)row * chunks, chunks, t, s_table);
             w.row = row;
             bool ok = false;
             if (base > r0) draft_of(row);
@@ -370,230 +385,133 @@ __global__ void __launch_bounds__(kStopThreads) verify_stop_kernel(const FlVerif
         }
         __syncthreads();
         int stop = 0;
-        while (stop < kStopThreads / 32 && s_ok[stop]) stop++;
-        if (stop < kStopThreads / 32) {
+        while (stop < kFinWarps && s_ok[stop]) stop++;
+        if (stop < kFinWarps) {
             d = s_row[stop];
             break;
         }
         __syncthreads();
     }
-    if (chunk == 0 && threadIdx.x == 0) sp.dec[s] = d;
-    if (greedy || !(d.m > -INFINITY)) return;
-    /* the chunk's sum over the row that it stopped at */
-    const int skip = d.rej && !g.probs ? g.draft[d.row] : -1;
-    const Exp64 ew = exp64_of(d.m, t, s_table);
-    double sum = 0.0;
-    each<kStopThreads>(static_cast<const T*>(g.logits) + d.row * g.logits_stride, chunk * kChunk, min(g.vocab, (chunk + 1) * kChunk),
-         [&](int x, int n, const float* l) {
-#pragma unroll
-             for (int j = 0; j < 16 / (int)sizeof(T); j++)
-                 if (j < n && x + j != skip) sum += ew(l[j]);
-         });
-    sum = warp_sum(sum);
-    if (lane == 0) s_d[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kStopThreads / 32; w++) sum += s_d[w];
-        sp.sums[(size_t)s * chunks + chunk].e = sum;
-    }
-}
-
-/* The sum of a sequence's chunks, the same in every thread of a warp. */
-template <bool REST>
-__device__ __forceinline__ double total_of(const Sums* __restrict__ s, int chunks)
-{
-    double v = 0.0;
-    for (int c = threadIdx.x & 31; c < chunks; c += 32) v += REST ? s[c].rest : s[c].e;
-    return warp_sum(v);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rest_kernel(const FlVerify g)
-{
-    __shared__ double s_d[kThreads / 32], s_table[32];
-    const int chunk = blockIdx.y, s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = gridDim.y;
-    fl_pdl_trigger();
-    const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
-    const float t = g.temperature[s];
-    exp64_table(s_table);
-    __syncthreads();
-    fl_pdl_wait();
-    const Decision d = sp.dec[s];
-    if (d.row < 0 || !d.rej || !(t > 0.0f) || !(d.m > -INFINITY)) return;
-    const double z = total_of<false>(sp.sums + (size_t)s * chunks, chunks);
-    const Exp64 ew = exp64_of(d.m, t, s_table);
-    const float* q = g.probs + d.row * g.probs_stride;
-    double sum = 0.0;
-    each<kThreads>(static_cast<const T*>(g.logits) + d.row * g.logits_stride, chunk * kChunk,
-                   min(g.vocab, (chunk + 1) * kChunk), [&](int x, int n, const float* l) {
-             constexpr int VE = 16 / (int)sizeof(T);
-             float p[VE] = {};
-             if (n == VE && reinterpret_cast<uintptr_t>(q + x) % 16 == 0) {
-#pragma unroll
-                 for (int j = 0; j < VE; j += 4) {
-                     const float4 v = __ldg(reinterpret_cast<const float4*>(q + x + j));
-                     p[j] = v.x, p[j + 1] = v.y, p[j + 2] = v.z, p[j + 3] = v.w;
-                 }
-             } else {
-#pragma unroll
-                 for (int j = 0; j < VE; j++)
-                     if (j < n) p[j] = q[x + j];
-             }
-#pragma unroll
-             for (int j = 0; j < VE; j++)
-                 if (j < n) sum += fmax(ew(l[j]) - (double)(p[j] > 0.0f ? p[j] : 0.0f) * z, 0.0);
-         });
-    sum = warp_sum(sum);
-    if (lane == 0) s_d[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 32; w++) sum += s_d[w];
-        sp.sums[(size_t)s * chunks + chunk].rest = sum;
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const FlVerify g)
-{
-    constexpr int PER = kChunk / kDrawThreads; /* consecutive entries of a thread */
-    __shared__ double s_w[kDrawThreads / 32], s_table[32];
-    __shared__ double s_before;
-    __shared__ int s_chunk, s_tok, s_last;
-    const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = chunks_of(g.vocab);
-    const Space sp = space(g.workspace, g.n_rows, g.n_seqs, g.vocab);
-    const int r0 = max(g.row_start[s], 0), r1 = min(g.row_start[s + 1], g.n_rows);
-    const float t = g.temperature[s];
-    exp64_table(s_table);
-    __syncthreads();
-    fl_pdl_wait();
-    const Decision d = sp.dec[s];
-    if (d.row < 0) {
-        if (threadIdx.x == 0) g.accepted[s] = 0;
+    auto write = [&](int token, int first, int step) {
+        for (int row = r0 + first; row < r1; row += step)
+            g.tokens[row] = row < d.row ? g.draft[row] : row == d.row ? token : -1;
+        if (first == 0) g.accepted[s] = d.row - r0;
+    };
+    if (greedy || !(d.m > -INFINITY)) {
+        if (rank == 0) write(d.m > -INFINITY ? d.best : -1, threadIdx.x, kFinThreads);
         return;
     }
-    int token = -1;
-    const Sums* sums = sp.sums + (size_t)s * chunks;
-    const bool greedy = !(t > 0.0f);
-    const double z = greedy || !(d.m > -INFINITY) ? 0.0 : total_of<false>(sums, chunks);
+    /* the sums over the row that it stopped at; this warp's entries: [x0, x1) */
+    const int per = (g.vocab + kCluster * kFinWarps - 1) / (kCluster * kFinWarps);
+    const int x0 = min(g.vocab, (rank * kFinWarps + warp) * per), x1 = min(g.vocab, x0 + per);
+    const T* row = static_cast<const T*>(g.logits) + d.row * g.logits_stride;
+    const Exp64 ew = exp64_of(d.m, t, s_table);
     const int skip = d.rej && !g.probs ? g.draft[d.row] : -1;
-    if (d.m > -INFINITY && greedy) {
-        token = d.best;
-    } else if (d.m > -INFINITY && !(z > 0.0)) {
-        token = skip; /* the draft is all of p */
-    } else if (d.m > -INFINITY) {
-        const Exp64 ew = exp64_of(d.m, t, s_table);
-        bool rest = d.rej && g.probs;
-        double all = z;
-        if (rest) {
-            all = total_of<true>(sums, chunks);
-            if (!(all > 0.0)) rest = false, all = z; /* nothing is left of p - q: p itself */
-        }
-        const double goal = (double)g.u_sample[s] * all;
-        /* the first chunk whose running sum exceeds the goal; else the last that has any weight */
-        if (warp == 0) {
-            double before = 0.0, before_last = 0.0;
-            int hit = -1, last = 0;
-            for (int c0 = 0; c0 < chunks && hit < 0; c0 += 32) {
-                const int c = c0 + lane;
-                const double w = c < chunks ? (rest ? sums[c].rest : sums[c].e) : 0.0;
-                double run = w;
+    double sum = 0.0;
+    each(row, x0, x1, [&](int x, int n, const float* l) {
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double u = __shfl_up_sync(0xffffffffu, run, o);
-                    if (lane >= o) run += u;
-                }
-                const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-                const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && before + run > goal);
-                const int at = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : -1;
-                if (at >= 0) {
-                    last = c0 + at;
-                    before_last = before + __shfl_sync(0xffffffffu, run - w, at);
-                }
-                if (over) hit = last;
-                before += __shfl_sync(0xffffffffu, run, 31);
-            }
-            if (lane == 0) s_chunk = last, s_before = before_last, s_tok = INT_MAX, s_last = -1;
-        }
-        __syncthreads();
-        /* the entry in it */
-        const int x0 = s_chunk * kChunk + threadIdx.x * PER;
-        const T* l = static_cast<const T*>(g.logits) + d.row * g.logits_stride;
-        const float* q = rest ? g.probs + d.row * g.probs_stride : nullptr;
-        double w[PER], mine = 0.0;
+        for (int j = 0; j < 16 / (int)sizeof(T); j++)
+            if (j < n && x + j != skip) sum += ew(l[j]);
+    });
+    const double z = share(sum, s_warps[0], s_ranks[0]);
+    if (!(z > 0.0)) { /* the draft is all of p */
+        if (rank == 0) write(skip, threadIdx.x, kFinThreads);
+        return;
+    }
+    double all = z;
+    const float* probs = d.rej && g.probs ? g.probs + d.row * g.probs_stride : nullptr;
+    if (probs) {
+        sum = 0.0;
+        each(row, x0, x1, [&](int x, int n, const float* l) {
+            constexpr int VE = 16 / (int)sizeof(T);
+            float p[VE] = {};
+            if (n == VE && reinterpret_cast<uintptr_t>(probs + x) % 16 == 0) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int x = x0 + i;
-            w[i] = 0.0;
-            if (x < g.vocab && x != skip) {
-                w[i] = ew(clean(fl_to_float(l[x])));
-                if (rest) w[i] = fmax(w[i] - (double)prob(q, x) * z, 0.0);
+                for (int j = 0; j < VE; j += 4) {
+                    const float4 v = __ldg(reinterpret_cast<const float4*>(probs + x + j));
+                    p[j] = v.x, p[j + 1] = v.y, p[j + 2] = v.z, p[j + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VE; j++)
+                    if (j < n) p[j] = probs[x + j];
             }
-            mine += w[i];
+#pragma unroll
+            for (int j = 0; j < VE; j++)
+                if (j < n) sum += fmax(ew(l[j]) - (double)(p[j] > 0.0f ? p[j] : 0.0f) * z, 0.0);
+        });
+        all = share(sum, s_warps[1], s_ranks[1]);
+        if (!(all > 0.0)) probs = nullptr, all = z; /* nothing is left of p - q: p itself */
+    }
+    /* whose range the draw falls into, and the entry in it */
+    const double goal = (double)g.u_sample[s] * all;
+    const int w = probs ? 1 : 0;
+    double before = 0.0;
+    if (part_of(s_ranks[w], kCluster, goal, before) != rank) return;
+    if (part_of(s_warps[w], kFinWarps, goal, before) != warp) return;
+    int token = -1;
+    bool found = false;
+    for (int base = x0; base < x1 && !found; base += 32 * 8) { /* eight entries of a lane, consecutive */
+        const int at = base + lane * 8;
+        double e[8], mine = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            e[j] = 0.0;
+            if (at + j < x1 && at + j != skip) {
+                e[j] = ew(clean(fl_to_float(row[at + j])));
+                if (probs) e[j] = fmax(e[j] - (double)prob(probs, at + j) * z, 0.0);
+            }
+            mine += e[j];
         }
         double run = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const double u = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += u;
+            const double v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
         }
-        if (lane == 31) s_w[warp] = run;
-        __syncthreads();
-        double c = s_before + run - mine;
-        for (int i = 0; i < warp; i++) c += s_w[i];
-        int last = -1, hit = INT_MAX;
+        double c = before + run - mine;
+        int hit = INT_MAX, last = -1;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            c += w[i];
-            if (w[i] > 0.0) {
-                last = x0 + i;
-                if (c > goal && hit == INT_MAX) hit = x0 + i;
+        for (int j = 0; j < 8; j++) {
+            c += e[j];
+            if (e[j] > 0.0) {
+                last = at + j;
+                if (c > goal && hit == INT_MAX) hit = at + j;
             }
         }
-        if (hit != INT_MAX) atomicMin(&s_tok, hit);
-        if (last >= 0) atomicMax(&s_last, last);
-        __syncthreads();
-        token = s_tok != INT_MAX ? s_tok : s_last;
+        hit = __reduce_min_sync(0xffffffffu, hit);
+        last = __reduce_max_sync(0xffffffffu, last);
+        found = hit != INT_MAX;
+        if (found)
+            token = hit;
+        else if (last >= 0)
+            token = last; /* rounding may leave the goal above every sum */
+        before += __shfl_sync(0xffffffffu, run, 31);
     }
-    for (int row = r0 + threadIdx.x; row < r1; row += kDrawThreads)
-        g.tokens[row] = row < d.row ? g.draft[row] : row == d.row ? token : -1;
-    if (threadIdx.x == 0) g.accepted[s] = d.row - r0;
+    write(token, lane, 32);
 }
 
-template <typename K>
-cudaError_t after(K kernel, dim3 grid, int threads, const FlVerify& v, cudaStream_t st)
+template <typename T>
+cudaError_t launch(const FlVerify& v, cudaStream_t st)
 {
+    if (v.n_rows > 0) verify_rows_kernel<T><<<dim3(v.n_rows, chunks_of(v.vocab)), kThreads, 0, st>>>(v);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
+    cfg.gridDim = dim3((unsigned)v.n_seqs * kCluster);
+    cfg.blockDim = dim3(kFinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, v);
-}
-
-template <typename T>
-cudaError_t launch(const FlVerify& v, cudaStream_t st)
-{
-    const unsigned chunks = chunks_of(v.vocab);
-    if (v.n_rows > 0) verify_rows_kernel<T><<<dim3(v.n_rows, chunks), kThreads, 0, st>>>(v);
-    cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) e = after(verify_stop_kernel<T>, dim3(v.n_seqs, chunks), kStopThreads, v, st);
-    if (e == cudaSuccess && v.probs) e = after(verify_rest_kernel<T>, dim3(v.n_seqs, chunks), kThreads, v, st);
-    if (e == cudaSuccess) e = after(verify_draw_kernel<T>, dim3(v.n_seqs), kDrawThreads, v, st);
-    return e;
+    return cudaLaunchKernelEx(&cfg, verify_finish_kernel<T>, v);
 }
 
 } // namespace
 
-size_t fl_verify_workspace_bytes(int n_rows, int n_seqs, int vocab)
-{
-    size_t bytes;
-    space(nullptr, n_rows, n_seqs, vocab, &bytes);
-    return bytes;
-}
+size_t fl_verify_workspace_bytes(int n_rows, int, int vocab) { return (size_t)n_rows * chunks_of(vocab) * sizeof(RowPart); }
 
 cudaError_t fl_launch_verify(const FlVerify& v, cudaStream_t st)
 {
