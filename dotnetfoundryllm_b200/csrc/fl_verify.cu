@@ -47,44 +47,76 @@ __host__ __device__ __forceinline__ int chunks_of(int vocab) { return (vocab + k
 /* NaN is masked, +infinity is the largest finite value. */
 __device__ __forceinline__ float clean(float l) { return l != l ? -INFINITY : fminf(l, FLT_MAX); }
 
-/* e^((l - m) / T) in 64 bits as 2^(k / 32), k = (l - m) A with A = 32 log2(e) /
- * T: k = n + f, |f| <= 1/2; 2^(n / 32) from a table of 32 and an exponent,
- * 2^(f / 32) by its Taylor series to f^5 (the next term is below 2^-48). */
-constexpr double kL = 0.69314718055994531 / 32.0;
+/* Exponentials in 64 bits as 2^(k / 256): k = n + f, |f| <= 1/2; 2^(n / 256) from
+ * a table of 256 and an exponent, 2^(f / 256) by its Taylor series to f^3 (the
+ * next term is below 2^-42 of the value; a draw's borders are some 2^-20 apart).
+ * 64-bit operations bound the sums, so they are few: with b whole, one FMA
+ * against 1.5 2^52 + b rounds k = l A + b, one sum takes n away, one FMA gives f.
+ * A table of 32 with a copy per lane, free of bank conflicts but with a longer
+ * series, took 78 us for a call of 64 sequences where this takes 66. */
+constexpr int kTabBits = 8, kTab = 1 << kTabBits;
+constexpr double kL = 0.69314718055994531 / kTab, kUnit = kTab * 1.4426950408889634;
+struct Table {
+    double v[kTab];
+};
+constexpr Table make_table()
+{
+    Table t{};
+    for (int i = 0; i < kTab; i++) {
+        double p = 1.0; /* e^(i kL), i kL < 0.7 */
+        for (int k = 20; k > 0; k--) p = 1.0 + p * (kL * i) / k;
+        t.v[i] = p;
+    }
+    return t;
+}
+__device__ const Table c_table = make_table();
+
+__device__ __forceinline__ double series(double f)
+{
+    return fma(fma(fma(kL * kL * kL / 6.0, f, kL * kL / 2.0), f, kL), f, 1.0);
+}
+
 struct Exp64 {
-    double a, m;
-    const double* table; /* 2^(i / 32), i < 32, in shared memory */
-    __device__ __forceinline__ double operator()(float l) const
+    double a, bm;        /* A = 256 log2(e) / T; magic + b */
+    const double* table; /* in shared memory */
+    float least;         /* logits below count as masked */
+    /* the value is p * scale: a caller that sums uses one FMA */
+    __device__ __forceinline__ void operator()(float l, double& p, double& scale) const
     {
-        const double k = ((double)l - m) * a;
-        if (!(k > -32.0 * 1021.0)) return 0.0; /* below 2^-1021; masked */
-        const double magic = 6755399441055744.0; /* 1.5 * 2^52: the sum's low word is k rounded */
-        const double t = k + magic;
-        const int n = __double2loint(t);
-        const double f = k - (t - magic);
-        double p = kL * kL * kL * kL * kL / 120.0;
-        p = fma(p, f, kL * kL * kL * kL / 24.0);
-        p = fma(p, f, kL * kL * kL / 6.0);
-        p = fma(p, f, kL * kL / 2.0);
-        p = fma(p, f, kL);
-        p = fma(p, f, 1.0);
-        p *= table[n & 31];
-        return __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+        const double x = (double)(l < least ? -INFINITY : l), t = fma(x, a, bm);
+        const double f = fma(x, a, bm - t);
+        const int n = __double2loint(t); /* k rounded, while it fits; l = -infinity gives t = -infinity */
+        p = series(f);
+        const double e = table[n & (kTab - 1)];
+        scale = __hiloint2double(__double2hiint(e) + ((n >> kTabBits) << 20), __double2loint(e));
+        if (!(t > 6755399441055744.0 - kTab * 1021.0)) p = scale = 0.0; /* below 2^-1021; masked */
+    }
+    __device__ __forceinline__ double value(float l) const
+    {
+        double p, scale;
+        (*this)(l, p, scale);
+        return p * scale;
     }
 };
 __device__ __forceinline__ void exp64_table(double* table)
 {
-    if (threadIdx.x < 32) {
-        /* e^(i kL) by its series; i kL < 0.7 */
-        const double y = kL * (double)(int)threadIdx.x;
-        double p = 1.0;
-        for (int i = 20; i > 0; i--) p = fma(p, y / (double)i, 1.0);
-        table[threadIdx.x] = p;
-    }
+    for (int i = threadIdx.x; i < kTab; i += blockDim.x) table[i] = c_table.v[i];
 }
+/* e^((l - m) / T) up to a factor 2^(c / 256), |c| <= 1/2, common to all l.  From
+ * |m| A = 2^40 on, neighbouring floats differ by 2^16 in k: only the maximum's
+ * equals have weight. */
 __device__ __forceinline__ Exp64 exp64_of(float m, float t, const double* table)
 {
-    return Exp64{46.166241308446828 / (double)t, (double)m, table}; /* 32 log2(e) */
+    const double a = kUnit / (double)t, b = (double)m * a;
+    if (fabs(b) < 1099511627776.0) return Exp64{a, 6755399441055744.0 - rint(b), table, -INFINITY};
+    return Exp64{fabs(1.0 / (double)m), 6755399441055744.0 - (m > 0.0f ? 1.0 : -1.0), table, m};
+}
+/* e^(x / T) for x <= 0, itself */
+__device__ __forceinline__ double exp_over(double x, float t, const double* table)
+{
+    const double k = fmax(x * (kUnit / (double)t), -(double)kTab * 1100.0), n = rint(k);
+    const int i = (int)n;
+    return i <= -kTab * 1021 ? 0.0 : series(k - n) * table[i & (kTab - 1)] * __hiloint2double((1023 + (i >> kTabBits)) << 20, 0);
 }
 
 __device__ __forceinline__ double warp_sum(double v)
@@ -250,12 +282,12 @@ __device__ __forceinline__ Decision merge_row(const RowPart* __restrict__ part, 
         if (m2 > d.m || (m2 == d.m && b2 < d.best)) d.m = m2, d.best = b2;
     }
     if (t > 0.0f && d.m > -INFINITY) {
-        const Exp64 e = exp64_of(d.m, t, table);
+        auto add = [&](const RowPart& r) {
+            if (r.m > -INFINITY) d.z += (double)r.z * exp_over((double)r.m - (double)d.m, t, table);
+        };
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (p[i].m > -INFINITY) d.z += (double)p[i].z * e(p[i].m);
-        for (int c = lane + 128; c < chunks; c += 32)
-            if (part[c].m > -INFINITY) d.z += (double)part[c].z * e(part[c].m);
+        for (int i = 0; i < 4; i++) add(p[i]);
+        for (int c = lane + 128; c < chunks; c += 32) add(part[c]);
     }
     d.z = warp_sum(d.z);
     return d;
@@ -276,7 +308,9 @@ __device__ __forceinline__ void each(const T* __restrict__ row, int x0, int x1, 
     const int lane = threadIdx.x & 31, n = max(0, x1 - x0);
     const int head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(row + x0) % 16) % 16 / sizeof(T)));
     const int nv = (n - head) / VE;
-    float l[VE] = {};
+    float l[VE]; /* entries past the n are masked */
+#pragma unroll
+    for (int j = 1; j < VE; j++) l[j] = -INFINITY;
     if (lane < head) {
         l[0] = clean(fl_to_float(row[x0 + lane]));
         f(x0 + lane, 1, l);
@@ -292,6 +326,8 @@ __device__ __forceinline__ void each(const T* __restrict__ row, int x0, int x1, 
     }
     const int tail = x0 + head + nv * VE + lane;
     if (tail < x1) {
+#pragma unroll
+        for (int j = 1; j < VE; j++) l[j] = -INFINITY;
         l[0] = clean(fl_to_float(row[tail]));
         f(tail, 1, l);
     }
@@ -339,13 +375,14 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) 
 {
     __shared__ Decision s_row[kFinWarps];
     __shared__ int s_ok[kFinWarps];
-    __shared__ double s_table[32], s_warps[2][kFinWarps], s_ranks[2][kCluster];
+    __shared__ double s_table[kTab], s_warps[2][kFinWarps], s_ranks[2][kCluster];
     const int s = blockIdx.x / kCluster, rank = blockIdx.x % kCluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int chunks = chunks_of(g.vocab);
     const RowPart* part = static_cast<const RowPart*>(g.workspace);
     const int r0 = max(g.row_start[s], 0), r1 = min(g.row_start[s + 1], g.n_rows);
     const float t = g.temperature[s];
     const bool greedy = !(t > 0.0f);
+    const double* table = s_table;
     exp64_table(s_table);
     /* what a row's test compares; the first rows' before the wait */
     int x = -1;
@@ -372,12 +409,12 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) 
     for (int base = r0;; base += kFinWarps) {
         const int row = base + warp;
         if (row < r1) {
-            Decision w = merge_row(part + (size_t)row * chunks, chunks, t, s_table);
+            Decision w = merge_row(part + (size_t)row * chunks, chunks, t, table);
             w.row = row;
             bool ok = false;
             if (base > r0) draft_of(row);
             if (x >= 0 && w.m > -INFINITY)
-                ok = greedy ? x == w.best : (double)u * (double)q * w.z < exp64_of(w.m, t, s_table)(l);
+                ok = greedy ? x == w.best : (double)u * (double)q * w.z < exp_over((double)l - (double)w.m, t, table);
             w.rej = row < r1 - 1;
             if (lane == 0) s_row[warp] = w, s_ok[warp] = ok;
         } else if (lane == 0) {
@@ -405,15 +442,18 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) 
     const int per = (g.vocab + kCluster * kFinWarps - 1) / (kCluster * kFinWarps);
     const int x0 = min(g.vocab, (rank * kFinWarps + warp) * per), x1 = min(g.vocab, x0 + per);
     const T* row = static_cast<const T*>(g.logits) + d.row * g.logits_stride;
-    const Exp64 ew = exp64_of(d.m, t, s_table);
+    const Exp64 ew = exp64_of(d.m, t, table);
     const int skip = d.rej && !g.probs ? g.draft[d.row] : -1;
-    double sum = 0.0;
-    each(row, x0, x1, [&](int x, int n, const float* l) {
+    double sum[2] = {0.0, 0.0};
+    each(row, x0, x1, [&](int x, int, const float* l) {
 #pragma unroll
-        for (int j = 0; j < 16 / (int)sizeof(T); j++)
-            if (j < n && x + j != skip) sum += ew(l[j]);
+        for (int j = 0; j < 16 / (int)sizeof(T); j++) {
+            double p, scale;
+            ew(x + j == skip ? -INFINITY : l[j], p, scale);
+            sum[j & 1] = fma(p, scale, sum[j & 1]);
+        }
     });
-    const double z = share(sum, s_warps[0], s_ranks[0]);
+    const double z = share(sum[0] + sum[1], s_warps[0], s_ranks[0]);
     if (!(z > 0.0)) { /* the draft is all of p */
         if (rank == 0) write(skip, threadIdx.x, kFinThreads);
         return;
@@ -421,7 +461,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) 
     double all = z;
     const float* probs = d.rej && g.probs ? g.probs + d.row * g.probs_stride : nullptr;
     if (probs) {
-        sum = 0.0;
+        sum[0] = sum[1] = 0.0;
         each(row, x0, x1, [&](int x, int n, const float* l) {
             constexpr int VE = 16 / (int)sizeof(T);
             float p[VE] = {};
@@ -438,9 +478,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) 
             }
 #pragma unroll
             for (int j = 0; j < VE; j++)
-                if (j < n) sum += fmax(ew(l[j]) - (double)(p[j] > 0.0f ? p[j] : 0.0f) * z, 0.0);
+                sum[j & 1] += fmax(fma((double)(p[j] > 0.0f ? -p[j] : 0.0f), z, ew.value(l[j])), 0.0);
         });
-        all = share(sum, s_warps[1], s_ranks[1]);
+        all = share(sum[0] + sum[1], s_warps[1], s_ranks[1]);
         if (!(all > 0.0)) probs = nullptr, all = z; /* nothing is left of p - q: p itself */
     }
     /* whose range the draw falls into, and the entry in it */
@@ -458,8 +498,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) 
         for (int j = 0; j < 8; j++) {
             e[j] = 0.0;
             if (at + j < x1 && at + j != skip) {
-                e[j] = ew(clean(fl_to_float(row[at + j])));
-                if (probs) e[j] = fmax(e[j] - (double)prob(probs, at + j) * z, 0.0);
+                e[j] = ew.value(clean(fl_to_float(row[at + j])));
+                if (probs) e[j] = fmax(fma(-(double)prob(probs, at + j), z, e[j]), 0.0);
             }
             mine += e[j];
         }
