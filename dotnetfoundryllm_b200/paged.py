@@ -21,6 +21,7 @@ hold their own), and do not synchronize.  Argument errors raise
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -34,7 +35,7 @@ ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # GGML typ
 def _cuda_tensor(name: str, t: torch.Tensor, device: torch.device) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ArgumentError(f"{name} must be a CUDA tensor")
-    if t.device != device:
+    if t.get_device() != device.index:
         raise ArgumentError(f"{name} is on {t.device}, the others on {device}")
 
 
@@ -51,24 +52,29 @@ def _row_type(name: str, dtype: torch.dtype) -> int:
     return rt
 
 
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _enqueue(device: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, stream) on the device's current stream, with that device current for the call."""
+    i = device.index
+    stream = torch._C._cuda_getCurrentRawStream(i)
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, stream)
+    if rc:
+        check(rc, what)
 
 
-class _on:
-    """The device of a call's tensors made current for the call (a no-op when it is)."""
+def _raw(name: str, *types):
+    """The library's entry `name` with descriptors passed as packed bytes, which are quicker to make than ctypes structures."""
+    fn = N.cuda()[name]
+    fn.restype, fn.argtypes = C.c_int, types
+    return fn
 
-    def __init__(self, device: torch.device):
-        self.want = device.index
 
-    def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.want:
-            torch.cuda.set_device(self.want)
-
-    def __exit__(self, *exc):
-        if self.was != self.want:
-            torch.cuda.set_device(self.was)
+# fl_paged_attn_desc, as _native.FlPagedAttnDesc
+_ATTN = struct.Struct("=5i2fiQqQqQQQ")
+assert _ATTN.size == C.sizeof(N.FlPagedAttnDesc)
 
 
 class PagedBatch:
@@ -93,6 +99,8 @@ class PagedBatch:
         self.desc = N.FlPagedBatch(C.sizeof(N.FlPagedBatch), n, page_table.shape[1], max_rows, page_table.data_ptr(),
                                    seq_len.data_ptr(), row_start.data_ptr())
         self._ref = C.byref(self.desc)
+        self._at = C.addressof(self.desc)
+        self._sizes = (n, page_table.shape[1], max_rows)
 
 
 class PagedKvCache:
@@ -132,7 +140,14 @@ class PagedKvCache:
                                 v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
                                 v_scale.data_ptr() if v_scale is not None else None)
         self._ref = C.byref(self.desc)
+        self._at = C.addressof(self.desc)
         self.lib = N.cuda()
+        self._append = _raw("fl_kv_append_device", *[C.c_void_p] * 2, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                            C.c_int64, C.c_void_p)
+        self._gather = _raw("fl_kv_gather_device", *[C.c_void_p] * 2, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                            C.c_int64, C.c_void_p)
+        self._attend = _raw("fl_attn_paged_device", C.c_void_p, C.c_void_p, C.c_char_p, C.c_void_p)
+        self._space: dict[tuple, int] = {}  # workspace bytes by sizes
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype,
@@ -149,7 +164,8 @@ class PagedKvCache:
     def _rows(self, name: str, t: torch.Tensor, heads: int) -> int:
         """Checks a packed row tensor [rows, heads, head_dim]; its row stride in elements."""
         _cuda_tensor(name, t, self.device)
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim:
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim:
             raise ArgumentError(f"{name} must be [rows, {heads}, {self.head_dim}], not {tuple(t.shape)}")
         s = t.stride()
         if s[2] != 1 or (s[1] != self.head_dim and heads > 1):
@@ -157,7 +173,7 @@ class PagedKvCache:
         return s[0]
 
     def _batch(self, batch: PagedBatch) -> None:
-        if batch.device != self.device:
+        if batch.device is not self.device and batch.device != self.device:
             raise ArgumentError(f"the batch is on {batch.device}, the cache on {self.device}")
 
     def append(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -167,9 +183,8 @@ class PagedKvCache:
         ks, vs = self._rows("k", k, self.n_kv_heads), self._rows("v", v, self.n_kv_heads)
         if v.dtype != k.dtype or v.shape[0] != k.shape[0]:
             raise ArgumentError("k and v must have the same type and number of rows")
-        with _on(self.device):
-            check(self.lib.fl_kv_append_device(self._ref, batch._ref, _row_type("k", k.dtype), k.shape[0], k.data_ptr(), ks,
-                                               v.data_ptr(), vs, _stream(self.device)), "fl_kv_append_device")
+        _enqueue(self.device, "fl_kv_append_device", self._append, self._at, batch._at, _row_type("k", k.dtype), k.shape[0],
+                 k.data_ptr(), ks, v.data_ptr(), vs)
 
     def gather(self, batch: PagedBatch, n_rows: int, dtype: torch.dtype = torch.float32,
                out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -188,9 +203,8 @@ class PagedKvCache:
         ks, vs = self._rows("k", k, self.n_kv_heads), self._rows("v", v, self.n_kv_heads)
         if v.dtype != k.dtype or k.shape[0] != n_rows or v.shape[0] != n_rows:
             raise ArgumentError(f"out must be two tensors of one type with {n_rows} rows")
-        with _on(self.device):
-            check(self.lib.fl_kv_gather_device(self._ref, batch._ref, _row_type("out", k.dtype), n_rows, k.data_ptr(), ks,
-                                               v.data_ptr(), vs, _stream(self.device)), "fl_kv_gather_device")
+        _enqueue(self.device, "fl_kv_gather_device", self._gather, self._at, batch._at, _row_type("out", k.dtype), n_rows,
+                 k.data_ptr(), ks, v.data_ptr(), vs)
         return out
 
     def attention(self, batch: PagedBatch, q: torch.Tensor, scale: float, window: int = 0, softcap: float = 0.0,
@@ -217,14 +231,16 @@ class PagedKvCache:
             _cuda_tensor("lse", lse, self.device)
             if lse.dtype != torch.float32 or tuple(lse.shape) != (n_rows, n_heads) or not lse.is_contiguous():
                 raise ArgumentError(f"lse must be a contiguous float32 tensor of shape {(n_rows, n_heads)}")
-        with _on(self.device):
-            need = C.c_uint64()
-            check(self.lib.fl_attn_paged_workspace(self._ref, batch._ref, n_rows, n_heads, C.byref(need)),
-                  "fl_attn_paged_workspace")
-            ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-            d = N.FlPagedAttnDesc(C.sizeof(N.FlPagedAttnDesc), rt, n_rows, n_heads, window, scale, softcap, 0, q.data_ptr(),
-                                  qs, out.data_ptr(), os, lse.data_ptr() if lse is not None else None, ws.data_ptr(),
-                                  need.value)
-            check(self.lib.fl_attn_paged_device(self._ref, batch._ref, C.byref(d), _stream(self.device)),
-                  "fl_attn_paged_device")
+        key = (n_rows, n_heads, batch._sizes)
+        need = self._space.get(key)
+        if need is None:
+            got = C.c_uint64()
+            check(self.lib.fl_attn_paged_workspace(self._ref, batch._ref, n_rows, n_heads, C.byref(got)), "fl_attn_paged_workspace")
+            if len(self._space) >= 4096:
+                self._space.clear()
+            need = self._space[key] = got.value
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        d = _ATTN.pack(_ATTN.size, rt, n_rows, n_heads, window, scale, softcap, 0, q.data_ptr(), qs, out.data_ptr(), os,
+                       lse.data_ptr() if lse is not None else 0, ws.data_ptr(), need)
+        _enqueue(self.device, "fl_attn_paged_device", self._attend, self._at, batch._at, d)
         return out

@@ -8,12 +8,31 @@ speculative decoding.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 
 import torch
 
 from . import _native as N
-from .paged import _cuda_tensor, _int32, _on, _row_type, _stream
+from .paged import _cuda_tensor, _enqueue, _int32, _raw, _row_type
 from .runtime import ArgumentError, check
+
+
+# fl_verify_desc, as _native.FlVerifyDesc
+_DESC = struct.Struct("=6iQqQq9Q")
+assert _DESC.size == C.sizeof(N.FlVerifyDesc)
+
+
+@functools.lru_cache(maxsize=None)
+def _entry():
+    return _raw("fl_verify_device", C.c_char_p, C.c_void_p)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(rows: int, n: int, vocab: int) -> int:
+    need = C.c_uint64()
+    check(N.cuda().fl_verify_workspace(rows, n, vocab, C.byref(need)), "fl_verify_workspace")
+    return need.value
 
 
 def _floats(name: str, t: torch.Tensor, n: int, device: torch.device) -> None:
@@ -60,15 +79,12 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, draft: torch.Te
     else:
         _int32("tokens", tokens, (rows,), device)
     accepted = torch.empty(n, dtype=torch.int32, device=device)
-    lib = N.cuda()
-    with _on(device):
-        need = C.c_uint64()
-        check(lib.fl_verify_workspace(rows, n, vocab, C.byref(need)), "fl_verify_workspace")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-        d = N.FlVerifyDesc(C.sizeof(N.FlVerifyDesc), rt, rows, n, vocab, 0, logits.data_ptr(), logits.stride(0),
-                           draft_probs.data_ptr() if draft_probs is not None else None,
-                           draft_probs.stride(0) if draft_probs is not None else 0, row_start.data_ptr(), draft.data_ptr(),
-                           temperature.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(), tokens.data_ptr(),
-                           accepted.data_ptr(), ws.data_ptr(), need.value)
-        check(lib.fl_verify_device(C.byref(d), _stream(device)), "fl_verify_device")
+    need = _workspace_bytes(rows, n, vocab)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    d = _DESC.pack(_DESC.size, rt, rows, n, vocab, 0, logits.data_ptr(), logits.stride(0),
+                   draft_probs.data_ptr() if draft_probs is not None else 0,
+                   draft_probs.stride(0) if draft_probs is not None else 0, row_start.data_ptr(), draft.data_ptr(),
+                   temperature.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
+                   ws.data_ptr(), need)
+    _enqueue(device, "fl_verify_device", _entry(), d)
     return tokens, accepted
