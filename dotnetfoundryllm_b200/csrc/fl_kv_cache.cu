@@ -14,39 +14,71 @@ namespace {
 
 constexpr int kThreads = 256;
 
-/* q = x / s rounded to the nearest integer, ties to even, from the exact
- * quotient: x * (1/s) is off by a few ulp at most, so the rounded candidate
- * can only be wrong next to a border k + 1/2; the remainder x - q s is exact in
- * one FMA (a multiple of the smaller ulp, at most about s/2), and comparing
- * it with s/2 decides. */
-__device__ __forceinline__ int quant_q8(float x, float s, float inv)
+/* Eight quotients x / s rounded to the nearest integer, ties to even, as bytes.
+ * x * (1/s) is off by a few ulp at most, so the rounded candidate can only be
+ * wrong next to a border k + 1/2: the remainder x - q s is exact in one FMA (a
+ * multiple of the smaller ulp, at most about s/2), and where it reaches s/2,
+ * which is rare, it decides.  Adding 1.5 2^23 rounds, and leaves the byte in the
+ * low bits: no conversion instructions, whose rate bound the kernel. */
+__device__ __forceinline__ uint2 quant_q8(const float (&x)[8], float s, float inv)
 {
-    float q = rintf(x * inv);
-    const float r = fmaf(-q, s, x), h = 0.5f * s;
-    if (fabsf(r) >= h) {
-        const float up = r > 0.0f ? 1.0f : -1.0f;
-        if (fabsf(r) > h || ((int)q & 1)) q += up;
+    constexpr float kMagic = 12582912.0f;
+    const float h = 0.5f * s;
+    float t[8];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        t[i] = fmaf(x[i], inv, kMagic);
+        near |= fabsf(fmaf(kMagic - t[i], s, x[i])) >= h;
     }
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float q = t[i] - kMagic;
+            const float r = fmaf(-q, s, x[i]);
+            if (fabsf(r) > h || (fabsf(r) == h && ((int)q & 1))) q += r > 0.0f ? 1.0f : -1.0f;
+            t[i] = fminf(fmaxf(q, -127.0f), 127.0f) + kMagic; /* a subnormal scale is rounded itself */
+        }
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        w[i] = __byte_perm(__byte_perm(__float_as_uint(t[4 * i]), __float_as_uint(t[4 * i + 1]), 0x0040),
+                           __byte_perm(__float_as_uint(t[4 * i + 2]), __float_as_uint(t[4 * i + 3]), 0x0040), 0x5410);
+    return make_uint2(w[0], w[1]);
 }
 
-/* x / s as a float that rounds to e4m3 as the exact quotient does.  Borders
+/* Eight quotients x / s rounded to e4m3 as the exact quotients round.  Borders
  * between e4m3 values have at most 5 significant bits; where x * (1/s) comes
- * within a few ulp of such a number t, the sign of x - t s (one FMA, exact in
- * sign) tells on which side the quotient lies, and t or its neighbour stands
- * for it. */
-__device__ __forceinline__ float quot_f8(float x, float s, float inv)
+ * within a few ulp of such a number t, which is rare, the sign of x - t s (one
+ * FMA, exact in sign) tells on which side the quotient lies, and t or its
+ * neighbour stands for it. */
+__device__ __forceinline__ uint2 quant_f8(const float (&x)[8], float s, float inv)
 {
-    const float y = x * inv;
-    if (fabsf(y) < 2.4414062e-4f) return y; /* 2^-12: far below half the smallest value, 2^-10 */
-    const uint32_t b = __float_as_uint(y);
-    const uint32_t t = (b + (1u << 18)) & ~((1u << 19) - 1u); /* nearest with 4 fraction bits */
-    const int d = (int)(b - t);
-    if (d > 8 || d < -8) return y;
-    const float tf = __uint_as_float(t);
-    const float r = fmaf(-tf, s, x);
-    if (r == 0.0f) return tf;
-    return __uint_as_float((r > 0.0f) == (tf > 0.0f) ? t + 1u : t - 1u);
+    float y[8];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        y[i] = x[i] * inv;
+        near |= ((__float_as_uint(y[i]) + 8u) & ((1u << 19) - 1u)) <= 16u;
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t b = __float_as_uint(y[i]), t = (b + (1u << 18)) & ~((1u << 19) - 1u); /* 4 fraction bits */
+            const int d = (int)(b - t);
+            /* below 2^-12 everything rounds to 0: half the smallest value is 2^-10 */
+            if (d > 8 || d < -8 || fabsf(y[i]) < 2.4414062e-4f) continue;
+            const float tf = __uint_as_float(t), r = fmaf(-tf, s, x[i]);
+            y[i] = r == 0.0f ? tf : __uint_as_float((r > 0.0f) == (tf > 0.0f) ? t + 1u : t - 1u);
+        }
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[4 * i], y[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
+               (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[4 * i + 2], y[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
+    return make_uint2(w[0], w[1]);
 }
 
 template <int KV>
@@ -86,25 +118,17 @@ __device__ __forceinline__ Packed8<KV> quantize8(const float (&x)[8], float& sca
         constexpr float top = KV == FL_KV_Q8 ? 127.0f : 448.0f;
         const float s = finite ? __fdiv_rn(__uint_as_float(a), top) : __uint_as_float(0x7fffffffu);
         scale = s;
-        uint32_t w[2] = {0, 0};
-        if (s > 0.0f) { /* false for NaN */
-            /* a scale below 2^-100 is scaled up with its row, so that its reciprocal is finite */
-            const float up = s < 7.8886091e-31f ? 1.2676506e30f : 1.0f; /* 2^100 */
-            const float su = s * up, inv = __fdiv_rn(1.0f, su);
+        out.w = make_uint2(0, 0);
+        if (s >= 7.8886091e-31f) { /* 2^-100; false for NaN */
+            out.w = KV == FL_KV_Q8 ? quant_q8(x, s, __fdiv_rn(1.0f, s)) : quant_f8(x, s, __fdiv_rn(1.0f, s));
+        } else if (s > 0.0f) {
+            /* scaled up with its row, so that its reciprocal is finite */
+            float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                uint32_t p;
-                if constexpr (KV == FL_KV_Q8) {
-                    const int q0 = quant_q8(x[i] * up, su, inv), q1 = quant_q8(x[i + 1] * up, su, inv);
-                    p = ((uint32_t)q0 & 0xffu) | (((uint32_t)q1 & 0xffu) << 8);
-                } else {
-                    const float2 f = make_float2(quot_f8(x[i] * up, su, inv), quot_f8(x[i + 1] * up, su, inv));
-                    p = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-                }
-                w[i >> 2] |= p << (8 * (i & 2));
-            }
+            for (int i = 0; i < 8; i++) y[i] = x[i] * 1.2676506e30f; /* 2^100 */
+            const float su = s * 1.2676506e30f;
+            out.w = KV == FL_KV_Q8 ? quant_q8(y, su, __fdiv_rn(1.0f, su)) : quant_f8(y, su, __fdiv_rn(1.0f, su));
         }
-        out.w = make_uint2(w[0], w[1]);
     }
     return out;
 }
@@ -122,15 +146,14 @@ __device__ __forceinline__ void dequantize8(const Packed8<KV>& p, float s, float
     } else {
         const uint32_t w[2] = {p.w.x, p.w.y};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t b = (w[i >> 2] >> (8 * (i & 3))) & 0xffu;
-            float f;
-            if constexpr (KV == FL_KV_Q8) {
-                f = (float)(int8_t)b;
-            } else {
-                f = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+        for (int i = 0; i < 2; i++) {
+            uint32_t h[2];
+            fl_widen4<KV>(w[i], h[0], h[1]);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+                x[4 * i + 2 * j] = f.x * s, x[4 * i + 2 * j + 1] = f.y * s;
             }
-            x[i] = f * s;
         }
     }
 }
@@ -157,31 +180,28 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const FlPaged c, co
     const int64_t warp = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
     const int64_t pair0 = warp * PER_WARP, n_pairs = (int64_t)c.n_rows * c.n_kv;
     if (pair0 >= n_pairs) return;
-    int64_t at[PER_WARP];
+    const int mine = lane / LANES;
+    /* the rows, under way while their places are looked up */
+    float xk[8], xv[8];
+    {
+        const int64_t pair = min(pair0 + mine, n_pairs - 1);
+        const int row = (int)((uint32_t)pair / (uint32_t)c.n_kv), head = (int)(pair - (int64_t)row * c.n_kv);
+        fl_load8(k + row * k_stride + head * HD + e, xk);
+        fl_load8(v + row * v_stride + head * HD + e, xv);
+    }
     /* each pair's place; consecutive pairs are mostly heads of one row */
     int prev = -1, s = -1;
+    int64_t my_at = -1;
 #pragma unroll
     for (int i = 0; i < PER_WARP; i++) {
         const int64_t pair = pair0 + i;
-        at[i] = -1;
         if (pair < n_pairs) {
-            const int row = (int)(pair / c.n_kv), head = (int)(pair - (int64_t)row * c.n_kv);
+            const int row = (int)((uint32_t)pair / (uint32_t)c.n_kv), head = (int)(pair - (int64_t)row * c.n_kv);
             if (row != prev) s = fl_row_seq(c.row_start, c.n_seqs, row);
             prev = row;
-            if (s >= 0) at[i] = fl_cache_row(c, s, __ldg(c.seq_len + s) - (__ldg(c.row_start + s + 1) - row), head);
+            if (s >= 0 && i == mine)
+                my_at = fl_cache_row(c, s, __ldg(c.seq_len + s) - (__ldg(c.row_start + s + 1) - row), head);
         }
-    }
-    const int mine = lane / LANES;
-    int64_t my_at = -1;
-#pragma unroll
-    for (int i = 0; i < PER_WARP; i++)
-        if (i == mine) my_at = at[i];
-    const int64_t pair = pair0 + mine;
-    const int row = (int)(pair / c.n_kv), head = (int)(pair - (int64_t)row * c.n_kv);
-    float xk[8] = {}, xv[8] = {};
-    if (my_at >= 0) {
-        fl_load8(k + row * k_stride + head * HD + e, xk);
-        fl_load8(v + row * v_stride + head * HD + e, xv);
     }
     float sk = 0.0f, sv = 0.0f;
     const Packed8<KV> pk = quantize8<KV, LANES>(xk, sk), pv = quantize8<KV, LANES>(xv, sv);
