@@ -48,37 +48,45 @@ __device__ __forceinline__ uint2 quant_q8(const float (&x)[8], float s, float in
     return make_uint2(w[0], w[1]);
 }
 
-/* Eight quotients x / s rounded to e4m3 as the exact quotients round.  Borders
- * between e4m3 values have at most 5 significant bits; where x * (1/s) comes
- * within a few ulp of such a number t, which is rare, the sign of x - t s (one
- * FMA, exact in sign) tells on which side the quotient lies, and t or its
- * neighbour stands for it. */
-__device__ __forceinline__ uint2 quant_f8(const float (&x)[8], float s, float inv)
+/* Eight numbers as e4m3 bytes. */
+__device__ __forceinline__ uint2 pack_f8(const float (&y)[8])
 {
-    float y[8];
-    bool near = false;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        y[i] = x[i] * inv;
-        near |= ((__float_as_uint(y[i]) + 8u) & ((1u << 19) - 1u)) <= 16u;
-    }
-    if (near) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t b = __float_as_uint(y[i]), t = (b + (1u << 18)) & ~((1u << 19) - 1u); /* 4 fraction bits */
-            const int d = (int)(b - t);
-            /* below 2^-12 everything rounds to 0: half the smallest value is 2^-10 */
-            if (d > 8 || d < -8 || fabsf(y[i]) < 2.4414062e-4f) continue;
-            const float tf = __uint_as_float(t), r = fmaf(-tf, s, x[i]);
-            y[i] = r == 0.0f ? tf : __uint_as_float((r > 0.0f) == (tf > 0.0f) ? t + 1u : t - 1u);
-        }
-    }
     uint32_t w[2];
 #pragma unroll
     for (int i = 0; i < 2; i++)
         w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[4 * i], y[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
                (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[4 * i + 2], y[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
     return make_uint2(w[0], w[1]);
+}
+
+/* Eight quotients x / s rounded to e4m3 as the exact quotients round.  x * (1/s)
+ * is within 2 ulp of the quotient, so where 4 ulp (2^-21) less and 4 ulp more of
+ * it round alike, the quotient does too.  Elsewhere, which is rare, a border
+ * between e4m3 values lies in between: a number t of at most 5 significant bits.
+ * The sign of x - t s (one FMA, exact in sign) tells on which side of t the
+ * quotient lies, and t or its neighbour stands for it. */
+__device__ __forceinline__ uint2 quant_f8(const float (&x)[8], float s, float inv)
+{
+    float y[8];
+    const float lo = fmaf(inv, -4.7683716e-7f, inv), hi = fmaf(inv, 4.7683716e-7f, inv);
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = x[i] * lo;
+    const uint2 a = pack_f8(y);
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = x[i] * hi;
+    const uint2 b = pack_f8(y);
+    if (((a.x ^ b.x) | (a.y ^ b.y)) == 0) return a;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        y[i] = x[i] * inv;
+        const uint32_t b = __float_as_uint(y[i]), t = (b + (1u << 18)) & ~((1u << 19) - 1u); /* 4 fraction bits */
+        const int d = (int)(b - t);
+        /* below 2^-12 everything rounds to 0: half the smallest value is 2^-10 */
+        if (d > 16 || d < -16 || fabsf(y[i]) < 2.4414062e-4f) continue;
+        const float tf = __uint_as_float(t), r = fmaf(-tf, s, x[i]);
+        y[i] = r == 0.0f ? tf : __uint_as_float((r > 0.0f) == (tf > 0.0f) ? t + 1u : t - 1u);
+    }
+    return pack_f8(y);
 }
 
 template <int KV>
