@@ -82,6 +82,17 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t 
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
+/* d += (lo + hi) b with the sum over steps rounded to nearest: the tensor core truncates its sums, which over a
+ * long row of keys adds up to more than fp32 sums would lose. */
+__device__ __forceinline__ void mma_f16_add(float (&d)[4], const uint4& lo, const uint4& hi, uint32_t b0, uint32_t b1)
+{
+    float x[4] = {};
+    mma_f16(x, lo, b0, b1);
+    mma_f16(x, hi, b0, b1);
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] += x[i];
+}
+
 /* All bits of the halves of h that are NaN or infinite. */
 __device__ __forceinline__ uint32_t odd_halves(uint32_t h)
 {
@@ -358,8 +369,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                                 b0 = w[u][n][2 * e], b1 = w[u][n][2 * e + 1];
                             else
                                 fl_widen4<KV>(w[u][n][e], b0, b1);
-                            if (SPLIT) mma_f16(s[u][n], lo, b0, b1);
-                            mma_f16(s[u][n], hi, b0, b1);
+                            if constexpr (SPLIT) {
+                                mma_f16_add(s[u][n], lo, hi, b0, b1);
+                            } else {
+                                mma_f16(s[u][n], hi, b0, b1);
+                            }
                         }
                 }
             }
@@ -539,8 +553,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                                     b1[e] &= ~f1;
                                 }
                             }
-                            if (SPLIT) mma_f16(acc[n], pl[u], b0[e], b1[e]);
-                            mma_f16(acc[n], pa[u], b0[e], b1[e]);
+                            if constexpr (SPLIT) {
+                                mma_f16_add(acc[n], pl[u], pa[u], b0[e], b1[e]);
+                            } else {
+                                mma_f16(acc[n], pa[u], b0[e], b1[e]);
+                            }
                         }
                     }
                 }
