@@ -76,6 +76,9 @@ struct Cfg {
     /* of a key tile: scales of K, of V; (exponent that V's count in, mapped 16-key groups); exponents and findings of the
      * loading warps; values' flags: a byte a key, a bit an element */
     static constexpr int HEAD = BK * 8, EVS = HEAD + 16, BAD = EVS + 32, ODD = BAD + BK, INFO = ODD + BK * HD / 8;
+    /* 32-bit rows: key tiles whose products the tensor core sums before the sum is added to one rounded to nearest.  It
+     * truncates every sum of 16 products, which always errs towards zero: 5.6 k keys in one run were off by 9.5e-6. */
+    static constexpr int RUN = 512 / BK;
     static constexpr int NI = 4;                           /* infos in flight: more than stages, so that they need no release */
     static constexpr int SMEM = QBYTES + STAGES * 2 * TBYTES + NI * INFO + 1024 + 512;
     /* tensor memory columns: two sets of scores (weights over them), the outputs, the weights' low halves */
@@ -235,6 +238,21 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar)
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+/* What sums that count in (m0, e0) are worth where others count in (m, e). */
+__device__ __forceinline__ float part_unit(float m0, float m, int e0, int e)
+{
+    return (m0 == m ? 1.0f : fl_ex2(m0 - m)) * fl_ex2((float)(e0 - e));
+}
+__device__ __forceinline__ void add_part(const float* part, float unit, float (&v)[32])
+{
+#pragma unroll
+    for (int z = 0; z < 32; z += 4) {
+        const float4 p = *reinterpret_cast<const float4*>(part + z);
+        v[z] = fmaf(p.x, unit, v[z]), v[z + 1] = fmaf(p.y, unit, v[z + 1]);
+        v[z + 2] = fmaf(p.z, unit, v[z + 2]), v[z + 3] = fmaf(p.w, unit, v[z + 3]);
+    }
+}
 
 #define FL_F32(c, v) \
     c(v[0]), c(v[1]), c(v[2]), c(v[3]), c(v[4]), c(v[5]), c(v[6]), c(v[7]), c(v[8]), c(v[9]), c(v[10]), c(v[11]), c(v[12]), \
@@ -711,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         if (!(ok = wait_bar(&p_full[buf], (p_ph >> buf) & 1, abort))) break;
                         p_ph ^= 1u << buf;
                         fence_after();
-                        values(q, buf, sv, j > 0);
+                        values(q, buf, sv, SPLIT ? (j & (C::RUN - 1)) != 0 : j > 0);
                         if (NQ == 1) umma_commit(pv_done);
                         if (NQ == 2 && more) {
                             if (q == 0 && !(ok = wait_bar(&k_full[sk], k_par, abort))) break;
@@ -795,6 +813,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             float m = -INFINITY, l = 0.0f;
             int e_acc = -100; /* exponent of the values' scales that O counts in */
             bool any_nan = false;
+            /* where the item's sums are kept: its partial result's place, which is this CTA's */
+            const int slot = 2 * (int)blockIdx.x + (seg.j0 == 0 ? 1 : 0);
+            float* part = ws.o + ((size_t)slot * RT + row) * HD;
+            float m_part = 0.0f; /* the maximum and the exponent that they count in */
+            int e_part = 0;
             for (int j = 0; j < tiles; j++, n++, key0 += BK) {
                 const int st = n % ST, buf = NQ == 1 ? j & 1 : q;
                 const uint8_t* inf = info + (n % C::NI) * C::INFO;
@@ -880,7 +903,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     if (!(ok = wait_warp(&v_full[st], (n / ST) & 1, abort))) break;
                     odd = evs[4] | evs[5] | evs[6] | evs[7];
                 }
-                if (j > 0 && __any_sync(0xffffffffu, moved)) {
+                const bool flush = SPLIT && j > 0 && (j & (C::RUN - 1)) == 0;
+                if (flush || (j > 0 && __any_sync(0xffffffffu, moved))) {
                     if (NQ == 1) {
                         /* the products of the tile before are still counted up; for two row tiles S's came after them */
                         if (!(ok = wait_warp(pv_done, (pv_ph + j - 1) & 1, abort))) break;
@@ -893,9 +917,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         tmem_wait_ld(v);
 #pragma unroll
                         for (int z = 0; z < 32; z++) v[z] *= f;
-                        tmem_st32(lanes + C::O_COL + q * HD + b, v);
+                        if (flush) {
+                            if (j > C::RUN) add_part(part + b, part_unit(m_part, m, e_part, e_acc), v);
+#pragma unroll
+                            for (int z = 0; z < 32; z += 4)
+                                *reinterpret_cast<float4*>(part + b + z) = make_float4(v[z], v[z + 1], v[z + 2], v[z + 3]);
+                        } else {
+                            tmem_st32(lanes + C::O_COL + q * HD + b, v);
+                        }
                     }
-                    tmem_wait_st();
+                    if (flush) {
+                        m_part = m;
+                        e_part = e_acc;
+                    } else {
+                        tmem_wait_st();
+                    }
                 }
                 if (odd) {
                     /* value elements that are NaN or infinite were left out of the products of a tile that not every
@@ -963,7 +999,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 ok = ok && wait_warp(o_full, segs & 1, abort);
                 fence_after();
                 const bool whole = seg.j0 == 0 && seg.j1 == seg.it.tiles;
-                const int slot = 2 * (int)blockIdx.x + (seg.j0 == 0 ? 1 : 0);
                 const int fold = seg.it.f0 + row, i = fl_div_grp(a, fold), h = seg.head * a.grp + fold - i * a.grp;
                 const bool mine = row < seg.it.rows;
                 if (!ok) l = __uint_as_float(0x7fffffffu); /* a wait ran out: NaN, not a number that is wrong */
@@ -975,12 +1010,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 if (mine && whole && a.lse)
                     a.lse[(int64_t)(seg.sw.row0 + i) * a.n_heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147181f;
                 T* out = static_cast<T*>(a.out) + (int64_t)(seg.sw.row0 + i) * a.out_stride + (int64_t)h * HD;
-                float* part = ws.o + ((size_t)slot * RT + row) * HD;
 #pragma unroll
                 for (int b = 0; b < HD; b += 32) {
                     float v[32];
                     tmem_ld32(lanes + C::O_COL + q * HD + b, v);
                     tmem_wait_ld(v);
+                    if (SPLIT && tiles > C::RUN) add_part(part + b, part_unit(m_part, m, e_part, e_acc), v);
 #pragma unroll
                     for (int z = 0; z < 32; z += 8) {
                         float x[8];

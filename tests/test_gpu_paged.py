@@ -372,7 +372,7 @@ def test_attention_window_and_softcap(window, softcap, kv, act, hd, rows):
 @pytest.mark.parametrize("rows", [1, 70])
 def test_attention_pages_and_holes(page, rows):
     """Lengths that end inside a tile and a page, and unmapped pages in the middle."""
-    su = Setup("q8", 64, 1, page, [2 * page + 77, 3 * page, page + 1], [rows] * 3, seed=page)
+    su = Setup("q8", 64, 1, page, [2 * page + 77, 4 * page, page + 1], [rows] * 3, seed=page)
     su.table[1, 1] = -1
     q = torch.randn(su.n_rows, 4, 64, generator=su.g, device=DEV)
     check_attention(su, q, 0.125, out=su.cache.attention(su.batch, q, 0.125))
@@ -418,6 +418,27 @@ def test_what_is_masked_does_not_touch_a_row(kv, act, rows, hd):
         assert torch.equal(got[:rows - 1], clean[:rows - 1])
         assert got[rows - 1].isnan().any()
         assert torch.equal(got[rows:], clean[rows:])
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_32_bit_rows_over_long_sequences_do_not_drift(hd):
+    """Equal weights over values of one sign: the output is their mean.  A tensor
+    core truncates each of its sums of 16 products, by at most 2^-23 of the sum;
+    in a run of 512 keys there are 64 of them (two halves of a weight), and each
+    run's sum, the weights' sum and the quotient are rounded to nearest: at
+    16,000 keys (64 + 32 / 2 + 4) 2^-23 = 1.0e-5 in all."""
+    n, seqs, rows = 16000, 20, 6
+    su = Setup("f16", hd, 4, 64, [n], [rows], seed=hd)
+    su.cache.v.copy_(1 + torch.rand(su.cache.v.shape, generator=su.g, device=DEV))
+    batch = PagedBatch(su.table.repeat(seqs, 1), su.seq_len.repeat(seqs),
+                       torch.arange(seqs + 1, dtype=torch.int32, device=DEV) * rows, max_rows=rows)
+    out = su.cache.attention(batch, torch.zeros(seqs * rows, 32, hd, device=DEV), 0.1).view(seqs, rows, 4, 8, hd).double()
+    V = su.cache.v[su.table[0].long()].double().transpose(1, 2).reshape(-1, 4, hd)[:n].cumsum(0)
+    for i in range(rows):
+        seen = n - rows + i + 1
+        ref = V[seen - 1] / seen
+        worst = ((out[:, i] - ref[None, :, None]).abs() / ref[None, :, None]).max()
+        assert float(worst) < 84 * 2.0 ** -23
 
 
 def test_scores_of_any_size():
