@@ -7,23 +7,53 @@
 
 namespace {
 
-/* Query rows per kv head and sequence, heads of the group included, from which
- * the tcgen05 kernel is taken; below, the streaming one. */
-constexpr int kTcRows = 33;
+/* The tcgen05 kernel is taken from this many 16-row tiles per kv head and
+ * sequence on (heads of the group included), the streaming one below.  The
+ * streaming kernel passes over a sequence's keys once per 16-row tile, so its
+ * time is proportional to the tiles; the tcgen05 kernel's is about the same up to
+ * 128 rows, but higher for 8 bits (every element is widened into shared memory)
+ * and for 32-bit rows (twice the products), which is why the border moves.
+ * Measured in us, streaming / tcgen05, 8 kv heads of 4, 16 sequences of 4096 keys:
+ *   rows               16         20         48         64
+ *   f16,  F16, 64    42 /  70   65 /  70   90 /  73  113 /  74   from 3 tiles
+ *   f16,  F16, 128   71 /  84  119 /  86  174 /  95  228 /  96   from 2
+ *   f16,  F16, 256  161 / 139  296 / 146  442 / 163  583 / 167   from 2
+ *   f16,  Q8,  64    31 /  81   49 /  81   67 /  82   85 /  83   from 4
+ *   bf16, Q8,  128   47 / 110   77 / 111  110 / 116  140 / 117   from 4
+ *   bf16, Q8,  256   86 / 163  144 / 166  212 / 183  275 / 185   from 3
+ *   bf16, F8,  64    39 /  85   63 /  85   89 /  86  113 /  87   from 3
+ *   bf16, F8,  128   72 / 117  120 / 119  172 / 124  223 / 126   from 3
+ *   bf16, F8,  256  147 / 172  261 / 176  381 / 192  513 / 194   from 2
+ *   f32,  F16, 64    47 / 118   73 / 118  102 / 120  129 / 121   from 4
+ *   f32,  F16, 128   89 / 139  152 / 139  223 / 148  297 / 150   from 2
+ *   f32,  F16, 256  256 / 269  478 / 273  715 / 291  944 / 292   from 2
+ *   f32,  Q8,  64    39 / 141   62 / 141   87 / 146  111 / 144   from 6
+ *   f32,  Q8,  128   61 / 179  101 / 179  145 / 184  185 / 186   from 5
+ *   f32,  Q8,  256  139 / 298  252 / 304  381 / 319  499 / 320   from 3
+ *   f32,  F8,  64    46 / 140   76 / 140  107 / 145  136 / 145   from 5
+ *   f32,  F8,  128   89 / 187  151 / 188  218 / 193  280 / 194   from 3
+ *   f32,  F8,  256  301 / 308  566 / 314  846 / 329 1117 / 329   from 2 */
+int tc_tiles(int kv_dtype, int hd, bool wide)
+{
+    static constexpr int8_t from[2][3][3] = {{{3, 2, 2}, {4, 4, 3}, {3, 3, 2}}, {{4, 2, 2}, {6, 5, 3}, {5, 3, 2}}};
+    return from[wide][kv_dtype - FL_KV_F16][hd == 64 ? 0 : hd == 128 ? 1 : 2];
+}
 
-/* The rows of a sequence: the caller's bound, else the average. */
-bool takes_tc(const FlPaged& c, int n_heads)
+/* The rows of a sequence are the caller's bound, else the average.  `wide`: 32-bit rows. */
+bool takes_tc(const FlPaged& c, int n_heads, bool wide)
 {
     const int rows = c.max_rows > 0 ? c.max_rows : c.n_seqs > 0 ? (c.n_rows + c.n_seqs - 1) / c.n_seqs : 0;
-    return (int64_t)rows * (n_heads / c.n_kv) >= kTcRows;
+    return (int64_t)rows * (n_heads / c.n_kv) > flps::kRows * (tc_tiles(c.kv_dtype, c.hd, wide) - 1);
 }
 
 } // namespace
 
+/* For every row type: 16-bit rows take the tcgen05 kernel wherever 32-bit ones do, and its space is the larger. */
 size_t fl_paged_attn_workspace(const FlPaged& c, int n_heads)
 {
     size_t bytes;
-    if (takes_tc(c, n_heads)) /* row tiles of 256 where two fit, which the bound takes for all types */
+    static_assert(flpt::kMaxCtas * 128 >= flps::kMaxCtas * flps::kRows, "the space of either kernel");
+    if (takes_tc(c, n_heads, false)) /* row tiles of 256 where two fit, which the bound takes for all types */
         fl_attn_space(nullptr, c.n_seqs, flpt::kMaxCtas, c.hd == 256 ? 128 : 256, c.hd, &bytes);
     else
         fl_attn_space(nullptr, c.n_seqs, flps::kMaxCtas, flps::kRows, c.hd, &bytes);
@@ -32,7 +62,7 @@ size_t fl_paged_attn_workspace(const FlPaged& c, int n_heads)
 
 bool fl_paged_attn_fits(const FlPaged& c, int n_heads)
 {
-    const bool tc = takes_tc(c, n_heads);
+    const bool tc = takes_tc(c, n_heads, true);
     const double rows = tc ? 128 : flps::kRows, keys = tc ? 64 : flps::kTile, start = tc ? flpt::kItemCost : flps::kItemCost;
     const double items = (double)c.n_rows * n_heads / rows + (double)c.n_seqs * c.n_kv;
     return items * (start + (double)((int64_t)c.cols << c.page_shift) / keys + 2) < 4294967295.0;
@@ -40,7 +70,7 @@ bool fl_paged_attn_fits(const FlPaged& c, int n_heads)
 
 cudaError_t fl_launch_paged_attn(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
 {
-    const bool tc = takes_tc(c, a.n_heads);
+    const bool tc = takes_tc(c, a.n_heads, a.type == 0);
     switch (c.hd) {
     case 64: return tc ? fl_launch_paged_tc_hd64(c, a, st) : fl_launch_paged_stream_hd64(c, a, st);
     case 128: return tc ? fl_launch_paged_tc_hd128(c, a, st) : fl_launch_paged_stream_hd128(c, a, st);
