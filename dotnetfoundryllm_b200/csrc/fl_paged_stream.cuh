@@ -35,6 +35,7 @@
 #ifndef FL_PAGED_STREAM_CUH
 #define FL_PAGED_STREAM_CUH
 
+#include <atomic>
 #include <climits>
 
 #include "fl_paged.cuh"
@@ -191,7 +192,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
     for (uint32_t at = w0; at < w1;) {
         while (at - seq_at >= sw.units) {
             seq_at += sw.units;
-            sw = seq_work(c, a, ++seq);
+            if (++seq >= c.n_seqs) return; /* only where row_start decreases */
+            sw = seq_work(c, a, seq);
         }
         /* the segment: tiles [j0, j1) of item (head, row tile) */
         const uint32_t item = (at - seq_at) / sw.cost;
@@ -633,10 +635,10 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const FlPaged c, const FlPagedAttn a)
 {
     const int64_t pair = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
-    if (pair >= (int64_t)c.n_rows * a.n_heads) return;
+    if (pair >= (int64_t)c.n_rows * a.n_heads) return fl_pdl_wait(); /* this grid may not end before the one it depends on */
     const int row = (int)((uint32_t)pair / (uint32_t)a.n_heads), h = (int)(pair - (int64_t)row * a.n_heads);
     const int seq = fl_row_seq(c.row_start, c.n_seqs, row);
-    if (seq < 0) return;
+    if (seq < 0) return fl_pdl_wait();
     const SeqWork sw = seq_work(c, a, seq);
     const int head = fl_div_grp(a, h), f = (row - sw.row0) * a.grp + h - head * a.grp;
     const int item = head * sw.nrt + f / kRows;
@@ -653,7 +655,7 @@ cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
 {
     using C = Cfg<KV, HD, sizeof(T) == 4>;
     static_assert(C::CTAS * 148 <= kMaxCtas, "workspace slots");
-    static int sms[64] = {}; /* SMs of a device, once its kernel is configured */
+    static std::atomic<int> sms[64] = {}; /* SMs of a device, once its kernel is configured */
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -666,7 +668,7 @@ cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
         if (e != cudaSuccess) return e;
         sms[dev] = n < 148 ? n : 148;
     }
-    paged_stream_kernel<T, KV, HD><<<sms[dev] * C::CTAS, kThreads, C::SMEM, st>>>(c, a);
+    paged_stream_kernel<T, KV, HD><<<sms[dev].load() * C::CTAS, kThreads, C::SMEM, st>>>(c, a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const int64_t pairs = (int64_t)c.n_rows * a.n_heads, per_block = kWarps;

@@ -41,6 +41,7 @@
 #ifndef FL_PAGED_TC_CUH
 #define FL_PAGED_TC_CUH
 
+#include <atomic>
 #include <climits>
 #include <type_traits>
 
@@ -352,6 +353,10 @@ struct Segments {
         while (at < end) {
             while (at - seq_at >= head_u * c.n_kv) {
                 seq_at += head_u * c.n_kv;
+                if (seq + 1 >= c.n_seqs) { /* only where row_start decreases */
+                    at = end;
+                    return false;
+                }
                 enter(c, a, seq + 1);
             }
             uint32_t off = at - seq_at;
@@ -1057,10 +1062,10 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const FlPaged c, const
 {
     using C = Cfg<KV, HD, sizeof(T) == 4, std::is_same<T, __nv_bfloat16>::value>;
     const int64_t pair = ((int64_t)blockIdx.x * 128 + threadIdx.x) >> 5;
-    if (pair >= (int64_t)c.n_rows * a.n_heads) return;
+    if (pair >= (int64_t)c.n_rows * a.n_heads) return fl_pdl_wait(); /* this grid may not end before the one it depends on */
     const int row = (int)((uint32_t)pair / (uint32_t)a.n_heads), h = (int)(pair - (int64_t)row * a.n_heads);
     const int seq = fl_row_seq(c.row_start, c.n_seqs, row);
-    if (seq < 0) return;
+    if (seq < 0) return fl_pdl_wait();
     const SeqWork sw = seq_work<C::RT>(c, a, seq);
     const int head = fl_div_grp(a, h), f = (row - sw.row0) * a.grp + h - head * a.grp, rt = f / C::RT;
     /* units of the head's row tiles, and of those before this one */
@@ -1085,7 +1090,7 @@ template <typename T, int KV, int HD>
 cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
 {
     using C = Cfg<KV, HD, sizeof(T) == 4, std::is_same<T, __nv_bfloat16>::value>;
-    static int sms[64] = {}; /* SMs of a device, once its kernel is configured */
+    static std::atomic<int> sms[64] = {}; /* SMs of a device, once its kernel is configured */
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -1101,9 +1106,9 @@ cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
         sms[dev] = n < kMaxCtas ? n : kMaxCtas;
     }
     if (a.softcap > 0.0f)
-        paged_tc_kernel<T, KV, HD, true><<<sms[dev], kThreads, C::SMEM, st>>>(c, a);
+        paged_tc_kernel<T, KV, HD, true><<<sms[dev].load(), kThreads, C::SMEM, st>>>(c, a);
     else
-        paged_tc_kernel<T, KV, HD, false><<<sms[dev], kThreads, C::SMEM, st>>>(c, a);
+        paged_tc_kernel<T, KV, HD, false><<<sms[dev].load(), kThreads, C::SMEM, st>>>(c, a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

@@ -1562,7 +1562,7 @@ static int check_paged(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t n
         return fail(FL_ERR_ARG, "n_pages %d or n_kv_heads %d out of range", kv->n_pages, kv->n_kv_heads);
     if (b->n_seqs < 0 || b->table_cols < 0 || b->max_rows < 0 || n_rows < 0)
         return fail(FL_ERR_ARG, "n_seqs, table_cols, max_rows and n_rows must be >= 0");
-    if ((int64_t)b->table_cols * kv->page_size > INT32_MAX)
+    if ((int64_t)b->table_cols * kv->page_size > INT32_MAX - 4096) /* a tile past the last one is still in range */
         return fail(FL_ERR_ARG, "%d pages of %d positions: positions are out of 32-bit range", b->table_cols, kv->page_size);
     if (!kv->k || !kv->v) return fail(FL_ERR_ARG, "null cache pointer");
     if (misaligned(kv->k, 16) || misaligned(kv->v, 16)) return fail(FL_ERR_ARG, "cache pointers must be 16-byte aligned");
@@ -1682,6 +1682,8 @@ extern "C" int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch*
     p.grp_inv = p.grp > 1 ? ~0ull / (unsigned)p.grp + 1 : 0; /* exact: floor((2^64 - 1) / grp) + 1 >= 2^64 / grp */
     p.window = a->window;
     p.score_unit = a->softcap > 0.0f ? a->scale / a->softcap : a->scale * 1.44269504f;
+    if (!std::isfinite(p.score_unit))
+        return fail(FL_ERR_ARG, "scale %g with softcap %g: their quotient is out of F32's range", a->scale, a->softcap);
     p.softcap = a->softcap;
     p.q = a->q;
     p.q_stride = a->q_stride;
@@ -1696,6 +1698,7 @@ extern "C" int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch*
 static int check_verify_sizes(int32_t n_rows, int32_t n_seqs, int32_t vocab)
 {
     if (n_rows < 0 || n_seqs < 0) return fail(FL_ERR_ARG, "n_rows and n_seqs must be >= 0");
+    if (n_seqs > 1 << 27) return fail(FL_ERR_ARG, "n_seqs %d is more than %d", n_seqs, 1 << 27);
     if (vocab < 1 || vocab > (1 << 24)) return fail(FL_ERR_ARG, "vocab %d is outside [1, %d]", vocab, 1 << 24);
     return FL_OK;
 }
@@ -1724,6 +1727,7 @@ extern "C" int fl_verify_device(const fl_verify_desc* d, void* stream)
         if (d->n_rows > 1 && (d->logits_stride < d->vocab || (d->draft_probs && d->probs_stride < d->vocab)))
             return fail(FL_ERR_ARG, "rows of %d logits or probabilities overlap", d->vocab);
         if (misaligned(d->logits, d->type == 0 ? 4 : 2)) return fail(FL_ERR_ARG, "logits must be aligned to their type");
+        if (misaligned(d->draft_probs, 4)) return fail(FL_ERR_ARG, "draft_probs must be 4-byte aligned");
     }
     const size_t need = fl_verify_workspace_bytes(d->n_rows, d->n_seqs, d->vocab);
     if (d->workspace_bytes < need || (need && !d->workspace) || misaligned(d->workspace, 256))

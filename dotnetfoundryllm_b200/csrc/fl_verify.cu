@@ -545,7 +545,7 @@ cudaError_t launch(const FlVerify& v, cudaStream_t st)
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = v.n_rows > 0 ? 1 : 0; /* with no rows the kernel before is not this call's */
     return cudaLaunchKernelEx(&cfg, verify_finish_kernel<T>, v);
 }
 

@@ -21,6 +21,10 @@ scale * sum_i |q_i k_ji| of the row:
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+from concurrent.futures import ThreadPoolExecutor
+from pathlib import Path
 
 import pytest
 import torch
@@ -528,6 +532,72 @@ def test_another_stream_than_the_default():
         for o in os:
             assert torch.equal(o, outs[0][0])
     check_attention(su, q, 0.1, out=outs[0][0])
+
+
+def test_threads_on_their_own_streams():
+    """Calls from several host threads at once, each on a stream of its own."""
+    su = Setup("q8", 128, 2, 32, [700, 650], [4, 40], seed=4)
+    q = torch.randn(44, 8, 128, generator=su.g, device=DEV).to(torch.bfloat16)
+    one = PagedBatch(su.table, su.seq_len, torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV), max_rows=1)
+    want = su.cache.attention(su.batch, q, 0.09), su.cache.attention(one, q[:2], 0.09)
+    torch.cuda.synchronize()
+
+    def work(_):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [(su.cache.attention(su.batch, q, 0.09), su.cache.attention(one, q[:2], 0.09)) for _ in range(8)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
+
+
+COLD = """
+import torch
+from dotnetfoundryllm_b200.paged import PagedBatch, PagedKvCache
+from dotnetfoundryllm_b200.speculate import verify_drafts
+i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+cache = PagedKvCache.empty(4, 16, 2, 64, torch.int8, "cuda")
+cache.k.zero_(), cache.v.zero_(), cache.k_scale.zero_(), cache.v_scale.zero_()
+batches = [PagedBatch(i32(0, 1, 2, 3).view(1, 4), i32(n), i32(0, n), max_rows=n) for n in (1, 60)]
+x = torch.randn(60, 2, 64, device="cuda")
+q = torch.randn(60, 8, 64, device="cuda")
+logits = torch.randn(2, 1000, device="cuda")
+args = i32(0, 2), i32(5, 0), torch.ones(1, device="cuda"), torch.rand(2, device="cuda"), torch.rand(1, device="cuda")
+def step():
+    out = []
+    for n, b in zip((1, 60), batches):
+        cache.append(b, x[:n], x[:n])
+        out += [cache.attention(b, q[:n], 0.1), *cache.gather(b, n, torch.float16)]
+    return out + list(verify_drafts(logits, *args))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = step()
+g.replay()
+torch.cuda.synchronize()
+b = step()
+assert all(torch.equal(p, q) for p, q in zip(a, b)), "replayed and called results differ"
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    r = subprocess.run([sys.executable, "-c", COLD], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_a_batch_of_absent_sequences_leaves_everything_alone(rows):
+    """Row arrays that are padding throughout: no sequence has a row."""
+    su = Setup("f8", 128, 2, 16, [40, 0], [0, 0])
+    q = torch.randn(rows, 4, 128, generator=su.g, device=DEV)
+    batch = PagedBatch(su.table, su.seq_len, su.row_start, max_rows=rows)
+    out = torch.full_like(q, 7.0)
+    before = su.cache.k.view(torch.uint8).clone()
+    su.cache.append(batch, q[:, :2].contiguous(), q[:, 2:].contiguous())
+    su.cache.attention(batch, q, 0.1, out=out)
+    assert bool((out == 7.0).all()) and torch.equal(su.cache.k.view(torch.uint8), before)
 
 
 def test_refusals_of_tensors():

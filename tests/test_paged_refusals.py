@@ -113,6 +113,8 @@ def test_bad_rows_are_refused(args, code):
     (dict(n_rows=1 << 30), N.FL_ERR_ARG),             # rows x heads past 32 bits
     (dict(scale=float("nan")), N.FL_ERR_ARG),
     (dict(softcap=float("inf")), N.FL_ERR_ARG),
+    (dict(scale=3e38), N.FL_ERR_ARG),                 # out of range in units of log2
+    (dict(softcap=1e-40), N.FL_ERR_ARG),              # scale / softcap likewise
     (dict(reserved=1), N.FL_ERR_ARG),
     (dict(q=None), N.FL_ERR_ARG),
     (dict(q=P + 4), N.FL_ERR_ARG),
@@ -144,6 +146,8 @@ def test_a_workspace_that_is_too_small_is_refused():
     (dict(type=8), N.FL_ERR_UNSUPPORTED),
     (dict(n_rows=-1), N.FL_ERR_ARG),
     (dict(n_seqs=-1), N.FL_ERR_ARG),
+    (dict(n_seqs=1 << 29), N.FL_ERR_ARG),
+    (dict(draft_probs=P + 2, probs_stride=100), N.FL_ERR_ARG),
     (dict(vocab=0), N.FL_ERR_ARG),
     (dict(vocab=(1 << 24) + 1, logits_stride=1 << 25), N.FL_ERR_ARG),
     (dict(reserved=3), N.FL_ERR_ARG),
