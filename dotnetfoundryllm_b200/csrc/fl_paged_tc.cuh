@@ -306,6 +306,20 @@ __device__ __forceinline__ void role_sync(int role)
     asm volatile("bar.sync %0, %1;" ::"r"(role + 1), "r"(role == 4 ? kCopyWarps * 32 : 128) : "memory");
 }
 
+/* Barriers that tell whether any thread passed `bad`: of a role, of the softmax warps. */
+__device__ __forceinline__ bool bar_any(int id, int threads, bool bad)
+{
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n bar.red.or.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(r)
+        : "r"(id), "r"(threads), "r"((uint32_t)bad)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ bool role_any(int role, bool bad) { return bar_any(role + 1, role == 4 ? kCopyWarps * 32 : 128, bad); }
+__device__ __forceinline__ bool pair_any(bool bad) { return bar_any(8, kSoftWarps * 32, bad); }
+
 /* Bounded wait (~2 s); false once it ran out or another role of the CTA gave up. */
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort)
 {
@@ -405,7 +419,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     __shared__ int s_seq;
     __shared__ float s_fr[RT];                    /* score units of a row's scaled q */
     __shared__ Segments<RT, BK> s_seg[5];
-    __shared__ uint32_t s_nan[RT][HD / 32]; /* elements of a row's output that are NaN */
+    __shared__ uint32_t s_nan[256][HD / 32]; /* elements of a row's output that are NaN, as a softmax thread found them */
+    /* one row tile: what the two threads of a row tell each other */
+    constexpr bool PAIR = NQ == 1;
+    __shared__ float2 s_ref[PAIR ? 128 : 1];      /* maximum and exponent of the last tile so far */
+    __shared__ float4 s_end[2][PAIR ? 128 : 1];   /* at a segment's end: l, its maximum, flags, kept sums' maximum */
+    __shared__ int s_end_e[PAIR ? 128 : 1];       /* and their exponent */
+    __shared__ uint64_t s_turn[2][4];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const FlAttnSpace ws = fl_attn_space(a.workspace, c.n_seqs, kMaxCtas, RT, HD);
     fl_pdl_trigger(); /* the merge kernel may take its place; it waits for this grid's end */
@@ -425,7 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             fl_mbar_init(&s_full[b], 1);
             fl_mbar_init(&p_full[b], 4);
         }
-        fl_mbar_init(q_full, NQ * 4);
+        fl_mbar_init(q_full, kSoftWarps);
+        for (int i = 0; i < 8; i++) fl_mbar_init(&s_turn[i >> 2][i & 3], 1);
         fl_mbar_init(o_full, 1);
         fl_mbar_init(pv_done, 1);
         fl_mbar_init(done, 1);
@@ -494,9 +515,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         seg.seq_at = s_at;
         seg.enter(c, a, s_seq);
     }
-    /* the next segment, for all warps of a role */
-    auto next_segment = [&]() {
-        role_sync(role);
+    /* the next segment, for all warps of a role; none once a wait of one of them ran out */
+    auto next_segment = [&](bool ok) {
+        if (role_any(role, !ok)) return false;
         if (leads) seg.more = seg.next(c, a);
         role_sync(role);
         return seg.more;
@@ -514,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         const int k_in = C::ES == 2 ? lt / C::PIECES : (warp & 3) * (32 / C::PIECES) + (lane >> 3) * 4 / C::PIECES * 2 + ((lane >> 2) & 1);
         int n = 0; /* key tiles so far */
         bool ok = true;
-        while (ok && next_segment()) {
+        while (next_segment(ok)) {
             const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max;
             const int see_lo = a.window > 0 ? max(0, pos_min + 1 - a.window) : 0; /* keys that some row sees */
             const int see_hi = min(seg.sw.len, pos_max + 1);
@@ -630,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             const uint32_t mine = C::place(lane / C::PIECES, lane % C::PIECES);
             int n = 0;
             bool ok = true;
-            while (ok && next_segment()) {
+            while (next_segment(ok)) {
                 const int32_t* table = c.table + (size_t)seg.seq * c.cols;
                 const int see_hi = min(seg.sw.len, seg.it.pos_max + 1), head = seg.head, in_page = (1 << c.page_shift) - 1;
                 const int key_end = (seg.it.tile0 + seg.j1) * BK;
@@ -775,19 +796,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int q = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        int n = 0;
-        uint32_t segs = 0, s_ph = 0, pv_ph = 0; /* phases: bit b of s_ph for scores b */
-        bool ok = q < NQ;
-        while (ok && next_segment()) {
+        /* One row tile: the two warps of 32 rows take its key tiles in turn.  A tile's scores are fetched, scaled, curved
+         * and searched for their maximum beside the other warp's exponentials; only the reference goes from one to the
+         * other, tile by tile. */
+        const int mine_q = PAIR ? 0 : q, row = mine_q * 128 + r;
+        int n0 = 0; /* tiles of the segments before */
+        uint32_t segs = 0, s_ph = 0, pv_ph = 0, turns = 0; /* phases: bit b of s_ph for scores b; turns: of the other warp */
+        bool ok = true;
+        while (next_segment(ok)) {
             const int tiles = seg.j1 - seg.j0;
-            const bool live = NQ == 1 || q == 0 || seg.it.rows > 128; /* a second row tile may be empty */
+            const bool live = PAIR || q == 0 || seg.it.rows > 128; /* a second row tile may be empty */
             /* q of this warp's 32 rows, as fp16 of largest magnitude in [2^14, 2^15) */
             {
                 constexpr int LANES = HD / 8, PER = 32 / LANES;
                 const float sign = a.score_unit < 0.0f ? -1.0f : 1.0f;
 #pragma unroll 2
-                for (int x = 0; x < 32; x += PER) {
-                    const int row = q * 128 + quarter * 32 + x + lane / LANES, e = (lane % LANES) * 8;
+                for (int x = PAIR ? q * 16 : 0; x < (PAIR ? q * 16 + 16 : 32); x += PER) {
+                    const int row = mine_q * 128 + quarter * 32 + x + lane / LANES, e = (lane % LANES) * 8;
                     float v[8] = {};
                     if (row < seg.it.rows) {
                         const int f = seg.it.f0 + row, i = fl_div_grp(a, f);
@@ -810,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         l[z] = fl_pack_half2(y0 - f.x, y1 - f.y);
                     }
                     const int rr = quarter * 32 + x + lane / LANES;
-                    const uint32_t at = s_q + q * (SPLIT ? 2 : 1) * C::QTILE + (e >> 6) * 16384 + rr * 128 +
+                    const uint32_t at = s_q + mine_q * (SPLIT ? 2 : 1) * C::QTILE + (e >> 6) * 16384 + rr * 128 +
                                         ((((e >> 3) & 7) ^ (rr & 7)) << 4);
                     sts16(at, h[0], h[1], h[2], h[3]);
                     if (SPLIT) sts16(at + C::QTILE, l[0], l[1], l[2], l[3]);
@@ -818,12 +843,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 fl_fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) fl_mbar_arrive(q_full);
+                if (PAIR) ok = wait_warp(q_full, segs & 1, abort); /* the other warp's rows */
             }
-            const int row = q * 128 + r;
             const float fr = s_fr[row];
             const int pos = row < seg.it.rows ? seg.sw.first + fl_div_grp(a, seg.it.f0 + row) : -1;
             const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max, len = seg.sw.len;
-            int key0 = (seg.it.tile0 + seg.j0) * BK;
+            const int key_first = (seg.it.tile0 + seg.j0) * BK;
             float m = -INFINITY, l = 0.0f;
             int e_acc = -100; /* exponent of the values' scales that O counts in */
             bool any_nan = false;
@@ -832,8 +857,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             float* part = ws.o + ((size_t)slot * RT + row) * HD;
             float m_part = 0.0f; /* the maximum and the exponent that they count in */
             int e_part = 0;
-            for (int j = 0; j < tiles; j++, n++, key0 += BK) {
-                const int st = n % ST, buf = NQ == 1 ? j & 1 : q;
+            for (int j = PAIR ? q : 0; ok && j < tiles; j += PAIR ? 2 : 1) {
+                const int n = n0 + j, key0 = key_first + j * BK, st = n % ST, buf = q;
                 const uint8_t* inf = info + (n % C::NI) * C::INFO;
                 if (!live) continue;
                 if (!(ok = wait_warp(&i_full[n % C::NI], (n / C::NI) & 1, abort))) break;
@@ -895,6 +920,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 } else {
                     mx *= fr;
                 }
+                if (PAIR && j > 0) { /* the other warp's tile moved the reference */
+                    if (!(ok = wait_warp(&s_turn[q ^ 1][quarter], (turns + ((j - 1) >> 1)) & 1, abort))) break;
+                    const float2 ref = s_ref[row];
+                    if (ref.x > m) {
+                        l *= fl_ex2(m - ref.x);
+                        m = ref.x;
+                    }
+                    e_acc = (int)ref.y;
+                }
                 /* O is rescaled when the maximum grew far, or the values' scales did */
                 float f = 1.0f;
                 bool moved = false;
@@ -910,6 +944,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         e_acc = head.x;
                         moved = true;
                     }
+                }
+                if (PAIR) {
+                    s_ref[row] = make_float2(m, (float)e_acc);
+                    __syncwarp();
+                    if (lane == 0) fl_mbar_arrive(&s_turn[q][quarter]);
                 }
                 bool odd = false;
                 if (partial) {
@@ -927,7 +966,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
 #pragma unroll 1
                     for (int b = 0; b < HD; b += 32) {
                         float v[32];
-                        tmem_ld32(lanes + C::O_COL + q * HD + b, v);
+                        tmem_ld32(lanes + C::O_COL + mine_q * HD + b, v);
                         tmem_wait_ld(v);
 #pragma unroll
                         for (int z = 0; z < 32; z++) v[z] *= f;
@@ -937,7 +976,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                             for (int z = 0; z < 32; z += 4)
                                 *reinterpret_cast<float4*>(part + b + z) = make_float4(v[z], v[z + 1], v[z + 2], v[z + 3]);
                         } else {
-                            tmem_st32(lanes + C::O_COL + q * HD + b, v);
+                            tmem_st32(lanes + C::O_COL + mine_q * HD + b, v);
                         }
                     }
                     if (flush) {
@@ -952,10 +991,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                      * row sees whole: the rows that see them have NaN there in the end */
                     const uint32_t* bits = reinterpret_cast<const uint32_t*>(inf + C::ODD);
                     for (int w = 0; w < HD / 32; w++) {
-                        uint32_t b = any_nan ? s_nan[row][w] : 0u;
+                        uint32_t b = any_nan ? s_nan[q * 128 + r][w] : 0u;
                         for (int k = max(0, c_lo + 1); k < min(BK, c_hi + 1); k++)
                             if (head.y >> (k >> 4) & 1) b |= bits[k * (HD / 32) + w];
-                        s_nan[row][w] = b;
+                        s_nan[q * 128 + r][w] = b;
                     }
                     any_nan = true;
                 }
@@ -1008,35 +1047,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 if (lane == 0) fl_mbar_arrive(&p_full[buf]);
             }
             pv_ph += tiles;
+            n0 += tiles;
+            turns += PAIR ? (tiles + q) >> 1 : 0; /* the other warp's tiles */
             /* ── the output ── */
             if (live) {
                 ok = ok && wait_warp(o_full, segs & 1, abort);
                 fence_after();
+                bool nan_pair[2] = {any_nan, any_nan}; /* of this thread, or of both of the row */
+                if constexpr (PAIR) {
+                    /* both threads of a row go on with its whole state, and write half of it */
+                    s_end[q][row] = make_float4(l, m, any_nan ? 1.0f : 0.0f, m_part);
+                    if (q == 0) s_end_e[row] = e_part; /* runs end at even tiles */
+                    ok = !pair_any(!ok);
+                    const float4 a0 = s_end[0][row], a1 = s_end[1][row];
+                    const float2 ref = s_ref[row];
+                    m = ref.x;
+                    e_acc = (int)ref.y;
+                    l = (a0.y == m ? a0.x : a0.x * fl_ex2(a0.y - m)) + (a1.y == m ? a1.x : a1.x * fl_ex2(a1.y - m));
+                    m_part = a0.w;
+                    e_part = s_end_e[row];
+                    nan_pair[0] = a0.z != 0.0f;
+                    nan_pair[1] = a1.z != 0.0f;
+                    pair_any(false);
+                }
                 const bool whole = seg.j0 == 0 && seg.j1 == seg.it.tiles;
                 const int fold = seg.it.f0 + row, i = fl_div_grp(a, fold), h = seg.head * a.grp + fold - i * a.grp;
-                const bool mine = row < seg.it.rows;
+                const bool mine = row < seg.it.rows, first = !PAIR || q == 0;
                 if (!ok) l = __uint_as_float(0x7fffffffu); /* a wait ran out: NaN, not a number that is wrong */
                 /* o counts in 2^(e_acc - kUp); F16's weights, and their sum, in 2^-kUp */
                 const float unit = fl_scale2(1.0f, (C::ES == 1 ? e_acc : 0) - kUp);
                 if (C::ES == 2) l *= 1.0f / (1 << kUp);
                 const float inv = whole ? (l == 0.0f ? 0.0f : unit / l) : unit;
-                if (mine && !whole) ws.ml[slot * RT + row] = make_float2(m, l);
-                if (mine && whole && a.lse)
+                if (mine && first && !whole) ws.ml[slot * RT + row] = make_float2(m, l);
+                if (mine && first && whole && a.lse)
                     a.lse[(int64_t)(seg.sw.row0 + i) * a.n_heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147181f;
                 T* out = static_cast<T*>(a.out) + (int64_t)(seg.sw.row0 + i) * a.out_stride + (int64_t)h * HD;
 #pragma unroll
-                for (int b = 0; b < HD; b += 32) {
+                for (int b0 = 0; b0 < (PAIR ? HD / 2 : HD); b0 += 32) {
+                    const int b = PAIR ? q * (HD / 2) + b0 : b0;
                     float v[32];
-                    tmem_ld32(lanes + C::O_COL + q * HD + b, v);
+                    tmem_ld32(lanes + C::O_COL + mine_q * HD + b, v);
                     tmem_wait_ld(v);
                     if (SPLIT && tiles > C::RUN) add_part(part + b, part_unit(m_part, m, e_part, e_acc), v);
+                    uint32_t nans = 0;
+                    if (PAIR ? nan_pair[0] : nan_pair[q]) nans = s_nan[row][b / 32];
+                    if (PAIR && nan_pair[1]) nans |= s_nan[128 + r][b / 32];
 #pragma unroll
                     for (int z = 0; z < 32; z += 8) {
                         float x[8];
 #pragma unroll
                         for (int y = 0; y < 8; y++) {
                             x[y] = l == 0.0f ? 0.0f : v[z + y] * inv;
-                            if (any_nan && (s_nan[row][b / 32] >> (z + y) & 1u)) x[y] = __uint_as_float(0x7fffffffu);
+                            if (nans >> (z + y) & 1u) x[y] = __uint_as_float(0x7fffffffu);
                         }
                         if (mine && whole) fl_store8(out + b + z, x);
                         if (mine && !whole) fl_store8(part + b + z, x);
