@@ -17,25 +17,25 @@ namespace {
  *   rows               16         20         48         64
  *   f16,  F16, 64    42 /  70   65 /  70   90 /  73  113 /  74   from 3 tiles
  *   f16,  F16, 128   71 /  84  119 /  86  174 /  95  228 /  96   from 2
- *   f16,  F16, 256  161 / 139  296 / 146  442 / 163  583 / 167   from 2
+ *   f16,  F16, 256  161 / 130  296 / 131  442 / 137  583 / 140   from 2
  *   f16,  Q8,  64    31 /  81   49 /  81   67 /  82   85 /  83   from 4
  *   bf16, Q8,  128   47 / 110   77 / 111  110 / 116  140 / 117   from 4
- *   bf16, Q8,  256   86 / 163  144 / 166  212 / 183  275 / 185   from 3
+ *   bf16, Q8,  256   86 / 159  144 / 159  212 / 163  275 / 165   from 3
  *   bf16, F8,  64    39 /  85   63 /  85   89 /  86  113 /  87   from 3
  *   bf16, F8,  128   72 / 117  120 / 119  172 / 124  223 / 126   from 3
- *   bf16, F8,  256  147 / 172  261 / 176  381 / 192  513 / 194   from 2
+ *   bf16, F8,  256  147 / 164  261 / 164  381 / 168  513 / 170   from 2
  *   f32,  F16, 64    47 / 118   73 / 118  102 / 120  129 / 121   from 4
- *   f32,  F16, 128   89 / 139  152 / 139  223 / 148  297 / 150   from 2
- *   f32,  F16, 256  256 / 269  478 / 273  715 / 291  944 / 292   from 2
+ *   f32,  F16, 128   89 / 130  152 / 130  223 / 134  297 / 137   from 2
+ *   f32,  F16, 256  256 / 264  478 / 265  715 / 273  944 / 275   from 2
  *   f32,  Q8,  64    39 / 141   62 / 141   87 / 146  111 / 144   from 6
- *   f32,  Q8,  128   61 / 179  101 / 179  145 / 184  185 / 186   from 5
- *   f32,  Q8,  256  139 / 298  252 / 304  381 / 319  499 / 320   from 3
+ *   f32,  Q8,  128   61 / 164  101 / 164  145 / 167  185 / 169   from 4
+ *   f32,  Q8,  256  139 / 296  252 / 296  381 / 302  499 / 305   from 3
  *   f32,  F8,  64    46 / 140   76 / 140  107 / 145  136 / 145   from 5
- *   f32,  F8,  128   89 / 187  151 / 188  218 / 193  280 / 194   from 3
- *   f32,  F8,  256  301 / 308  566 / 314  846 / 329 1117 / 329   from 2 */
+ *   f32,  F8,  128   89 / 172  151 / 173  218 / 176  280 / 176   from 3
+ *   f32,  F8,  256  301 / 301  566 / 302  846 / 309 1117 / 311   from 2 */
 int tc_tiles(int kv_dtype, int hd, bool wide)
 {
-    static constexpr int8_t from[2][3][3] = {{{3, 2, 2}, {4, 4, 3}, {3, 3, 2}}, {{4, 2, 2}, {6, 5, 3}, {5, 3, 2}}};
+    static constexpr int8_t from[2][3][3] = {{{3, 2, 2}, {4, 4, 3}, {3, 3, 2}}, {{4, 2, 2}, {6, 4, 3}, {5, 3, 2}}};
     return from[wide][kv_dtype - FL_KV_F16][hd == 64 ? 0 : hd == 128 ? 1 : 2];
 }
 
