@@ -43,7 +43,6 @@
 
 #include <atomic>
 #include <climits>
-#include <type_traits>
 
 #include "fl_paged.cuh"
 
@@ -61,7 +60,7 @@ constexpr int kMinUnits = 2;
 constexpr float kLazy = 8.0f; /* log2 of how far weights may exceed 1 */
 constexpr int kUp = 6;        /* weights are stored times 2^kUp: below 2^15 with the values' scales below 2 */
 
-template <int KV, int HD, bool SPLIT, bool BF16>
+template <int KV, int HD, bool SPLIT>
 struct Cfg {
     static constexpr int ES = KV == FL_KV_F16 ? 2 : 1;
     static constexpr int ROW = HD * ES;
@@ -80,9 +79,6 @@ struct Cfg {
         return ES == 2 ? (pc >> 3) * (BK * 128) + key * 128 + (((pc & 7) ^ (key & 7)) << 4)
                        : (pc >> 2) * (BK * 128) + key * 128 + (((pc & 3) * 2 ^ (key & 7)) << 4);
     }
-    /* bf16 rows: V's scales multiply weights that are already fp16, two at a time; each is rounded to 11 bits once more,
-     * far below the output's 8, for half the shared-memory reads (2048 rows at 16384 keys: 682 us, 689 with fp32 scales) */
-    static constexpr bool HALF_V = ES == 1 && BF16;
     /* of a key tile: scales of K, of V; (exponent that V's count in, mapped 16-key groups); exponents and findings of the
      * loading warps; values' flags: a byte a key, a bit an element */
     static constexpr int HEAD = BK * 8, EVS = HEAD + 16, BAD = EVS + 32, ODD = BAD + BK, INFO = ODD + BK * HD / 8;
@@ -400,7 +396,7 @@ template <typename T, int KV, int HD, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, const FlPagedAttn a)
 {
     constexpr bool SPLIT = sizeof(T) == 4;
-    using C = Cfg<KV, HD, SPLIT, std::is_same<T, __nv_bfloat16>::value>;
+    using C = Cfg<KV, HD, SPLIT>;
     constexpr int NQ = C::NQ, BK = C::BK, ST = C::STAGES, RT = C::RT;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = fl_smem_u32(smem_raw), s_base = (raw + 1023u) & ~1023u;
@@ -582,13 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     }
                     role_sync(2);
                     e_run = max(e_run, max(max(evs[0], evs[1]), max(evs[2], evs[3])));
-                    if (lt < BK) {
-                        const float v = fl_scale2(sv, kUp - e_run);
-                        if (C::HALF_V)
-                            reinterpret_cast<__half*>(inf + BK * 4)[lt] = __float2half_rn(v);
-                        else
-                            reinterpret_cast<float*>(inf)[BK + lt] = v;
-                    }
+                    if (lt < BK) reinterpret_cast<float*>(inf)[BK + lt] = fl_scale2(sv, kUp - e_run);
                 }
                 if (lt == 0) *reinterpret_cast<int*>(inf + C::HEAD) = e_run;
                 fl_mbar_arrive(&i_full[n % C::NI]);
@@ -1028,7 +1018,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         for (int y = 0; y < 4; y++) x[z + y] = fl_ex2(x[z + y]);
                         add2(sum[0], sum[1], x[z], x[z + 1]);
                         add2(sum[2], sum[3], x[z + 2], x[z + 3]);
-                        if (C::ES == 1 && !C::HALF_V) {
+                        if (C::ES == 1) {
                             const float4 v4 = *reinterpret_cast<const float4*>(sv + z);
                             mul2(x[z], x[z + 1], v4.x, v4.y);
                             mul2(x[z + 2], x[z + 3], v4.z, v4.w);
@@ -1036,15 +1026,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         const int i = (z - b) / 2;
                         hi[i] = fl_pack_half2(x[z], x[z + 1]);
                         hi[i + 1] = fl_pack_half2(x[z + 2], x[z + 3]);
-                        if (C::HALF_V && (z & 4)) { /* eight scales at a time */
-                            const uint4 v8 = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(sv) + z - 4);
-                            const uint32_t w[4] = {v8.x, v8.y, v8.z, v8.w};
-#pragma unroll
-                            for (int y = 0; y < 4; y++) {
-                                uint32_t& h = hi[i - 2 + y];
-                                h = fl_half2_bits(__hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&w[y])));
-                            }
-                        }
                         if (SPLIT) {
                             const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
                             const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[i + 1]));
@@ -1137,7 +1118,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
 template <typename T, int KV, int HD>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const FlPaged c, const FlPagedAttn a)
 {
-    using C = Cfg<KV, HD, sizeof(T) == 4, std::is_same<T, __nv_bfloat16>::value>;
+    using C = Cfg<KV, HD, sizeof(T) == 4>;
     const int64_t pair = ((int64_t)blockIdx.x * 128 + threadIdx.x) >> 5;
     if (pair >= (int64_t)c.n_rows * a.n_heads) return fl_pdl_wait(); /* this grid may not end before the one it depends on */
     const int row = (int)((uint32_t)pair / (uint32_t)a.n_heads), h = (int)(pair - (int64_t)row * a.n_heads);
@@ -1166,7 +1147,7 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const FlPaged c, const
 template <typename T, int KV, int HD>
 cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
 {
-    using C = Cfg<KV, HD, sizeof(T) == 4, std::is_same<T, __nv_bfloat16>::value>;
+    using C = Cfg<KV, HD, sizeof(T) == 4>;
     static std::atomic<int> sms[64] = {}; /* SMs of a device, once its kernel is configured */
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);

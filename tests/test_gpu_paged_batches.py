@@ -1,0 +1,87 @@
+"""Attention over a paged KV cache for batches that give every SM several items
+(a sequence's kv head, up to 128 or 256 query rows with the heads of its group),
+short and long ones in turn, and for masks and units at the ends of their range.
+The tolerance is derived in test_gpu_paged.py.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged import ACT, DEV, Setup
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(su: Setup, q, scale, window=0, softcap=0.0):
+    """out, lse and the tolerance scales A, X in 64 bits, a sequence at a time."""
+    K, V = su.values("k"), su.values("v")
+    n_rows, H, hd = q.shape
+    grp = H // su.n_kv
+    out = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    A = torch.zeros_like(out)
+    X = torch.zeros(n_rows, H, dtype=torch.float64, device=DEV)
+    lse = torch.full((n_rows, H), -math.inf, dtype=torch.float64, device=DEV)
+    for b, (n, r) in enumerate(zip(su.lens, su.rows)):
+        n_pages = min(-(-n // su.page), su.cols)
+        if r == 0 or n_pages <= 0:
+            continue
+        pages = su.table[b, :n_pages].long()
+        there = ((pages >= 0) & (pages < K.shape[0])).repeat_interleave(su.page)[:n]
+        pages = pages.clamp(0, K.shape[0] - 1)
+        k = K[pages].transpose(1, 2).reshape(-1, su.n_kv, hd)[:n].repeat_interleave(grp, 1)  # [keys, H, hd]
+        v = V[pages].transpose(1, 2).reshape(-1, su.n_kv, hd)[:n].repeat_interleave(grp, 1)
+        at = slice(su.start[b], su.start[b] + r)
+        qq = q[at].double()
+        x = torch.einsum("rhd,nhd->rhn", qq, k) * scale
+        bound = torch.einsum("rhd,nhd->rhn", qq.abs(), k.abs()) * abs(scale)
+        if softcap > 0:
+            x = softcap * torch.tanh(x / softcap)
+        pos = n - r + torch.arange(r, device=DEV)[:, None]
+        key = torch.arange(len(k), device=DEV)[None]
+        seen = (key <= pos) & there[None]
+        if window > 0:
+            seen &= key > pos - window
+        some = seen.any(1)
+        seen = seen[:, None]
+        w = torch.softmax(x.masked_fill(~seen, -math.inf), -1).masked_fill(~some[:, None, None], 0.0)
+        lse[at] = torch.logsumexp(x.masked_fill(~seen, -math.inf), -1)
+        out[at] = torch.einsum("rhn,nhd->rhd", w, v)
+        A[at] = torch.einsum("rhn,nhd->rhd", w, v.abs())
+        X[at] = bound.masked_fill(~seen, 0.0).amax(-1)
+    return out, lse, A, X
+
+
+def check(su, q, scale, window=0, softcap=0.0, **kw):
+    """Calls the operator and compares out and lse, as check_attention of test_gpu_paged.py does."""
+    lse = torch.full(q.shape[:2], 7.0, device=DEV)
+    out = su.cache.attention(su.batch, q, scale, window=window, softcap=softcap, lse=lse, **kw)
+    want, want_lse, A, X = attend(su, q, scale, window, softcap)
+    f32 = q.dtype == torch.float32
+    n = max(1, max(su.lens))
+    score = 4 * (su.hd + 8) * 2.0 ** -24 * X + 2.0 ** -21 * (X + 4)
+    rel = 2 * score[..., None] + (2.0 ** -21 if f32 else 2.0 ** -11) + (n / 16 + 16) * 2.0 ** -23
+    tol = rel * A + torch.finfo(q.dtype).eps / 2 * want.abs() * (1 + rel) + 1e-30
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), f"off by {(err / tol).nan_to_num(math.inf).max().item():.3g} of the tolerance"
+    live = want_lse > -math.inf
+    assert torch.equal(lse == -math.inf, ~live)
+    e = (lse.double() - want_lse).abs()[live]
+    t = (score + 2.0 ** -22 * (want_lse.abs() + 16) + (n / 16 + 16) * 2.0 ** -23)[live]
+    assert (e <= t).all(), f"lse off by {(e / t).nan_to_num(math.inf).max().item():.3g} of the tolerance"
+    return out
+
+
+def queries(su, heads, act, f=1.0):
+    return (f * torch.randn(su.n_rows, heads, su.hd, generator=su.g, device=DEV)).to(ACT[act])
+
+
+@pytest.mark.parametrize("kv,hd,rows", [("f8", 64, 32), ("q8", 64, 32), ("f8", 128, 32), ("q8", 128, 32), ("q8", 256, 32)])
+def test_weights_of_16_bit_rows_are_rounded_once(kv, hd, rows):
+    """Causal prompts, whose first rows have a few large weights: a weight and the scale of its value make one
+    product, and the tolerance has room for one rounding of it to 11 bits."""
+    for seed in range(12):
+        su = Setup(kv, hd, 8, 16, [rows] * 18, [rows] * 18, seed=seed)
+        check(su, queries(su, 32, "bf16"), 1 / math.sqrt(hd))
