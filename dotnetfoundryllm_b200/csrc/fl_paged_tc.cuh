@@ -832,7 +832,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 fl_fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) fl_mbar_arrive(q_full);
-                if (PAIR) ok = wait_warp(q_full, segs & 1, abort); /* the other warp's rows */
+                /* Every warp waits for the others' rows, those of an empty row tile too, which have nothing else to wait
+                 * for: without it they would arrive for later items in place of the warps that still read this one's. */
+                ok = wait_warp(q_full, segs & 1, abort);
             }
             const float fr = s_fr[row];
             const int pos = row < seg.it.rows ? seg.sw.first + fl_div_grp(a, seg.it.f0 + row) : -1;

@@ -85,3 +85,47 @@ def test_weights_of_16_bit_rows_are_rounded_once(kv, hd, rows):
     for seed in range(12):
         su = Setup(kv, hd, 8, 16, [rows] * 18, [rows] * 18, seed=seed)
         check(su, queries(su, 32, "bf16"), 1 / math.sqrt(hd))
+
+
+# cache, rows' type, head size, drafted rows that the tcgen05 kernel takes at 4 heads a group
+SHORT = [("f16", "bf16", 128, 5), ("f16", "f16", 64, 9), ("f16", "f32", 64, 13), ("f16", "f32", 128, 5), ("f16", "bf16", 256, 5),
+         ("q8", "bf16", 128, 13), ("q8", "f16", 64, 13), ("q8", "f32", 64, 21), ("f8", "bf16", 64, 9), ("f8", "f16", 128, 9),
+         ("f8", "f32", 64, 17)]
+
+
+@pytest.mark.parametrize("kv,act,hd,rows", SHORT)
+def test_many_sequences_of_a_few_drafted_rows(kv, act, hd, rows):
+    """100 sequences x 8 kv heads: five or six items an SM, none with a second row tile."""
+    g = torch.Generator().manual_seed(hd + rows)
+    lens = [rows + int(x) for x in torch.randint(0, 700, (100,), generator=g)]
+    su = Setup(kv, hd, 8, 16, lens, [rows] * 100, seed=1)
+    check(su, queries(su, 32, act), 1 / math.sqrt(hd))
+
+
+@pytest.mark.parametrize("kv,act,hd,rows", SHORT)
+def test_many_short_prompts(kv, act, hd, rows):
+    su = Setup(kv, hd, 8, 16, [32] * 96, [32] * 96, seed=2)
+    check(su, queries(su, 32, act), 1 / math.sqrt(hd))
+
+
+@pytest.mark.parametrize("kv,act,hd,rows", SHORT)
+def test_single_tokens_beside_a_chunk(kv, act, hd, rows):
+    g = torch.Generator().manual_seed(hd)
+    lens = [1 + int(x) for x in torch.randint(0, 900, (80,), generator=g)]
+    lens[40] = 1100
+    su = Setup(kv, hd, 8, 32, lens, [1] * 40 + [512] + [1] * 39, seed=3)
+    check(su, queries(su, 32, act), 1 / math.sqrt(hd))
+
+
+@pytest.mark.parametrize("kv,act,hd,rows", SHORT)
+def test_items_with_one_and_with_two_row_tiles_in_turn(kv, act, hd, rows):
+    """Rows that fill a row tile (32 x 4), fall short of it, pass it by one row, fill two and pass two."""
+    kinds = [1, 32, 33, 2, 64, 17, 65, 31, 40, 1, 1, 1, 64, 0, 5]
+    g = torch.Generator().manual_seed(hd + 7)
+    n_rows = [kinds[int(x)] for x in torch.randint(0, len(kinds), (120,), generator=g)]
+    lens = [r + int(x) for r, x in zip(n_rows, torch.randint(0, 300, (120,), generator=g))]
+    su = Setup(kv, hd, 8, 16, lens, n_rows, seed=4)
+    q = queries(su, 32, act)
+    out = check(su, q, 1 / math.sqrt(hd), window=150)
+    for _ in range(3):
+        assert torch.equal(su.cache.attention(su.batch, q, 1 / math.sqrt(hd), window=150), out)
