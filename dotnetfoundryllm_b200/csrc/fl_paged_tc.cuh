@@ -42,6 +42,7 @@
 #define FL_PAGED_TC_CUH
 
 #include <atomic>
+#include <cfloat>
 #include <climits>
 
 #include "fl_paged.cuh"
@@ -798,7 +799,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             /* q of this warp's 32 rows, as fp16 of largest magnitude in [2^14, 2^15) */
             {
                 constexpr int LANES = HD / 8, PER = 32 / LANES;
-                const float sign = a.score_unit < 0.0f ? -1.0f : 1.0f;
+                /* The unit of a row's scores stays a normal number: -infinity, which stands for masked scores, times 0 would
+                 * be NaN.  Rows far below 2^-100 keep fewer bits for it, of scores that are 0 next to the others; with a unit
+                 * of 0 the queries are made 0 instead. */
+                const bool zero = a.score_unit == 0.0f;
+                const float sign = zero ? 0.0f : a.score_unit < 0.0f ? -1.0f : 1.0f;
+                const int up_max = max((int)(__float_as_uint(a.score_unit) >> 23 & 0xffu) - 1, 0);
 #pragma unroll 2
                 for (int x = PAIR ? q * 16 : 0; x < (PAIR ? q * 16 + 16 : 32); x += PER) {
                     const int row = mine_q * 128 + quarter * 32 + x + lane / LANES, e = (lane % LANES) * 8;
@@ -813,8 +819,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     for (int z = 0; z < 8; z++) top = max(top, __float_as_uint(v[z]) & 0x7fffffffu);
 #pragma unroll
                     for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    const int up = top < 0x7f800000u ? 14 + 127 - (int)(top >> 23) : 0;
-                    if (e == 0) s_fr[row] = fl_scale2(fabsf(a.score_unit), -up);
+                    const int up = top < 0x7f800000u ? min(14 + 127 - (int)(top >> 23), up_max) : 0;
+                    if (e == 0) s_fr[row] = zero ? FLT_MIN : fl_scale2(fabsf(a.score_unit), -up);
                     uint32_t h[4], l[4];
 #pragma unroll
                     for (int z = 0; z < 4; z++) {

@@ -129,3 +129,20 @@ def test_items_with_one_and_with_two_row_tiles_in_turn(kv, act, hd, rows):
     out = check(su, q, 1 / math.sqrt(hd), window=150)
     for _ in range(3):
         assert torch.equal(su.cache.attention(su.batch, q, 1 / math.sqrt(hd), window=150), out)
+
+
+@pytest.mark.parametrize("kv,act,hd", [("f16", "bf16", 64), ("f16", "f32", 128), ("q8", "bf16", 128), ("q8", "f16", 256), ("f8", "f32", 64),
+                                       ("f8", "bf16", 256)])
+@pytest.mark.parametrize("rows", [1, 3, 90])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-3, -1e-3, 1e-30, 1e-38])
+def test_units_of_zero_and_queries_of_zero(kv, act, hd, rows, scale):
+    """A scale of 0 gives the mean of what a row sees; so does a row of zeros, whatever the scale; rows of tiny
+    queries are next to it.  The page in the middle is not mapped."""
+    su = Setup(kv, hd, 2, 16, [rows + 200, rows, rows + 37], [rows] * 3, seed=rows)
+    su.table[0, 2] = -1
+    q = queries(su, 8, act)
+    q[::2, ::3] = 0.0
+    q[1::3, 1] *= 1e-30
+    check(su, q, scale)
+    check(su, q, scale, window=70)
+    check(su, q, scale, softcap=30.0)
