@@ -391,9 +391,15 @@ struct Segments {
     }
 };
 
-/* CAP: softcap > 0, a variant of its own because its 128 curves at once cost the
- * plain kernel registers that it does not have to spare. */
-template <typename T, int KV, int HD, bool CAP>
+/* Softcap's variants, each of its own because 128 curves at once cost the plain
+ * kernel registers that it does not have to spare: kCapFolded joins the curve to
+ * the weights' multiply and add, off by some 2^-22 of the cap, which up to kFoldMax
+ * is at most 2^-15 of a weight, a sixteenth of the rounding of one to fp16 (chunk
+ * with heads of 256: 233 us, with the curve by itself 266); kCapCurve, for larger
+ * caps and for 32-bit rows, is off by some 2^-21 of the score. */
+constexpr int kNoCap = 0, kCapFolded = 1, kCapCurve = 2;
+constexpr float kFoldMax = 128.0f;
+template <typename T, int KV, int HD, int CAP>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, const FlPagedAttn a)
 {
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -906,9 +912,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
 #pragma unroll
                     for (int y = 0; y < 4; y++) mx4[y] = fmaxf(mx4[y], x[z + y]);
                 float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), unit_x = fr, shift = 0.0f;
-                if constexpr (CAP) {
+                if constexpr (CAP != kNoCap) {
                     const float cap = a.softcap * 1.44269504f;
-                    if constexpr (SPLIT) {
+                    if constexpr (CAP == kCapCurve) {
                         if (mx > -INFINITY) mx = tanh_of(mx * fr) * cap; /* the curve grows with its argument */
 #pragma unroll
                         for (int z = 0; z < BK; z++)
@@ -916,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                         unit_x = 1.0f;
                     } else {
                         /* cap tanh y = cap - 2 cap d, d = 1 / (e^2y + 1): x becomes d, and the rest goes into the weights'
-                         * own multiply and add.  Off by some 2^-23 cap, which 16-bit rows do not resolve. */
+                         * own multiply and add */
                         const float unit = fr * 2.88539008f;
                         if (mx > -INFINITY) mx = fmaf(-2.0f * cap, recip(fl_ex2(mx * unit) + 1.0f), cap);
 #pragma unroll
@@ -1162,19 +1168,28 @@ cudaError_t launch(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!sms[dev]) {
-        e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD, kNoCap>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+            e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD, kCapCurve>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if constexpr (sizeof(T) == 2)
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(paged_tc_kernel<T, KV, HD, kCapFolded>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return e;
         int n = 0;
         e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess) return e;
         sms[dev] = n < kMaxCtas ? n : kMaxCtas;
     }
-    if (a.softcap > 0.0f)
-        paged_tc_kernel<T, KV, HD, true><<<sms[dev].load(), kThreads, C::SMEM, st>>>(c, a);
-    else
-        paged_tc_kernel<T, KV, HD, false><<<sms[dev].load(), kThreads, C::SMEM, st>>>(c, a);
+    const int grid = sms[dev].load();
+    bool folded = false;
+    if constexpr (sizeof(T) == 2) {
+        folded = a.softcap > 0.0f && a.softcap <= kFoldMax;
+        if (folded) paged_tc_kernel<T, KV, HD, kCapFolded><<<grid, kThreads, C::SMEM, st>>>(c, a);
+    }
+    if (!folded && a.softcap > 0.0f)
+        paged_tc_kernel<T, KV, HD, kCapCurve><<<grid, kThreads, C::SMEM, st>>>(c, a);
+    else if (!folded)
+        paged_tc_kernel<T, KV, HD, kNoCap><<<grid, kThreads, C::SMEM, st>>>(c, a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

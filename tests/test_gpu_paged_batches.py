@@ -1,7 +1,14 @@
 """Attention over a paged KV cache for batches that give every SM several items
 (a sequence's kv head, up to 128 or 256 query rows with the heads of its group),
 short and long ones in turn, and for masks and units at the ends of their range.
-The tolerance is derived in test_gpu_paged.py.
+The tolerance is derived in test_gpu_paged.py; where scores are far apart one more
+part of it counts, since an output may be made of small weights alone (the value of
+the largest is 0 there).  A weight p <= 2^8 is stored as fp16 of 2^6 p times its
+value's scale in units of the largest scale's power of two.  Below 2^-14 the steps of
+fp16 are 2^-24: half a step is 2^-25, so each weight times scale is off by at most
+2^-31 of the largest scale, each product by 2^-31 of that scale and the largest
+element (of the largest value, without scales).  n keys are off by n times that; the
+sum that divides them is at least 1, the weight of the reference.
 """
 from __future__ import annotations
 
@@ -63,7 +70,10 @@ def check(su, q, scale, window=0, softcap=0.0, **kw):
     n = max(1, max(su.lens))
     score = 4 * (su.hd + 8) * 2.0 ** -24 * X + 2.0 ** -21 * (X + 4)
     rel = 2 * score[..., None] + (2.0 ** -21 if f32 else 2.0 ** -11) + (n / 16 + 16) * 2.0 ** -23
-    tol = rel * A + torch.finfo(q.dtype).eps / 2 * want.abs() * (1 + rel) + 1e-30
+    largest = su.cache.v.float().abs().max().item()
+    if su.cache.v_scale is not None:
+        largest *= su.cache.v_scale.abs().max().item()
+    tol = rel * A + torch.finfo(q.dtype).eps / 2 * want.abs() * (1 + rel) + n * 2.0 ** -31 * largest
     err = (out.double() - want).abs()
     assert (err <= tol).all(), f"off by {(err / tol).nan_to_num(math.inf).max().item():.3g} of the tolerance"
     live = want_lse > -math.inf
@@ -146,3 +156,16 @@ def test_units_of_zero_and_queries_of_zero(kv, act, hd, rows, scale):
     check(su, q, scale)
     check(su, q, scale, window=70)
     check(su, q, scale, softcap=30.0)
+
+
+@pytest.mark.parametrize("kv,act,hd", [("f16", "bf16", 64), ("f16", "f16", 128), ("f16", "f32", 128), ("q8", "bf16", 128),
+                                       ("f8", "f16", 256), ("f8", "f32", 64)])
+@pytest.mark.parametrize("rows", [1, 90])
+@pytest.mark.parametrize("softcap", [0.02, 127.0, 129.0, 1e3, 1e4, 1e6, 1e8])
+def test_softcaps_of_any_size(softcap, kv, act, hd, rows):
+    """A cap far above the scores leaves them as they are; q runs to scores of some tens and, of 90 rows, hundreds."""
+    su = Setup(kv, hd, 2, 16, [rows + 250, rows], [rows, rows], seed=int(softcap) % 97)
+    su.table[0, 1] = -1
+    q = queries(su, 8, act, 8.0)
+    q[::5] *= 16
+    check(su, q, 1 / math.sqrt(hd), softcap=softcap)
