@@ -19,7 +19,8 @@ constexpr int kThreads = 256;
  * wrong next to a border k + 1/2: the remainder x - q s is exact in one FMA (a
  * multiple of the smaller ulp, at most about s/2), and where it reaches s/2,
  * which is rare, it decides.  Adding 1.5 2^23 rounds, and leaves the byte in the
- * low bits: no conversion instructions, whose rate bound the kernel. */
+ * low bits: no conversion instructions, whose rate bound the kernel.  |x| is at
+ * most 127 s (1 + 2^-24), which rounds to 127. */
 __device__ __forceinline__ uint2 quant_q8(const float (&x)[8], float s, float inv)
 {
     constexpr float kMagic = 12582912.0f;
@@ -37,7 +38,7 @@ __device__ __forceinline__ uint2 quant_q8(const float (&x)[8], float s, float in
             float q = t[i] - kMagic;
             const float r = fmaf(-q, s, x[i]);
             if (fabsf(r) > h || (fabsf(r) == h && ((int)q & 1))) q += r > 0.0f ? 1.0f : -1.0f;
-            t[i] = fminf(fmaxf(q, -127.0f), 127.0f) + kMagic; /* a subnormal scale is rounded itself */
+            t[i] = q + kMagic;
         }
     }
     uint32_t w[2];
@@ -130,11 +131,12 @@ __device__ __forceinline__ Packed8<KV> quantize8(const float (&x)[8], float& sca
         if (s >= 7.8886091e-31f) { /* 2^-100; false for NaN */
             out.w = KV == FL_KV_Q8 ? quant_q8(x, s, __fdiv_rn(1.0f, s)) : quant_f8(x, s, __fdiv_rn(1.0f, s));
         } else if (s > 0.0f) {
-            /* scaled up with its row, so that its reciprocal is finite */
+            /* scaled up with its row, so that its reciprocal is finite; a subnormal scale is rounded to a whole number of
+             * 2^-149, so that quotients may pass the largest code by any factor below 2: they are cut to it */
             float y[8];
+            const float su = s * 1.2676506e30f, most = top * su; /* 2^100 */
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = x[i] * 1.2676506e30f; /* 2^100 */
-            const float su = s * 1.2676506e30f;
+            for (int i = 0; i < 8; i++) y[i] = fminf(fmaxf(x[i] * 1.2676506e30f, -most), most);
             out.w = KV == FL_KV_Q8 ? quant_q8(y, su, __fdiv_rn(1.0f, su)) : quant_f8(y, su, __fdiv_rn(1.0f, su));
         }
     }
