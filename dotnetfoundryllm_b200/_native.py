@@ -185,6 +185,9 @@ PUBLIC_API = [
                                           C.POINTER(C.c_uint64)]),
     ("fl_attn_paged_device", C.c_int, [C.POINTER(FlPagedKv), C.POINTER(FlPagedBatch), C.POINTER(FlPagedAttnDesc),
                                        C.c_void_p]),
+    ("fl_attn_paged_status", C.c_int, [C.POINTER(C.c_uint32), C.c_void_p]),
+    ("fl_attn_paged_stall", C.c_int, [C.POINTER(FlPagedKv), C.POINTER(FlPagedBatch), C.POINTER(FlPagedAttnDesc),
+                                      C.c_void_p]),
     ("fl_verify_workspace", C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
     ("fl_verify_device", C.c_int, [C.POINTER(FlVerifyDesc), C.c_void_p]),
     ("fl_sample", C.c_int, [C.c_void_p, C.POINTER(FlSamplerDesc), C.c_void_p, C.c_int32, C.c_float,

@@ -295,6 +295,8 @@ struct FlPagedAttn {
     int32_t type, n_heads, grp, window; /* grp: query heads of a kv head */
     unsigned long long grp_inv;         /* floor(2^64 / grp) + 1; 0 for grp = 1 */
     float score_unit;                   /* of q . k: scale * log2(e), or scale / softcap */
+    float unit, q_sign;                 /* its magnitude and sign; 1 and 0 for a unit of 0 */
+    int32_t up_max;                     /* the largest power of two that leaves the unit divided by it a normal number */
     float softcap;
     const void* q;
     int64_t q_stride;
@@ -302,7 +304,11 @@ struct FlPagedAttn {
     int64_t out_stride;
     float* lse;
     void* workspace;
+    unsigned int* expired; /* the device's count of (row, head) outputs whose waits ran out */
+    bool stall;            /* a test: no copy arrives */
 };
+unsigned int* fl_paged_attn_expired(cudaError_t* e); /* that count's address on the current device */
+bool fl_paged_attn_waits(const FlPaged& c, int type, int n_heads); /* whether the kernel taken has waits */
 size_t fl_paged_attn_workspace(const FlPaged& c, int n_heads);
 bool fl_paged_attn_fits(const FlPaged& c, int n_heads); /* the schedule's units stay below 2^32 */
 cudaError_t fl_launch_paged_stream_hd64(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st);

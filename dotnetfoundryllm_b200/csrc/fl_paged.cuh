@@ -163,9 +163,12 @@ __device__ __forceinline__ void fl_cp_async_wait()
 /* The schedule of an attention kernel: units [c * per, (c + 1) * per) are CTA
  * c's range.  All below 2^32, which the host has checked on the largest
  * possible total. */
+constexpr int kFlWaitCtas = 148; /* CTAs at most of the kernel that has waits */
 struct FlSchedule {
     uint32_t total, per;
+    alignas(4) uint8_t expired[kFlWaitCtas]; /* whether a wait of the CTA ran out */
 };
+static_assert(sizeof(FlSchedule) <= 256, "its place in the workspace");
 
 /* Workspace: the schedule, the first unit of each sequence, then the partials'
  * (m, l) and outputs in two slots of `rows` rows per CTA: [2c] for a range that
@@ -192,6 +195,18 @@ __host__ __device__ __forceinline__ FlAttnSpace fl_attn_space(void* p, int n_seq
     at += (size_t)2 * ctas * rows * hd * 4;
     if (bytes) *bytes = at;
     return w;
+}
+
+/* The output of one (row, head) that a wait ran out on: no number, and counted, by a warp. */
+template <typename T, int HD>
+__device__ __forceinline__ void fl_nan_row(const FlPagedAttn& a, int row, int h)
+{
+    const float nan = __uint_as_float(0x7fffffffu);
+    const int lane = threadIdx.x & 31;
+    T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_stride + (int64_t)h * HD;
+    for (int e = lane; e < HD; e += 32) out[e] = fl_from_float<T>(nan);
+    if (a.lse && lane == 0) a.lse[(int64_t)row * a.n_heads + h] = nan;
+    if (lane == 0) atomicAdd(a.expired, 1u);
 }
 
 /* The output of one (row, head) whose item ranges c0 .. c1 share, its row r of

@@ -68,6 +68,27 @@ bool fl_paged_attn_fits(const FlPaged& c, int n_heads)
     return items * (start + (double)((int64_t)c.cols << c.page_shift) / keys + 2) < 4294967295.0;
 }
 
+__device__ unsigned int g_expired;
+
+/* Looked up once per device: in a captured call too, which a lookup does not disturb. */
+unsigned int* fl_paged_attn_expired(cudaError_t* e)
+{
+    static std::atomic<unsigned int*> at[64] = {};
+    int dev = 0;
+    *e = cudaGetDevice(&dev);
+    if (*e == cudaSuccess && (dev < 0 || dev >= 64)) *e = cudaErrorInvalidDevice;
+    if (*e != cudaSuccess) return nullptr;
+    if (!at[dev]) {
+        void* p = nullptr;
+        *e = cudaGetSymbolAddress(&p, g_expired);
+        if (*e != cudaSuccess) return nullptr;
+        at[dev] = static_cast<unsigned int*>(p);
+    }
+    return at[dev];
+}
+
+bool fl_paged_attn_waits(const FlPaged& c, int type, int n_heads) { return takes_tc(c, n_heads, type == 0); }
+
 cudaError_t fl_launch_paged_attn(const FlPaged& c, const FlPagedAttn& a, cudaStream_t st)
 {
     const bool tc = takes_tc(c, a.n_heads, a.type == 0);

@@ -155,7 +155,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
     if (lane == 31) s_scan[warp] = before;
     if (tid == 0) s_seq = -1;
     __syncthreads();
-    FlSchedule sc;
+    struct {
+        uint32_t total, per;
+    } sc;
     sc.total = 0;
     before -= mine;
 #pragma unroll
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
     const unsigned long long w0_64 = (unsigned long long)blockIdx.x * sc.per;
     const uint32_t w0 = (uint32_t)min(w0_64, (unsigned long long)sc.total);
     const uint32_t w1 = (uint32_t)min(w0_64 + sc.per, (unsigned long long)sc.total);
-    if (blockIdx.x == 0 && tid == 0) *ws.sched = sc;
+    if (blockIdx.x == 0 && tid == 0) ws.sched->total = sc.total, ws.sched->per = sc.per;
     const bool find = w0 < w1 && before <= w0 && w0 - before < mine;
     if (find || blockIdx.x == 0) {
         uint32_t at = before;

@@ -42,7 +42,6 @@
 #define FL_PAGED_TC_CUH
 
 #include <atomic>
-#include <cfloat>
 #include <climits>
 
 #include "fl_paged.cuh"
@@ -55,7 +54,7 @@ constexpr int kThreads = (kSoftWarps + kLoadWarps + 4) * 32; /* the last four: o
 /* registers of a softmax, widening and issuing thread, from the launch's 128 each: a softmax thread holds a row of scores */
 constexpr int kSoftRegs = 200, kLoadRegs = 64, kIssueRegs = 48;
 static_assert(kSoftWarps * kSoftRegs + kLoadWarps * kLoadRegs + 4 * kIssueRegs <= kThreads / 32 * 128, "register file");
-constexpr int kMaxCtas = 148;
+constexpr int kMaxCtas = kFlWaitCtas;
 constexpr int kItemCost = 3; /* what starting an item costs, in key tiles */
 constexpr int kMinUnits = 2;
 constexpr float kLazy = 8.0f; /* log2 of how far weights may exceed 1 */
@@ -333,6 +332,16 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
     }
 }
 
+/* *to = *flag, 0 or 1.  Written in C it had the register allocator spill in the softmax loop of the folded softcap (heads
+ * of 256, e4m3: 238 -> 250 us). */
+__device__ __forceinline__ void copy_flag(uint8_t* to, volatile int* flag)
+{
+    asm volatile("{\n .reg .u32 t;\n ld.volatile.shared.u32 t, [%0];\n st.global.u8 [%1], t;\n}\n" ::"r"(
+                     fl_smem_u32(const_cast<int*>(flag))),
+                 "l"(to)
+                 : "memory");
+}
+
 /* The same for a whole warp, which stays together. */
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort)
 {
@@ -482,7 +491,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     fence_before();
     __syncthreads();
     fence_after();
-    FlSchedule sc;
+    struct {
+        uint32_t total, per;
+    } sc;
     sc.total = 0;
     before -= mine;
     for (int w = 0; w < kThreads / 32; w++) {
@@ -493,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     const unsigned long long w0_64 = (unsigned long long)blockIdx.x * sc.per;
     const uint32_t range_lo = (uint32_t)min(w0_64, (unsigned long long)sc.total);
     const uint32_t range_hi = (uint32_t)min(w0_64 + sc.per, (unsigned long long)sc.total);
-    if (blockIdx.x == 0 && tid == 0) *ws.sched = sc;
+    if (blockIdx.x == 0 && tid == 0) ws.sched->total = sc.total, ws.sched->per = sc.per;
     const bool find = range_lo < range_hi && before <= range_lo && range_lo - before < mine;
     if (find || blockIdx.x == 0) {
         uint32_t at = before;
@@ -646,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             const int ct = tid - (kThreads - kCopyWarps * 32);
             const uint32_t mine = C::place(lane / C::PIECES, lane % C::PIECES);
             int n = 0;
-            bool ok = true;
+            bool ok = !a.stall;
             while (next_segment(ok)) {
                 const int32_t* table = c.table + (size_t)seg.seq * c.cols;
                 const int see_hi = min(seg.sw.len, seg.it.pos_max + 1), head = seg.head, in_page = (1 << c.page_shift) - 1;
@@ -805,12 +816,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
             /* q of this warp's 32 rows, as fp16 of largest magnitude in [2^14, 2^15) */
             {
                 constexpr int LANES = HD / 8, PER = 32 / LANES;
-                /* The unit of a row's scores stays a normal number: -infinity, which stands for masked scores, times 0 would
-                 * be NaN.  Rows far below 2^-100 keep fewer bits for it, of scores that are 0 next to the others; with a unit
-                 * of 0 the queries are made 0 instead. */
-                const bool zero = a.score_unit == 0.0f;
-                const float sign = zero ? 0.0f : a.score_unit < 0.0f ? -1.0f : 1.0f;
-                const int up_max = max((int)(__float_as_uint(a.score_unit) >> 23 & 0xffu) - 1, 0);
 #pragma unroll 2
                 for (int x = PAIR ? q * 16 : 0; x < (PAIR ? q * 16 + 16 : 32); x += PER) {
                     const int row = mine_q * 128 + quarter * 32 + x + lane / LANES, e = (lane % LANES) * 8;
@@ -825,12 +830,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                     for (int z = 0; z < 8; z++) top = max(top, __float_as_uint(v[z]) & 0x7fffffffu);
 #pragma unroll
                     for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    const int up = top < 0x7f800000u ? min(14 + 127 - (int)(top >> 23), up_max) : 0;
-                    if (e == 0) s_fr[row] = zero ? FLT_MIN : fl_scale2(fabsf(a.score_unit), -up);
+                    const int up = top < 0x7f800000u ? min(14 + 127 - (int)(top >> 23), a.up_max) : 0;
+                    if (e == 0) s_fr[row] = fl_scale2(a.unit, -up);
                     uint32_t h[4], l[4];
 #pragma unroll
                     for (int z = 0; z < 4; z++) {
-                        const float y0 = fl_scale2(v[2 * z], up) * sign, y1 = fl_scale2(v[2 * z + 1], up) * sign;
+                        const float y0 = fl_scale2(v[2 * z], up) * a.q_sign, y1 = fl_scale2(v[2 * z + 1], up) * a.q_sign;
                         h[z] = fl_pack_half2(y0, y1);
                         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[z]));
                         l[z] = fl_pack_half2(y0 - f.x, y1 - f.y);
@@ -1083,7 +1088,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
                 const bool whole = seg.j0 == 0 && seg.j1 == seg.it.tiles;
                 const int fold = seg.it.f0 + row, i = fl_div_grp(a, fold), h = seg.head * a.grp + fold - i * a.grp;
                 const bool mine = row < seg.it.rows, first = !PAIR || q == 0;
-                if (!ok) l = __uint_as_float(0x7fffffffu); /* a wait ran out: NaN, not a number that is wrong */
                 /* o counts in 2^(e_acc - kUp); F16's weights, and their sum, in 2^-kUp */
                 const float unit = fl_scale2(1.0f, (C::ES == 1 ? e_acc : 0) - kUp);
                 if (C::ES == 2) l *= 1.0f / (1 << kUp);
@@ -1123,6 +1127,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
     fence_before();
     __syncthreads();
     if (warp == kSoftWarps + kLoadWarps) {
+        if (lane == 0) /* where a wait ran out the merge kernel makes the rows of this range NaN */
+            copy_flag(&static_cast<FlSchedule*>(a.workspace)->expired[blockIdx.x], abort);
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -1152,9 +1158,17 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const FlPaged c, const
     const int tiles = item_work<C::RT, C::BK>(a, sw, rt).tiles;
     const FlAttnSpace ws = fl_attn_space(a.workspace, c.n_seqs, kMaxCtas, C::RT, HD);
     fl_pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const uint32_t* flags = reinterpret_cast<const uint32_t*>(ws.sched->expired);
+    const uint32_t any = flags[lane] | (lane < kFlWaitCtas / 4 - 32 ? flags[32 + lane] : 0u);
     const uint32_t per = ws.sched->per;
     const uint32_t t0 = ws.seq_unit[seq] + (uint32_t)head * all + before + kItemCost;
     const int c0 = (int)(t0 / per), c1 = (int)((t0 + tiles - 1) / per);
+    if (__any_sync(0xffffffffu, any != 0)) { /* rare: whether one of the item's ranges is meant */
+        bool expired = false;
+        for (int i = c0 + lane; i <= c1; i += 32) expired |= ws.sched->expired[i] != 0;
+        if (__any_sync(0xffffffffu, expired)) return fl_nan_row<T, HD>(a, row, h);
+    }
     if (c0 != c1) fl_merge_row<T, HD>(a, ws, c0, c1, f % C::RT, C::RT, row, h); /* else written by its range */
 }
 

@@ -1655,8 +1655,8 @@ extern "C" int fl_attn_paged_workspace(const fl_paged_kv* kv, const fl_paged_bat
     return FL_OK;
 }
 
-extern "C" int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_paged_attn_desc* a,
-                                    void* stream)
+static int attn_paged(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_paged_attn_desc* a, bool stall,
+                      void* stream)
 {
     if (!a) return fail(FL_ERR_ARG, "null argument");
     if (a->struct_size != (int32_t)sizeof(fl_paged_attn_desc)) return fail(FL_ERR_ARG, "fl_paged_attn_desc size mismatch");
@@ -1684,6 +1684,12 @@ extern "C" int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch*
     p.score_unit = a->softcap > 0.0f ? a->scale / a->softcap : a->scale * 1.44269504f;
     if (!std::isfinite(p.score_unit))
         return fail(FL_ERR_ARG, "scale %g with softcap %g: their quotient is out of F32's range", a->scale, a->softcap);
+    /* Units of rows are score units divided by what brings the row's queries up.  They stay normal numbers: -infinity,
+     * which stands for masked scores, times 0 would be NaN.  That leaves fewer bits only to rows whose scores are 0 next
+     * to the others'.  With a unit of 0 the queries are made 0 instead. */
+    p.unit = p.score_unit == 0.0f ? 1.0f : std::fabs(p.score_unit);
+    p.q_sign = p.score_unit == 0.0f ? 0.0f : p.score_unit < 0.0f ? -1.0f : 1.0f;
+    p.up_max = std::max(std::ilogb(p.unit) + 126, 0);
     p.softcap = a->softcap;
     p.q = a->q;
     p.q_stride = a->q_stride;
@@ -1691,8 +1697,46 @@ extern "C" int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch*
     p.out_stride = a->out_stride;
     p.lse = a->lse;
     p.workspace = a->workspace;
+    if (stall && !fl_paged_attn_waits(c, p.type, p.n_heads)) return fail(FL_ERR_ARG, "this call's kernel has no waits");
+    p.stall = stall;
+    cudaError_t e;
+    p.expired = fl_paged_attn_expired(&e);
+    CK(e);
     CK(fl_launch_paged_attn(c, p, static_cast<cudaStream_t>(stream)));
     return FL_OK;
+}
+
+extern "C" int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_paged_attn_desc* a,
+                                    void* stream)
+{
+    return attn_paged(kv, b, a, false, stream);
+}
+
+extern "C" int fl_attn_paged_stall(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_paged_attn_desc* a,
+                                   void* stream)
+{
+    return attn_paged(kv, b, a, true, stream);
+}
+
+extern "C" int fl_attn_paged_status(uint32_t* expired, void* stream)
+{
+    if (!expired) return fail(FL_ERR_ARG, "null argument");
+    static std::mutex lock;
+    static uint32_t known[64] = {}; /* the count at a device's last query */
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    cudaError_t e;
+    const unsigned int* at = fl_paged_attn_expired(&e);
+    CK(e);
+    uint32_t now = 0;
+    CK(cudaMemcpyAsync(&now, at, sizeof(now), cudaMemcpyDeviceToHost, static_cast<cudaStream_t>(stream)));
+    CK(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
+    std::lock_guard<std::mutex> g(lock);
+    /* another thread's query may have seen more by now */
+    *expired = (int32_t)(now - known[dev]) > 0 ? now - known[dev] : 0;
+    if (*expired == 0) return FL_OK;
+    known[dev] = now;
+    return fail(FL_ERR_TIMEOUT, "a bounded device wait of fl_attn_paged_device expired");
 }
 
 static int check_verify_sizes(int32_t n_rows, int32_t n_seqs, int32_t vocab)

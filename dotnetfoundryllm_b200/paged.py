@@ -244,3 +244,11 @@ class PagedKvCache:
                        lse.data_ptr() if lse is not None else 0, ws.data_ptr(), need)
         _enqueue(self.device, "fl_attn_paged_device", self._attend, self._at, batch._at, d)
         return out
+
+    def synchronize(self) -> None:
+        """``fl_attn_paged_status``: waits for the current stream of the cache's device and raises
+        ``DeviceTimeoutError`` if a bounded wait of an attention call on that device ran out since
+        the last query; the rows that it concerns are NaN."""
+        expired = C.c_uint32()
+        with torch.cuda.device(self.device):
+            check(self.lib.fl_attn_paged_status(C.byref(expired), torch.cuda.current_stream().cuda_stream), "fl_attn_paged_status")

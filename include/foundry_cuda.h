@@ -369,6 +369,19 @@ int fl_attn_paged_workspace(const fl_paged_kv* kv, const fl_paged_batch* b, int3
                             uint64_t* bytes);
 int fl_attn_paged_device(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_paged_attn_desc* a, void* stream);
 
+/* Whether calls did what they were to do: waits for the work that `stream`
+ * holds so far.  The waits of fl_attn_paged_device's kernels are bounded (2 s);
+ * where one runs out, every (row, head) of that SM's part of the call gets NaN
+ * in out and lse, and the device counts it.  *expired: how many since the last
+ * query on the current device, whichever calls they belong to; FL_ERR_TIMEOUT
+ * if any. */
+int fl_attn_paged_status(uint32_t* expired, void* stream);
+
+/* Test hook: fl_attn_paged_device with every copy held back, so that its
+ * waits run out.  FL_ERR_ARG for a call with so few rows that its kernel has
+ * no waits. */
+int fl_attn_paged_stall(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_paged_attn_desc* a, void* stream);
+
 /* Verification of drafted tokens (speculative decoding) against the target
  * model's logits; the draws are the caller's, as in fl_sample.  Sequence b
  * has rows row_start[b] .. row_start[b+1]-1: row i < last holds the target's

@@ -12,11 +12,14 @@ sum that divides them is at least 1, the weight of the reference.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 import pytest
 import torch
 
+from dotnetfoundryllm_b200 import _native as N
+from dotnetfoundryllm_b200.runtime import DeviceTimeoutError
 from test_gpu_paged import ACT, DEV, Setup
 
 pytestmark = pytest.mark.gpu
@@ -169,3 +172,36 @@ def test_softcaps_of_any_size(softcap, kv, act, hd, rows):
     q = queries(su, 8, act, 8.0)
     q[::5] *= 16
     check(su, q, 1 / math.sqrt(hd), softcap=softcap)
+
+
+@pytest.mark.parametrize("kv,act,hd,lens,rows", [
+    ("f16", "bf16", 128, [700, 300], [500, 90]),            # items cut and whole, two row tiles and one
+    ("q8", "f16", 64, [40] * 60 + [300], [32] * 60 + [17]),  # several short items an SM
+    ("f8", "bf16", 256, [200, 600], [150, 33]),
+    ("q8", "f32", 128, [900], [200]),
+    ("f16", "f32", 64, [64, 2000], [64, 70]),
+])
+def test_a_wait_that_runs_out_is_reported(kv, act, hd, lens, rows):
+    """Copies held back: every row is NaN, whatever the buffers held, rows behind the last sequence stay as they were,
+    the device reports it once, and the next call is right."""
+    su = Setup(kv, hd, 4, 16, lens, rows, seed=hd)
+    c, n = su.cache, su.n_rows + 3
+    q = torch.randn(n, 16, hd, generator=su.g, device=DEV).to(ACT[act])
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((n, 16), 7.0, device=DEV)
+    want = c.attention(su.batch, q[:su.n_rows], 0.1)
+    need = C.c_uint64()
+    assert c.lib.fl_attn_paged_workspace(c._ref, su.batch._ref, n, 16, C.byref(need)) == N.FL_OK
+    ws = torch.zeros(need.value, dtype=torch.uint8, device=DEV)
+    d = N.FlPagedAttnDesc(C.sizeof(N.FlPagedAttnDesc), {"f32": 0, "f16": 1, "bf16": 30}[act], n, 16, 0, 0.1, 0.0, 0, q.data_ptr(),
+                          q.stride(0), out.data_ptr(), out.stride(0), lse.data_ptr(), ws.data_ptr(), need.value)
+    stream = torch.cuda.current_stream().cuda_stream
+    c.synchronize()
+    assert c.lib.fl_attn_paged_stall(c._ref, su.batch._ref, C.byref(d), stream) == N.FL_OK
+    with pytest.raises(DeviceTimeoutError):
+        c.synchronize()
+    c.synchronize()
+    assert out[:su.n_rows].isnan().all() and lse[:su.n_rows].isnan().all()
+    assert (out[su.n_rows:] == 7.0).all() and (lse[su.n_rows:] == 7.0).all()
+    assert torch.equal(c.attention(su.batch, q[:su.n_rows], 0.1), want)
+    c.synchronize()
