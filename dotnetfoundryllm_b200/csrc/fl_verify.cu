@@ -334,7 +334,8 @@ __device__ __forceinline__ void each(const T* __restrict__ row, int x0, int x1, 
 }
 
 /* This warp's sum, put beside the other warps'; the CTA's sum at its rank in
- * every CTA of the cluster; returns the total, the same everywhere. */
+ * every CTA of the cluster, all of which have started; returns the total, the same
+ * everywhere. */
 __device__ __forceinline__ double share(double v, double* warps, double* ranks)
 {
     namespace cg = cooperative_groups;
@@ -398,7 +399,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) 
         u = g.u_accept[row];
     };
     draft_of(r0 + warp);
-    __syncthreads();
+    /* every CTA of the cluster has started before any writes into another's memory (and the table stands); under way
+     * while the first kernel still runs */
+    cooperative_groups::this_cluster().sync();
     fl_pdl_wait();
     if (r1 <= r0) { /* this and every later return: alike in the whole cluster */
         if (rank == 0 && threadIdx.x == 0) g.accepted[s] = 0;
