@@ -340,9 +340,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<KV, HD, sizeof(T) == 4>::CTAS)
                 mapped[u] = __shfl_sync(0xffffffffu, pages, (i + u) & 31) >= 0;
                 any |= mapped[u];
             }
+            if (any) fl_cp_async_wait<C::STAGES - 1>();
+            __syncwarp(); /* scales and zeros are other lanes', and later copies into the place of unread zeros too */
             if (!any) continue;
-            fl_cp_async_wait<C::STAGES - 1>();
-            __syncwarp(); /* scales and zeros are other lanes' */
             const uint8_t* st = ring_p + ((i / U) % C::STAGES) * C::STAGE;
             const int key0 = (tile_first + i * kWarps) * kTile; /* tile u starts at key0 + u * kWarps * kTile */
 

@@ -205,3 +205,17 @@ def test_a_wait_that_runs_out_is_reported(kv, act, hd, lens, rows):
     assert (out[su.n_rows:] == 7.0).all() and (lse[su.n_rows:] == 7.0).all()
     assert torch.equal(c.attention(su.batch, q[:su.n_rows], 0.1), want)
     c.synchronize()
+
+
+@pytest.mark.parametrize("kv,act,hd", [("q8", "bf16", 64), ("f8", "f16", 64), ("q8", "f32", 64), ("q8", "bf16", 128), ("f16", "bf16", 64)])
+@pytest.mark.parametrize("rows", [1, 4, 90])
+@pytest.mark.parametrize("mapped", [0.02, 0.4])
+def test_most_pages_unmapped(kv, act, hd, rows, mapped):
+    """Single pages and runs of them among unmapped ones: places of a ring are zeroed and copied into in turn."""
+    lens = [3000, 1777, rows, 640]
+    su = Setup(kv, hd, 2, 16, lens, [rows] * 4, seed=rows)
+    su.table[torch.rand(su.table.shape, generator=su.g, device=DEV) > mapped] = -1
+    q = queries(su, 8, act)
+    out = check(su, q, 1 / math.sqrt(hd))
+    for _ in range(3):
+        assert torch.equal(su.cache.attention(su.batch, q, 1 / math.sqrt(hd)), out)
