@@ -104,6 +104,8 @@ __device__ __forceinline__ int64_t fl_cache_row(const FlPaged& c, int s, int p, 
 }
 
 /* ── attention helpers ── */
+/* The first position that a row at position p (which may be negative) sees; window > 0, or none. */
+__device__ __forceinline__ int fl_first_seen(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
 __device__ __forceinline__ float fl_ex2(float x)
 {
     float y;

@@ -66,8 +66,7 @@ __device__ __forceinline__ SeqWork seq_work(const FlPaged& c, const FlPagedAttn&
     w.n = max(r1 - r0, 0);
     w.first = len - w.n;
     w.len = max(0, min(len, c.cols << c.page_shift));
-    const int lo = a.window > 0 ? max(0, w.first + 1 - a.window) : 0;
-    w.tile0 = lo / kTile;
+    w.tile0 = fl_first_seen(w.first, a.window) / kTile;
     w.tiles = max(1, (w.len + kTile - 1) / kTile - w.tile0);
     w.nrt = (w.n * a.grp + kRows - 1) / kRows;
     w.cost = kItemCost + w.tiles;

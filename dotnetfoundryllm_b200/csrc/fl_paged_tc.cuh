@@ -123,8 +123,8 @@ __device__ __forceinline__ ItemWork item_work(const FlPagedAttn& a, const SeqWor
     w.rows = min(s.n * a.grp - w.f0, RT);
     w.pos_min = s.first + fl_div_grp(a, w.f0);
     w.pos_max = s.first + fl_div_grp(a, w.f0 + w.rows - 1);
-    const int lo = a.window > 0 ? max(0, w.pos_min + 1 - a.window) : 0, hi = max(0, min(s.len, w.pos_max + 1));
-    w.tile0 = lo / BK;
+    const int hi = max(0, min(s.len, w.pos_max + 1));
+    w.tile0 = fl_first_seen(w.pos_min, a.window) / BK;
     w.tiles = max(1, (hi + BK - 1) / BK - w.tile0);
     return w;
 }
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const FlPaged c, 
         bool ok = true;
         while (next_segment(ok)) {
             const int pos_min = seg.it.pos_min, pos_max = seg.it.pos_max;
-            const int see_lo = a.window > 0 ? max(0, pos_min + 1 - a.window) : 0; /* keys that some row sees */
+            const int see_lo = fl_first_seen(pos_min, a.window); /* keys that some row sees */
             const int see_hi = min(seg.sw.len, pos_max + 1);
             const int key_end = (seg.it.tile0 + seg.j1) * BK;
             int e_run = -100;

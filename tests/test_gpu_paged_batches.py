@@ -219,3 +219,12 @@ def test_most_pages_unmapped(kv, act, hd, rows, mapped):
     out = check(su, q, 1 / math.sqrt(hd))
     for _ in range(3):
         assert torch.equal(su.cache.attention(su.batch, q, 1 / math.sqrt(hd)), out)
+
+
+@pytest.mark.parametrize("kv,act,hd", [("f16", "bf16", 64), ("q8", "bf16", 128), ("f8", "f32", 256)])
+@pytest.mark.parametrize("rows", [7, 90])
+@pytest.mark.parametrize("window", [1, 2 ** 30, 2 ** 31 - 50, 2 ** 31 - 1])
+def test_the_largest_windows_with_rows_before_the_first_position(window, kv, act, hd, rows):
+    """A padded sequence: fewer positions than rows, so that its first rows lie at negative positions and see nothing."""
+    su = Setup(kv, hd, 2, 16, [rows // 2, rows + 300, 1], [rows, rows, rows], seed=rows)
+    check(su, queries(su, 8, act), 1 / math.sqrt(hd), window=window)
