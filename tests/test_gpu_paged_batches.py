@@ -68,7 +68,13 @@ def check(su, q, scale, window=0, softcap=0.0, **kw):
     """Calls the operator and compares out and lse, as check_attention of test_gpu_paged.py does."""
     lse = torch.full(q.shape[:2], 7.0, device=DEV)
     out = su.cache.attention(su.batch, q, scale, window=window, softcap=softcap, lse=lse, **kw)
-    want, want_lse, A, X = attend(su, q, scale, window, softcap)
+    compare(su, q, scale, window, softcap, out, lse)
+    return out
+
+
+def compare(su, q, scale, window, softcap, out, lse, rows=slice(None)):
+    want, want_lse, A, X = (t[rows] for t in attend(su, q, scale, window, softcap))
+    out, lse = out[rows], lse[rows]
     f32 = q.dtype == torch.float32
     n = max(1, max(su.lens))
     score = 4 * (su.hd + 8) * 2.0 ** -24 * X + 2.0 ** -21 * (X + 4)
@@ -84,7 +90,6 @@ def check(su, q, scale, window=0, softcap=0.0, **kw):
     e = (lse.double() - want_lse).abs()[live]
     t = (score + 2.0 ** -22 * (want_lse.abs() + 16) + (n / 16 + 16) * 2.0 ** -23)[live]
     assert (e <= t).all(), f"lse off by {(e / t).nan_to_num(math.inf).max().item():.3g} of the tolerance"
-    return out
 
 
 def queries(su, heads, act, f=1.0):
@@ -228,3 +233,24 @@ def test_the_largest_windows_with_rows_before_the_first_position(window, kv, act
     """A padded sequence: fewer positions than rows, so that its first rows lie at negative positions and see nothing."""
     su = Setup(kv, hd, 2, 16, [rows // 2, rows + 300, 1], [rows, rows, rows], seed=rows)
     check(su, queries(su, 8, act), 1 / math.sqrt(hd), window=window)
+
+
+@pytest.mark.parametrize("kv,act,hd", [("f16", "bf16", 64), ("q8", "bf16", 128), ("f8", "f32", 256)])
+@pytest.mark.parametrize("rows", [3, 90])
+@pytest.mark.parametrize("window", [0, 1, 40, 2 ** 31 - 60])
+def test_lengths_that_are_far_past_the_table_or_negative(window, kv, act, hd, rows):
+    """Rows at positions up to 2^31 - 2, none of whose keys but the table's are there; beside a sequence of the usual kind."""
+    su = Setup(kv, hd, 2, 16, [rows + 90, rows, rows + 30, 48], [rows] * 4, seed=rows)
+    q = queries(su, 8, act)
+    su.seq_len.copy_(torch.tensor([2 ** 31 - 1, -2 ** 31, rows + 30, -1], dtype=torch.int32))
+    lse = torch.full(q.shape[:2], 7.0, device=DEV)
+    out = su.cache.attention(su.batch, q, 0.1, window=window, lse=lse)
+    su.cache.synchronize()
+    compare(su, q, 0.1, window, 0.0, out, lse, slice(2 * rows, 3 * rows))
+    for at in ([1, 3] if window in (0, 2 ** 31 - 60) else [0, 1, 3]):
+        assert (out[at * rows:(at + 1) * rows] == 0).all() and (lse[at * rows:(at + 1) * rows] == -math.inf).all()
+    if window == 0:  # every position of the table
+        su.lens[0] = su.cols * su.page + rows
+        compare(su, q, 0.1, window, 0.0, out, lse, slice(0, rows))
+    su.cache.append(su.batch, q[:, :2].contiguous(), q[:, 2:4].contiguous())
+    torch.cuda.synchronize()
