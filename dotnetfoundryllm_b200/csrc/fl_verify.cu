@@ -44,6 +44,14 @@ struct Decision { /* of a sequence */
 
 __host__ __device__ __forceinline__ int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
 
+/* An infinite temperature is the largest finite one, at which logits of the usual size weigh the same too: divided by
+ * infinity, masked ones would be NaN. */
+__device__ __forceinline__ float temperature_of(const FlVerify& g, int s)
+{
+    const float t = g.temperature[s];
+    return t > FLT_MAX ? FLT_MAX : t; /* NaN stays: greedy */
+}
+
 /* NaN is masked, +infinity is the largest finite value. */
 __device__ __forceinline__ float clean(float l) { return l != l ? -INFINITY : fminf(l, FLT_MAX); }
 
@@ -200,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g)
     if (tail < n) ends[1] = clean(fl_to_float(l[x0 + tail]));
     const int s = fl_row_seq(g.row_start, g.n_seqs, row); /* while they are under way */
     if (s < 0) return;
-    const float t = g.temperature[s];
+    const float t = temperature_of(g, s);
     float m = fmaxf(ends[0], ends[1]);
 #pragma unroll
     for (int i = 0; i < NV; i++)
@@ -381,7 +389,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kFinThreads) 
     const int chunks = chunks_of(g.vocab);
     const RowPart* part = static_cast<const RowPart*>(g.workspace);
     const int r0 = max(g.row_start[s], 0), r1 = min(g.row_start[s + 1], g.n_rows);
-    const float t = g.temperature[s];
+    const float t = temperature_of(g, s);
     const bool greedy = !(t > 0.0f);
     const double* table = s_table;
     exp64_table(s_table);

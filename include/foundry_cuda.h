@@ -393,8 +393,9 @@ int fl_attn_paged_stall(const fl_paged_kv* kv, const fl_paged_batch* b, const fl
  * token is drawn from max(p - q, 0) (from p if that is 0 everywhere); with all
  * accepted, from p of the last row.  The draw is the first x whose cumulative
  * weight exceeds u_sample[b] times the total; sums are in 64 bits.
- * temperature[b] <= 0 is greedy: accepted iff draft is the argmax (first
- * maximum), the token is the argmax.
+ * temperature[b] <= 0 (or NaN) is greedy: accepted iff draft is the argmax
+ * (first maximum), the token is the argmax.  Infinity counts as the largest
+ * F32.
  * tokens[row]: the accepted drafts, then the token, then -1; accepted[b]: how
  * many drafts were accepted.  Entries of rows behind the last sequence are
  * left alone; accepted is 0 for a sequence without rows.
