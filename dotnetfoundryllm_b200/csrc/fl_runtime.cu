@@ -1777,6 +1777,9 @@ extern "C" int fl_verify_device(const fl_verify_desc* d, void* stream)
     if (d->workspace_bytes < need || (need && !d->workspace) || misaligned(d->workspace, 256))
         return fail(FL_ERR_ARG, "workspace: %llu bytes, 256-byte aligned, are needed (fl_verify_workspace)",
                     (unsigned long long)need);
+    const uintptr_t tok = reinterpret_cast<uintptr_t>(d->tokens), drf = reinterpret_cast<uintptr_t>(d->draft);
+    if (tok < drf + (size_t)d->n_rows * 4 && drf < tok + (size_t)d->n_rows * 4) /* written while others still read it */
+        return fail(FL_ERR_ARG, "tokens may not overlap draft");
     FlVerify v;
     v.type = d->type;
     v.n_rows = d->n_rows;

@@ -53,7 +53,8 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, draft: torch.Te
     float32, the distributions the drafts were drawn from, or None when each
     was certain.  Returns tokens [rows] int32 (the accepted drafts, the token
     after them, then -1) and accepted [n_seqs] int32.  Entries of ``tokens``
-    behind the last sequence are left as they were (undefined when new)."""
+    behind the last sequence are left as they were (undefined when new); it may
+    not share memory with ``draft``."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 2:
         raise ArgumentError("logits must be a [rows, vocab] CUDA tensor")
     device = logits.device

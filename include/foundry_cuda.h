@@ -403,7 +403,7 @@ int fl_attn_paged_stall(const fl_paged_kv* kv, const fl_paged_batch* b, const fl
  * NaN and negative draft probabilities count as 0.  A row with everything
  * masked accepts nothing and its token is -1; so is a draft outside
  * [0, vocab) accepted never.
- * vocab is at most 2^24.
+ * vocab is at most 2^24; tokens may not overlap draft.
  * logits: [n_rows][vocab] of `type` (GGML type id 0, 1 or 30), rows
  * logits_stride elements apart; draft_probs: F32, rows probs_stride apart;
  * elements dense.  workspace: fl_verify_workspace bytes, 256-byte aligned,
