@@ -1572,6 +1572,8 @@ static int check_paged(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t n
         return fail(FL_ERR_ARG, "k_scale and v_scale must be 16-byte aligned");
     if (b->n_seqs > 0 && n_rows > 0 && (!b->seq_len || !b->row_start || (!b->page_table && b->table_cols > 0)))
         return fail(FL_ERR_ARG, "null batch pointer");
+    if (misaligned(b->page_table, 4) || misaligned(b->seq_len, 4) || misaligned(b->row_start, 4))
+        return fail(FL_ERR_ARG, "page_table, seq_len and row_start must be 4-byte aligned");
     c.kv_dtype = kv->kv_dtype;
     c.n_pages = kv->n_pages;
     c.page_shift = 0;
@@ -1671,6 +1673,7 @@ static int attn_paged(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_p
     const int64_t width = (int64_t)a->n_heads * c.hd;
     if ((rc = check_rows("q", a->q, a->q_stride, width, a->n_rows, a->type))) return rc;
     if ((rc = check_rows("out", a->out, a->out_stride, width, a->n_rows, a->type))) return rc;
+    if (misaligned(a->lse, 4)) return fail(FL_ERR_ARG, "lse must be 4-byte aligned");
     const size_t need = fl_paged_attn_workspace(c, a->n_heads);
     if (a->workspace_bytes < need || (need && !a->workspace) || misaligned(a->workspace, 256))
         return fail(FL_ERR_ARG, "workspace: %llu bytes, 256-byte aligned, are needed (fl_attn_paged_workspace)",
@@ -1773,6 +1776,9 @@ extern "C" int fl_verify_device(const fl_verify_desc* d, void* stream)
         if (misaligned(d->logits, d->type == 0 ? 4 : 2)) return fail(FL_ERR_ARG, "logits must be aligned to their type");
         if (misaligned(d->draft_probs, 4)) return fail(FL_ERR_ARG, "draft_probs must be 4-byte aligned");
     }
+    for (const void* p : {(const void*)d->row_start, (const void*)d->draft, (const void*)d->temperature, (const void*)d->u_accept,
+                          (const void*)d->u_sample, (const void*)d->tokens, (const void*)d->accepted})
+        if (misaligned(p, 4)) return fail(FL_ERR_ARG, "arrays of 32-bit elements must be 4-byte aligned");
     const size_t need = fl_verify_workspace_bytes(d->n_rows, d->n_seqs, d->vocab);
     if (d->workspace_bytes < need || (need && !d->workspace) || misaligned(d->workspace, 256))
         return fail(FL_ERR_ARG, "workspace: %llu bytes, 256-byte aligned, are needed (fl_verify_workspace)",
