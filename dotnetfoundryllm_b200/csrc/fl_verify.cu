@@ -266,8 +266,10 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const FlVerify g)
 }
 
 /* A row's maximum, first index of it and sum, by a warp from its chunks: up to
- * 128 of them are loaded at once, more a second time. */
-__device__ __forceinline__ Decision merge_row(const RowPart* __restrict__ part, int chunks, float t, const double* table)
+ * 128 of them are loaded at once, more a second time.  Not __restrict__: the first
+ * kernel writes them while this one is already running, so they are not constant
+ * for its length, as loads that this allows would take for granted. */
+__device__ __forceinline__ Decision merge_row(const RowPart* part, int chunks, float t, const double* table)
 {
     const int lane = threadIdx.x & 31;
     Decision d{0.0, -INFINITY, 0, 0, INT_MAX};
