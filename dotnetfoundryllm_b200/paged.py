@@ -93,8 +93,8 @@ class PagedBatch:
         _int32("page_table", page_table, tuple(page_table.shape), self.device)
         _int32("seq_len", seq_len, (n,), self.device)
         _int32("row_start", row_start, (n + 1,), self.device)
-        if max_rows < 0:
-            raise ArgumentError("max_rows must be >= 0")
+        if not 0 <= max_rows < 2 ** 31:
+            raise ArgumentError(f"max_rows {max_rows} is not in [0, 2^31)")
         self.page_table, self.seq_len, self.row_start = page_table, seq_len, row_start
         self.desc = N.FlPagedBatch(C.sizeof(N.FlPagedBatch), n, page_table.shape[1], max_rows, page_table.data_ptr(),
                                    seq_len.data_ptr(), row_start.data_ptr())
@@ -240,8 +240,11 @@ class PagedKvCache:
                 self._space.clear()
             need = self._space[key] = got.value
         ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        d = _ATTN.pack(_ATTN.size, rt, n_rows, n_heads, window, scale, softcap, 0, q.data_ptr(), qs, out.data_ptr(), os,
-                       lse.data_ptr() if lse is not None else 0, ws.data_ptr(), need)
+        try:
+            d = _ATTN.pack(_ATTN.size, rt, n_rows, n_heads, window, scale, softcap, 0, q.data_ptr(), qs, out.data_ptr(), os,
+                           lse.data_ptr() if lse is not None else 0, ws.data_ptr(), need)
+        except (struct.error, OverflowError) as e:
+            raise ArgumentError(f"window {window}, scale {scale} or softcap {softcap} is no number of 32 bits: {e}") from None
         _enqueue(self.device, "fl_attn_paged_device", self._attend, self._at, batch._at, d)
         return out
 

@@ -19,7 +19,8 @@ import pytest
 import torch
 
 from dotnetfoundryllm_b200 import _native as N
-from dotnetfoundryllm_b200.runtime import DeviceTimeoutError
+from dotnetfoundryllm_b200.paged import PagedBatch
+from dotnetfoundryllm_b200.runtime import ArgumentError, DeviceTimeoutError
 from test_gpu_paged import ACT, DEV, Setup
 
 pytestmark = pytest.mark.gpu
@@ -254,3 +255,15 @@ def test_lengths_that_are_far_past_the_table_or_negative(window, kv, act, hd, ro
         compare(su, q, 0.1, window, 0.0, out, lse, slice(0, rows))
     su.cache.append(su.batch, q[:, :2].contiguous(), q[:, 2:4].contiguous())
     torch.cuda.synchronize()
+
+
+def test_numbers_out_of_range_are_refused():
+    su = Setup("q8", 128, 2, 16, [20], [2])
+    q = queries(su, 4, "bf16")
+    for kw in (dict(window=2 ** 31), dict(window=-2 ** 31 - 1), dict(window=1.5), dict(scale=1e39), dict(softcap=1e300),
+               dict(scale="1"), dict(softcap=None)):
+        with pytest.raises(ArgumentError):
+            su.cache.attention(su.batch, q, **{"scale": 0.1, **kw})
+    for max_rows in (-1, 2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ArgumentError):
+            PagedBatch(su.table, su.seq_len, su.row_start, max_rows=max_rows)
