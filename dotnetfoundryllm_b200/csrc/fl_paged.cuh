@@ -5,6 +5,8 @@
 #ifndef FL_PAGED_CUH
 #define FL_PAGED_CUH
 
+#include <climits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -104,8 +106,10 @@ __device__ __forceinline__ int64_t fl_cache_row(const FlPaged& c, int s, int p, 
 }
 
 /* ── attention helpers ── */
-/* The first position that a row at position p (which may be negative) sees; window > 0, or none. */
-__device__ __forceinline__ int fl_first_seen(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
+/* The first position that a row at position p (down to -n_rows: the host bounds the window by that) sees. */
+__device__ __forceinline__ int fl_first_seen(int p, int window) { return window > 0 ? max(p + 1 - window, 0) : 0; }
+/* A sequence's length, kept where a tile from its last position on is in range; no table reaches further. */
+__device__ __forceinline__ int fl_seq_len(const FlPaged& c, int s) { return min(max(__ldg(c.seq_len + s), 0), INT_MAX - 4096); }
 __device__ __forceinline__ float fl_ex2(float x)
 {
     float y;

@@ -61,12 +61,12 @@ __device__ __forceinline__ SeqWork seq_work(const FlPaged& c, const FlPagedAttn&
 {
     SeqWork w;
     const int r0 = max(__ldg(c.row_start + s), 0), r1 = min(__ldg(c.row_start + s + 1), c.n_rows);
-    const int len = max(__ldg(c.seq_len + s), 0);
+    const int len = fl_seq_len(c, s);
     w.row0 = r0;
     w.n = max(r1 - r0, 0);
     w.first = len - w.n;
     w.len = min(len, c.cols << c.page_shift);
-    w.tile0 = min(fl_first_seen(w.first, a.window), w.len) / kTile; /* within the table, wherever the window starts */
+    w.tile0 = fl_first_seen(w.first, a.window) / kTile;
     w.tiles = max(1, (w.len + kTile - 1) / kTile - w.tile0);
     w.nrt = (w.n * a.grp + kRows - 1) / kRows;
     w.cost = kItemCost + w.tiles;

@@ -106,7 +106,7 @@ __device__ __forceinline__ SeqWork seq_work(const FlPaged& c, const FlPagedAttn&
 {
     SeqWork w;
     const int r0 = max(__ldg(c.row_start + s), 0), r1 = min(__ldg(c.row_start + s + 1), c.n_rows);
-    const int len = max(__ldg(c.seq_len + s), 0);
+    const int len = fl_seq_len(c, s);
     w.row0 = r0;
     w.n = max(r1 - r0, 0);
     w.first = len - w.n;
@@ -124,7 +124,7 @@ __device__ __forceinline__ ItemWork item_work(const FlPagedAttn& a, const SeqWor
     w.pos_min = s.first + fl_div_grp(a, w.f0);
     w.pos_max = s.first + fl_div_grp(a, w.f0 + w.rows - 1);
     const int hi = max(0, min(s.len, w.pos_max + 1));
-    w.tile0 = min(fl_first_seen(w.pos_min, a.window), s.len) / BK; /* within the table, wherever the window starts */
+    w.tile0 = fl_first_seen(w.pos_min, a.window) / BK;
     w.tiles = max(1, (hi + BK - 1) / BK - w.tile0);
     return w;
 }

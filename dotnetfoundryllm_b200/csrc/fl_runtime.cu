@@ -1683,7 +1683,9 @@ static int attn_paged(const fl_paged_kv* kv, const fl_paged_batch* b, const fl_p
     p.n_heads = a->n_heads;
     p.grp = a->n_heads / c.n_kv;
     p.grp_inv = p.grp > 1 ? ~0ull / (unsigned)p.grp + 1 : 0; /* exact: floor((2^64 - 1) / grp) + 1 >= 2^64 / grp */
-    p.window = a->window;
+    /* Down to the position -n_rows, pos - window is in range.  Formed with more instructions on the device instead it
+     * cost the tcgen05 kernel 5 %, by another allocation of registers.  No sequence is as long as what this cuts off. */
+    p.window = std::min(a->window, INT32_MAX - a->n_rows);
     p.score_unit = a->softcap > 0.0f ? a->scale / a->softcap : a->scale * 1.44269504f;
     if (!std::isfinite(p.score_unit))
         return fail(FL_ERR_ARG, "scale %g with softcap %g: their quotient is out of F32's range", a->scale, a->softcap);

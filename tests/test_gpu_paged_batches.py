@@ -267,3 +267,15 @@ def test_numbers_out_of_range_are_refused():
     for max_rows in (-1, 2 ** 31, 2 ** 32 + 5):
         with pytest.raises(ArgumentError):
             PagedBatch(su.table, su.seq_len, su.row_start, max_rows=max_rows)
+
+
+@pytest.mark.parametrize("kv,act,hd", [("q8", "bf16", 128), ("f16", "f32", 64)])
+@pytest.mark.parametrize("hint", [1, 64])
+def test_more_sequences_than_threads_of_a_block(kv, act, hd, hint):
+    """Schedules in which a thread adds up several sequences; most have a row, some none, a few a prompt."""
+    g = torch.Generator().manual_seed(hd)
+    rows = [(1, 1, 1, 0, 2, 20)[int(x)] for x in torch.randint(0, 6, (1700,), generator=g)]
+    lens = [r + int(x) for r, x in zip(rows, torch.randint(0, 60, (1700,), generator=g))]
+    su = Setup(kv, hd, 2, 16, lens, rows, seed=hint)
+    su.batch = PagedBatch(su.table, su.seq_len, su.row_start, max_rows=hint)
+    check(su, queries(su, 8, act), 1 / math.sqrt(hd), window=40)
