@@ -12,27 +12,31 @@ namespace {
  * streaming kernel passes over a sequence's keys once per 16-row tile, so its
  * time is proportional to the tiles; the tcgen05 kernel's is about the same up to
  * 128 rows, but higher for 8 bits (every element is widened into shared memory)
- * and for 32-bit rows (twice the products), which is why the border moves.
- * Measured in us, streaming / tcgen05, 8 kv heads of 4, 16 sequences of 4096 keys:
+ * and for 32-bit rows (twice the products), which is why the border moves.  It is a
+ * rule on the rows of one sequence: a batch goes to one kernel whole, by its longest
+ * chunk, and each of its single tokens then takes a row tile of its own (31 tokens
+ * beside a chunk of 512 rows, int8: 203 us, as two calls 88 + 44).
+ * Measured in us, streaming / tcgen05, 8 kv heads of 4, 16 sequences of 4096 keys
+ * (other shapes move the border by how many items share the tcgen05 kernel's start):
  *   rows               16         20         48         64
- *   f16,  F16, 64    42 /  70   65 /  70   90 /  73  113 /  74   from 3 tiles
- *   f16,  F16, 128   71 /  84  119 /  86  174 /  95  228 /  96   from 2
- *   f16,  F16, 256  161 / 130  296 / 131  442 / 137  583 / 140   from 2
- *   f16,  Q8,  64    31 /  81   49 /  81   67 /  82   85 /  83   from 4
- *   bf16, Q8,  128   47 / 110   77 / 111  110 / 116  140 / 117   from 4
- *   bf16, Q8,  256   86 / 159  144 / 159  212 / 163  275 / 165   from 3
- *   bf16, F8,  64    39 /  85   63 /  85   89 /  86  113 /  87   from 3
- *   bf16, F8,  128   72 / 117  120 / 119  172 / 124  223 / 126   from 3
- *   bf16, F8,  256  147 / 164  261 / 164  381 / 168  513 / 170   from 2
- *   f32,  F16, 64    47 / 118   73 / 118  102 / 120  129 / 121   from 4
- *   f32,  F16, 128   89 / 130  152 / 130  223 / 134  297 / 137   from 2
- *   f32,  F16, 256  256 / 264  478 / 265  715 / 273  944 / 275   from 2
- *   f32,  Q8,  64    39 / 141   62 / 141   87 / 146  111 / 144   from 6
- *   f32,  Q8,  128   61 / 164  101 / 164  145 / 167  185 / 169   from 4
- *   f32,  Q8,  256  139 / 296  252 / 296  381 / 302  499 / 305   from 3
- *   f32,  F8,  64    46 / 140   76 / 140  107 / 145  136 / 145   from 5
- *   f32,  F8,  128   89 / 172  151 / 173  218 / 176  280 / 176   from 3
- *   f32,  F8,  256  301 / 301  566 / 302  846 / 309 1117 / 311   from 2 */
+ *   f16,  F16, 64   43 /  70   66 /  71   91 /  75  115 /  77   from 3 tiles
+ *   f16,  F16, 128  71 /  87  120 /  89  175 /  99  229 / 100   from 2
+ *   f16,  F16, 256 161 / 134  296 / 134  445 / 142  586 / 144   from 2
+ *   f16,  Q8,  64   33 /  83   50 /  84   69 /  86   87 /  89   from 4
+ *   bf16, Q8,  128  48 / 118   77 / 119  111 / 128  141 / 129   from 4
+ *   bf16, Q8,  256  86 / 159  145 / 160  212 / 165  276 / 166   from 3
+ *   bf16, F8,  64   40 /  87   65 /  89   90 /  92  114 /  94   from 3
+ *   bf16, F8,  128  74 / 121  125 / 124  178 / 132  230 / 134   from 3
+ *   bf16, F8,  256 147 / 168  262 / 169  385 / 173  518 / 175   from 2
+ *   f32,  F16, 64   49 / 122   75 / 123  104 / 126  132 / 129   from 4
+ *   f32,  F16, 128  91 / 133  156 / 133  229 / 137  305 / 139   from 2
+ *   f32,  F16, 256 261 / 270  482 / 270  722 / 277  951 / 280   from 2
+ *   f32,  Q8,  64   40 / 149   64 / 150   88 / 152  112 / 154   from 6
+ *   f32,  Q8,  128  62 / 166  102 / 166  146 / 169  187 / 170   from 4
+ *   f32,  Q8,  256 142 / 300  256 / 300  386 / 307  506 / 309   from 3
+ *   f32,  F8,  64   48 / 152   77 / 152  108 / 154  138 / 157   from 5
+ *   f32,  F8,  128  90 / 171  151 / 172  220 / 175  281 / 175   from 3
+ *   f32,  F8,  256 303 / 307  567 / 307  847 / 315  1116 / 318   from 2 */
 int tc_tiles(int kv_dtype, int hd, bool wide)
 {
     static constexpr int8_t from[2][3][3] = {{{3, 2, 2}, {4, 4, 3}, {3, 3, 2}}, {{4, 2, 2}, {6, 4, 3}, {5, 3, 2}}};

@@ -14,9 +14,9 @@
  *    core.  The two are apart because the fence that hands over waits for every
  *    copy its thread has under way: with both in one thread no tile's copies
  *    overlapped another's work (2048 rows at 16384 keys, 8 bits: 828 us, apart
- *    682).  V is read by the tensor core with the keys as its inner dimension,
- *    straight from rows of 64 elements (an MN-major operand), so nothing is
- *    transposed.
+ *    682 in builds of that time).  V is read by the tensor core with the keys as
+ *    its inner dimension, straight from rows of 64 elements (an MN-major operand),
+ *    so nothing is transposed.
  *  - one lane issues S = Q K^T into tensor memory and, once the weights are
  *    there, O += P V with P read from tensor memory.
  *  - 4 warps per 128 rows hold one row a thread: S is read from tensor memory
@@ -31,12 +31,14 @@
  * weight (22 bits) at twice the products.
  *
  * Measured, causal chunk of 2048 rows x 32 heads at the end of 16384 keys, heads
- * of 128: fp16 cache 528 us (977 TFLOP/s of the 1394 that the tensor cores keep
- * up), 8 bits 682 us (756), 32-bit rows over 8 bits 2254 us.  From fp16 the
- * exponentials and their row sums bound it (8 softmax warps, one row a thread),
- * from 8 bits those and the widening through shared memory, which the softmax
- * warps share for the scales.  With softcap (two more transcendental operations
- * a score) 0.2-0.5 k rows at 5 k keys, e4m3, heads of 256: 233 us, of 128: 138.
+ * of 128: fp16 cache 534 us (965 TFLOP/s of the 1394 that the tensor cores keep
+ * up), int8 688 us (749), e4m3 767 us, 32-bit rows over int8 2268 us.  In half of
+ * that from fp16 the tensor pipe is busy 39 % of the cycles and the exponentials'
+ * 39 %: the 8 softmax warps' own chain, one row a thread (scores out of tensor
+ * memory, exponentials, weights back), bounds it; from 8 bits (31 % each) that and
+ * the widening through shared memory, which the softmax warps read the scales
+ * from.  With softcap (two more transcendental operations a score) 0.2-0.5 k rows at
+ * 5 k keys, e4m3, heads of 256: 239 us (caps above 128: 371), of 128: 137 (237).
  */
 #ifndef FL_PAGED_TC_CUH
 #define FL_PAGED_TC_CUH
@@ -403,9 +405,10 @@ struct Segments {
 /* Softcap's variants, each of its own because 128 curves at once cost the plain
  * kernel registers that it does not have to spare: kCapFolded joins the curve to
  * the weights' multiply and add, off by some 2^-22 of the cap, which up to kFoldMax
- * is at most 2^-15 of a weight, a sixteenth of the rounding of one to fp16 (chunk
- * with heads of 256: 233 us, with the curve by itself 266); kCapCurve, for larger
- * caps and for 32-bit rows, is off by some 2^-21 of the score. */
+ * is at most 2^-15 of a weight, a sixteenth of the rounding of one to fp16;
+ * kCapCurve, for larger caps and for 32-bit rows, is off by some 2^-21 of the score
+ * (three chunks of 0.2-0.5 k rows, e4m3, heads of 256: 239 and 371 us, of 128: 137
+ * and 237). */
 constexpr int kNoCap = 0, kCapFolded = 1, kCapCurve = 2;
 constexpr float kFoldMax = 128.0f;
 template <typename T, int KV, int HD, int CAP>

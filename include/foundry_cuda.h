@@ -342,7 +342,12 @@ int fl_kv_gather_device(const fl_paged_kv* kv, const fl_paged_batch* b, int32_t 
  * A row that sees nothing gets out = 0, lse = -infinity.  What a row does not
  * see (NaN and infinities in masked places included) does not touch it.
  * Scores, the softmax's maximum and sum, and the output are accumulated in
- * F32.  Results are the same each time for the same inputs; how a sequence's
+ * F32.  For the products with V a weight, times its value's scale in the 8-bit
+ * formats, is rounded to fp16 for F16 and BF16 rows, and kept in 22 bits for F32
+ * ones; both no finer than 2^-31 of the largest weight (and of the largest
+ * scale that rows handled together see).  With a softcap up to 128 and many F16
+ * or BF16 rows the capped score is off by 2^-22 of the cap.
+ * Results are the same each time for the same inputs; how a sequence's
  * keys are split among the SMs, and with it the last bits of its rows, depends
  * on the lengths in the batch.
  * q, out: [n_rows][n_heads][head_dim] of `type`, rows q_stride / out_stride
@@ -392,7 +397,8 @@ int fl_attn_paged_stall(const fl_paged_kv* kv, const fl_paged_batch* b, const fl
  * u_accept[row] * q(draft) < p(draft).  At the first row that is not, the
  * token is drawn from max(p - q, 0) (from p if that is 0 everywhere); with all
  * accepted, from p of the last row.  The draw is the first x whose cumulative
- * weight exceeds u_sample[b] times the total; sums are in 64 bits.
+ * weight exceeds u_sample[b] times the total; sums are in 64 bits.  For the
+ * acceptance tests p's exponentials are in F32, 2^-20 relative.
  * temperature[b] <= 0 (or NaN) is greedy: accepted iff draft is the argmax
  * (first maximum), the token is the argmax.  Infinity counts as the largest
  * F32.
