@@ -15,7 +15,7 @@ there.
 
 All calls are enqueued on the current stream of the tensors' device, allocate
 only their outputs and a workspace (from torch's allocator, so captured graphs
-hold their own), and do not synchronize.  Argument errors raise
+hold their own), and, but for ``synchronize``, do not synchronize.  Argument errors raise
 ``ArgumentError`` / ``NotSupportedError`` before anything is enqueued.
 """
 from __future__ import annotations
